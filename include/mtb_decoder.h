@@ -31,6 +31,8 @@
  *   mtb_snapshot_save / _restore         (src/cpu_speculative.cpp:100-137)
  *   mtb_audio_load / _encode / _free     AudioEncoder (src/audio_encoder.cpp:16-75): WhisperMel,
  *                                        WhisperEncoder, AudioAdaptor on the device
+ *   mtb_rope_append, mtb_paged_attention, mtb_attention_weights, mtb_cache_evict,
+ *   mtb_logits_process                   operators on a caller's own device memory
  *
  * Conventions: every function returns 0 on success or a negative code and
  * sets a per-object error string; no C++ exception crosses the boundary.  One
@@ -41,6 +43,7 @@
 #ifndef MTB_DECODER_H
 #define MTB_DECODER_H
 
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -300,6 +303,155 @@ float mtb_audio_last_ms(const mtb_audio* a);
  * final LayerNorm, before the trim); n_samples <= samples per chunk (the rest
  * is zero-padded as in encode); either output may be NULL. */
 int mtb_audio_debug_chunk(mtb_audio* a, const float* samples, int n_samples, float* mel_out, float* enc_out);
+
+/* ---- Operators on a caller's own device memory ----
+ * For programs that keep their own projections, cache pool or logits and want
+ * this library's kernels for what lies between: rotary positions with the
+ * append to a paged cache, attention over it, eviction from it, and the logits
+ * that steer the next token.  No counterpart in the reference (its cache is
+ * one contiguous tensor per layer, its logits leave the device).
+ *
+ * Conventions, beside those above.  Every pointer is DEVICE memory unless it
+ * says host; nothing is allocated, no host copy is made and no call waits for
+ * the device.  `stream` is a cudaStream_t (NULL: the default stream); a call
+ * is asynchronous on it, may be captured into a graph, runs on the device that
+ * owns the memory and leaves the caller's current device as it found it.
+ * 0 on success; -1 for a CUDA error or a null or non-device pointer, -2 for
+ * an argument outside its limits, with mtb_global_error() set and nothing
+ * launched.  Sizes that live on the device (lengths, page-table entries) are
+ * checked by the kernels: a violated check sets its bit in *status (never
+ * cleared by the library) and the access is skipped, never made. */
+enum { MTB_T_F32 = 0, MTB_T_F16 = 1, MTB_T_BF16 = 2 };
+enum {
+    MTB_BAD_PAGE = 1,   /* a page-table entry outside [0, n_pages): its positions count as masked, are not written,
+                           and a sequence that has one is not evicted from */
+    MTB_BAD_LEN = 2,    /* kv_len outside [0, 64 table_stride] (clamped to it), or smaller than the new tokens */
+    MTB_BAD_TOKENS = 4  /* cu_tokens not ascending inside [0, n_tokens]: the sequence counts as one without tokens */
+};
+
+/* A view of one layer's paged cache in the caller's pool: 64 positions per
+ * page, position `slot` of a sequence in page page_table[seq][slot / 64], row
+ * slot % 64.  Dim d of KV head h is at k[page * page_stride + h * head_stride
+ * + row * head_dim + d] (strides in elements, the same for v), so a view of
+ * one layer of [page][layer][K/V][kv_head][64][head_dim] needs no copy.  k and
+ * v are 16-byte aligned and the strides multiples of 8 elements.  position and
+ * weight are the book-keeping of eviction, one value per cached position and
+ * KV head, [page][kv_head][64] without gaps; NULL where not wanted.  Sequences
+ * may share pages that a call only reads. */
+typedef struct mtb_paged_cache {
+    void* k;
+    void* v;
+    int32_t type;             /* MTB_T_F16 or MTB_T_BF16 */
+    int32_t head_dim;         /* 64 or 128 */
+    int32_t n_kv_heads;
+    int32_t n_pages;          /* pages in the pool */
+    int64_t page_stride, head_stride;
+    const int32_t* page_table; /* [n_seq][table_stride] */
+    int32_t table_stride;
+    int32_t n_seq;
+    const int32_t* kv_len;    /* [n_seq] positions held, the call's new tokens included */
+    int32_t* position;        /* or NULL */
+    float* weight;            /* or NULL */
+    int32_t* status;          /* one word of MTB_BAD_* bits, or NULL */
+} mtb_paged_cache;
+
+/* Scaling of rotary frequencies for contexts beyond the trained length.
+ * LINEAR: all frequencies / factor.  NTK: base * factor^(R / (R - 2)).  YARN:
+ * pairs that turn more than `fast` times over original_len keep their frequency,
+ * those below `slow` turns are divided, a ramp over the pair index between, and
+ * cos and sin are scaled by 0.1 ln(factor) + 1.  BANDS: the same blend with the
+ * ramp over the number of turns, unscaled. */
+enum { MTB_ROPE_PLAIN = 0, MTB_ROPE_LINEAR = 1, MTB_ROPE_NTK = 2, MTB_ROPE_YARN = 3, MTB_ROPE_BANDS = 4 };
+/* inv_freq [rotary_dim / 2] and *factor (both HOST memory) for
+ * mtb_rope_append; computed once by the caller, needs no GPU. */
+int mtb_rope_frequencies(int rotary_dim, double base, int kind, double factor, double original_len, double fast,
+                         double slow, double* inv_freq, float* out_factor);
+/* Rotary positions of q and k, and the append of k and v to the cache, in one
+ * pass.  Tokens cu_tokens[s] .. cu_tokens[s + 1] - 1 (cu_tokens [n_seq + 1])
+ * are the newest of sequence s: token i of n goes to slot kv_len[s] - n + i.
+ * q [n_tokens][n_heads][head_dim], k and v [n_tokens][n_kv_heads][head_dim], rows
+ * of a token contiguous, tokens `stride` elements apart, all of `in_type`;
+ * q_out has the cache's type (it may be q itself when in_type is that type and
+ * the strides are equal).  The first rotary_dim dims are rotated by
+ * positions[token] * inv_freq[pair] (64-bit, reduced before the sine), pairs
+ * (j, j + rotary_dim / 2) or, interleaved, (2j, 2j + 1); cos and sin times
+ * factor; the others pass.  Each result is rounded once.  Where the cache has
+ * them, position gets the token's position and weight 0.  Rows behind the last
+ * sequence are left as they are. */
+int mtb_rope_append(const mtb_paged_cache* cache, const int32_t* cu_tokens, int n_tokens, const int32_t* positions,
+                    int in_type, const void* q, int64_t q_stride, int n_heads, const void* k, int64_t k_stride,
+                    const void* v, int64_t v_stride, const double* inv_freq, int rotary_dim, int interleaved,
+                    float factor, void* q_out, int64_t q_out_stride, void* stream);
+
+/* Device bytes of mtb_paged_attention's workspace (any sizes).  Zeroed once
+ * before its first use; every call leaves it ready for the next.  Calls (and
+ * replays of captured graphs) that share one must not overlap. */
+enum { MTB_ATTENTION_WORKSPACE = 64 << 20 };
+/* Attention of the new tokens over the paged cache, causal: token i of a
+ * sequence's n sees the slots <= kv_len - n + i, so its own (appended before).
+ * q and out [n_tokens][n_heads][head_dim] of the cache's type (16-byte aligned,
+ * strides multiples of 8 elements); n_heads a multiple of n_kv_heads, at most
+ * 64 for each; head h reads KV head h / (n_heads / n_kv_heads).  scale times q.k
+ * (64-bit host value of the softmax's scale, 1 / sqrt(head_dim) usually).
+ * lse [n_tokens][n_heads] f32 (or NULL) gets log sum exp of the row's scores.
+ * A row that sees nothing gets out 0 and lse -inf; rows behind the last
+ * sequence are left as they are.  Slots a row does not see may hold anything
+ * in K; in V, slots at or behind kv_len may too, and a new token's V must be finite
+ * where earlier tokens of the same call matter.  max_tokens: the most new tokens
+ * of one sequence, if known (it only picks the kernel; <= 0: n_tokens). */
+int mtb_paged_attention(const mtb_paged_cache* cache, const int32_t* cu_tokens, int n_tokens, int max_tokens,
+                        const void* q, int64_t q_stride, int n_heads, float scale, void* out, int64_t out_stride,
+                        float* lse, void* workspace, size_t workspace_bytes, void* stream);
+/* The softmax weight each cached position received in that attention:
+ * cache->weight[slot] = decay * cache->weight[slot] + sum of exp(score - lse) over the
+ * new tokens that see the slot and the query heads of its KV head (decay 0
+ * ignores the old value).  Slots at or behind kv_len are left as they are;
+ * sequences without new tokens too.  Arguments as above. */
+int mtb_attention_weights(const mtb_paged_cache* cache, const int32_t* cu_tokens, int n_tokens, int max_tokens,
+                          const void* q, int64_t q_stride, int n_heads, float scale, const float* lse, float decay,
+                          void* stream);
+
+/* Device bytes of mtb_cache_evict's workspace (needs no GPU). */
+int64_t mtb_cache_evict_workspace(int n_seq, int n_kv_heads, int table_stride);
+/* Eviction by accumulated weight, in place, each KV head on its own: of a
+ * sequence with kv_len > keep the `keep` slots stay that rank highest, others go.
+ * Rank: first slots whose position is < sinks or among the `recent` highest
+ * (> newest - recent), then larger weight (NaN below all), then lower slot.
+ * Kept slots below `keep` stay where they are; the kept ones at or above it move
+ * into the gaps, both in ascending order (K, V, position and weight), so the cache
+ * is then slots [0, keep) in no particular order of positions: attention of later
+ * tokens does not depend on it, since rotary positions are in K.
+ * new_len[s] = min(kv_len, keep); it may be kv_len itself.  Needs position
+ * and weight, sinks + recent <= keep, pages that no other sequence shares. */
+int mtb_cache_evict(const mtb_paged_cache* cache, int keep, int sinks, int recent, int32_t* new_len, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* What mtb_logits_process applies; any pointer may be NULL (left out). */
+typedef struct mtb_logits_params {
+    const int32_t* history;     /* [history_len] ids; row r's are [history_begin[r], history_end[r]) (ranges may overlap) */
+    int64_t history_len;        /* the kernels cut ranges to it */
+    const int32_t *history_begin, *history_end; /* [rows] */
+    const float *repetition, *presence, *frequency; /* [rows] */
+    const int32_t* bias_ids;    /* [bias_len]; row r's entries are [bias_begin[r], bias_end[r]) */
+    const float* bias_values;   /* [bias_len] */
+    int64_t bias_len;
+    const int32_t *bias_begin, *bias_end; /* [rows] */
+    const uint32_t* mask;       /* bit i % 32 of word i / 32 of a mask row: id i is allowed */
+    int64_t mask_stride;        /* words between mask rows */
+    int32_t mask_rows;
+    const int32_t* mask_row;    /* [rows] the mask row of each logits row, NULL: its own index; a row outside
+                                   [0, mask_rows) is not masked */
+} mtb_logits_params;
+/* logits [rows][vocab] of `type`, rows `stride` elements apart; out the same type
+ * (it may be logits itself, or NULL), choice [rows] (or NULL).  For an id that
+ * occurs c > 0 times in its row's history: x > 0 ? x / repetition : x * repetition,
+ * then - frequency * c, then - presence (src/cpu_speculative.cpp:39-50 has the first);
+ * then + the bias of the id's last entry; then -inf where the mask forbids it.
+ * Evaluated in f32 in this order, each step rounded; out is rounded once more.
+ * choice: the lowest id of the largest f32 value; NaN never wins; -1 when no
+ * value is above -inf.  Ids outside [0, vocab) in history or biases are skipped. */
+int mtb_logits_process(const void* logits, int type, int rows, int vocab, int64_t stride,
+                       const mtb_logits_params* params, void* out, int64_t out_stride, int32_t* choice, void* stream);
 
 #ifdef __cplusplus
 }

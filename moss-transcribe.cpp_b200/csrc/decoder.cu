@@ -791,6 +791,9 @@ int mtb_bounds_check_status(int device) {
 void mtb_debug_fail_alloc(int n) { g_fail_alloc.store(n > 0 ? n : 0); }
 const char* mtb_global_error(void) { return g_error.c_str(); }
 
+// For the entries without an object in other files (ops_api.cu).
+__attribute__((visibility("hidden"))) void mtb_set_global_error(const char* text) { g_error = text; }
+
 int mtb_model_load(const char* path, int device, mtb_model** out) {
     if (!out || !path) { g_error = "null argument"; return -1; }
     *out = nullptr;

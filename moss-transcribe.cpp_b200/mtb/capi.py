@@ -9,11 +9,17 @@ tests read like the reference's own:
   - cpu_ngram_draft / cpu_greedy_choice -> src/cpu_speculative.cpp:27,39
 Every call goes to the CUDA library; there is no Python or CPU fallback, and
 loading fails loudly when the library or a GPU is missing.
+
+The operators on a caller's own device memory (PagedCache, rope_append,
+paged_attention, attention_weights, cache_evict, logits_process) take torch
+tensors on the GPU, or anything with the same data_ptr / shape / stride / dtype /
+device.
 """
 from __future__ import annotations
 
 import ctypes as C
 import os
+import sys
 
 import numpy as np
 
@@ -42,6 +48,27 @@ class Counters(C.Structure):
 
 DRAFT_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.POINTER(C.c_int32), C.c_int, C.c_int, C.POINTER(C.c_int32))
 COMMIT_FN = C.CFUNCTYPE(None, C.c_void_p, C.POINTER(C.c_int32), C.c_int, C.c_int, C.c_int)
+
+T_F32, T_F16, T_BF16 = 0, 1, 2
+BAD_PAGE, BAD_LEN, BAD_TOKENS = 1, 2, 4
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN, ROPE_BANDS = range(5)
+ATTENTION_WORKSPACE = 64 << 20
+PAGE = 64
+
+
+class PagedCacheView(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int32), ("head_dim", C.c_int32),
+                ("n_kv_heads", C.c_int32), ("n_pages", C.c_int32), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("page_table", C.c_void_p), ("table_stride", C.c_int32), ("n_seq", C.c_int32), ("kv_len", C.c_void_p),
+                ("position", C.c_void_p), ("weight", C.c_void_p), ("status", C.c_void_p)]
+
+
+class LogitsParams(C.Structure):
+    _fields_ = [("history", C.c_void_p), ("history_len", C.c_int64), ("history_begin", C.c_void_p), ("history_end", C.c_void_p),
+                ("repetition", C.c_void_p), ("presence", C.c_void_p), ("frequency", C.c_void_p), ("bias_ids", C.c_void_p),
+                ("bias_values", C.c_void_p), ("bias_len", C.c_int64), ("bias_begin", C.c_void_p), ("bias_end", C.c_void_p), ("mask", C.c_void_p),
+                ("mask_stride", C.c_int64), ("mask_rows", C.c_int32), ("mask_row", C.c_void_p)]
+
 
 # Every exported function with (restype, argtypes); used for binding and for
 # the export check of the boundary test.
@@ -116,6 +143,17 @@ SIGNATURES = {
     "mtb_audio_encode": (C.c_int, [_vp, _f32p, C.c_int, _f32p, C.c_int, _ip]),
     "mtb_audio_last_ms": (C.c_float, [_vp]),
     "mtb_audio_debug_chunk": (C.c_int, [_vp, _f32p, C.c_int, _f32p, _f32p]),
+    "mtb_rope_frequencies": (C.c_int, [C.c_int, C.c_double, C.c_int, C.c_double, C.c_double, C.c_double, C.c_double,
+                                       C.POINTER(C.c_double), _f32p]),
+    "mtb_rope_append": (C.c_int, [_vp, _vp, C.c_int, _vp, C.c_int, _vp, C.c_int64, C.c_int, _vp, C.c_int64, _vp,
+                                  C.c_int64, _vp, C.c_int, C.c_int, C.c_float, _vp, C.c_int64, _vp]),
+    "mtb_paged_attention": (C.c_int, [_vp, _vp, C.c_int, C.c_int, _vp, C.c_int64, C.c_int, C.c_float, _vp, C.c_int64,
+                                      _vp, _vp, C.c_size_t, _vp]),
+    "mtb_attention_weights": (C.c_int, [_vp, _vp, C.c_int, C.c_int, _vp, C.c_int64, C.c_int, C.c_float, _vp, C.c_float,
+                                        _vp]),
+    "mtb_cache_evict_workspace": (C.c_int64, [C.c_int, C.c_int, C.c_int]),
+    "mtb_cache_evict": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_size_t, _vp]),
+    "mtb_logits_process": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int64, _vp, _vp, C.c_int64, _vp, _vp]),
 }
 
 
@@ -521,3 +559,190 @@ def spec_run_group(decoders, max_steps: int = 0) -> int:
     if lib().mtb_spec_run_group(_group(decoders), len(decoders), int(max_steps), C.byref(n)) != 0:
         raise _group_error(decoders, "spec_run_group")
     return n.value
+
+
+# ---- operators on a caller's own device memory -----------------------------
+
+_TYPE_CODES = {}  # dtype object -> (name, element size), filled as dtypes are met
+_CODES = {"float32": T_F32, "float16": T_F16, "bfloat16": T_BF16}
+
+
+def _dtype(t):
+    name = _TYPE_CODES.get(t.dtype)
+    if name is None:
+        name = _TYPE_CODES[t.dtype] = str(t.dtype).rsplit(".", 1)[-1]
+    return name
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _need(ok, what):
+    if not ok:
+        raise MtbError(what)
+
+
+def _flat(t, name, dtype, n=None, device=None):
+    """The pointer of a tensor without gaps, 0 for None; n: the least number of its elements."""
+    if t is None:
+        return 0
+    if _dtype(t) != dtype or not t.is_contiguous() or (n is not None and t.numel() < n) or (device is not None and t.device != device):
+        raise MtbError(f"{name} must be contiguous {dtype}" + (f" with at least {n} elements" if n is not None else "")
+                       + (f" on {device}" if device is not None else ""))
+    return t.data_ptr()
+
+
+def _rows(t, name, heads, dim, device):
+    """(pointer, elements between tokens) of [tokens][heads][dim] whose tokens' rows have no gaps."""
+    sh, st = t.shape, t.stride()
+    if (len(sh) != 3 or (heads is not None and sh[1] != heads) or sh[2] != dim or st[2] != 1 or (sh[1] > 1 and st[1] != dim)
+            or t.device != device):
+        raise MtbError(f"{name} must be [tokens][{'heads' if heads is None else heads}][{dim}] on {device} with a token's rows "
+                       "contiguous")
+    return t.data_ptr(), (st[0] if sh[0] > 1 else max(st[0], sh[1] * dim))
+
+
+def _space(t, device):
+    """(pointer, bytes) of a workspace."""
+    if not t.is_contiguous() or t.device != device:
+        raise MtbError(f"workspace must be contiguous, on {device}")
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
+def _stream(t, stream):
+    """A cudaStream_t: the one given, else torch's current stream of the tensor's device."""
+    if stream is not None:
+        return stream if isinstance(stream, int) else stream.cuda_stream
+    torch = sys.modules.get("torch")
+    return torch._C._cuda_getCurrentRawStream(t.device.index) if torch is not None and t.device.type == "cuda" else 0
+
+
+def _ok(rc, what):
+    if rc != 0:
+        raise MtbError(f"{what}: {lib().mtb_global_error().decode()}")
+
+
+class PagedCache:
+    """A view of one layer's paged cache (mtb_paged_cache): k and v [pages][kv_heads][64][head_dim] with equal strides
+    (their pages and heads may be apart, as in one layer of a larger pool), page_table [sequences][pages of one], kv_len
+    [sequences] with the new tokens included; position (int32) and weight (f32) [pages][kv_heads][64] and status (int32,
+    BAD_* bits) where wanted.  It keeps the tensors alive and may be used for any number of calls."""
+
+    def __init__(self, k, v, page_table, kv_len, position=None, weight=None, status=None):
+        sh, st, name = k.shape, k.stride(), _dtype(k)
+        _need(len(sh) == 4 and sh[2] == PAGE and st[3] == 1 and st[2] == sh[3],
+              "k must be [pages][kv_heads][64][head_dim] with a page's rows contiguous")
+        _need(tuple(v.shape) == tuple(sh) and _dtype(v) == name and v.stride() == st, "v must have k's shape, strides and type")
+        _need(name in ("float16", "bfloat16"), "the cache's type is float16 or bfloat16")
+        _need(len(page_table.shape) == 2 and _dtype(page_table) == "int32" and page_table.is_contiguous() and page_table.device == k.device,
+              "page_table must be contiguous int32 [sequences][pages] on the cache's device")
+        n_seq, meta, dev = page_table.shape[0], sh[0] * sh[1] * PAGE, k.device
+        block = PAGE * sh[3]
+        self.kept = (k, v, page_table, kv_len, position, weight, status)
+        self.heads, self.dim, self.type, self.n_seq, self.device = sh[1], sh[3], name, n_seq, dev
+        self.view = PagedCacheView(
+            k.data_ptr(), v.data_ptr(), _CODES[name], sh[3], sh[1], sh[0], st[0] if sh[0] > 1 else max(st[0], sh[1] * block),
+            st[1] if sh[1] > 1 else max(st[1], block), page_table.data_ptr(), page_table.shape[1], n_seq,
+            _flat(kv_len, "kv_len", "int32", n_seq, dev), _flat(position, "position", "int32", meta, dev),
+            _flat(weight, "weight", "float32", meta, dev), _flat(status, "status", "int32", 1, dev))
+        self.ref = C.byref(self.view)
+
+
+def rope_frequencies(rotary_dim: int, base: float, kind: int = ROPE_PLAIN, factor: float = 1.0, original_len: float = 0.0,
+                     fast: float = 32.0, slow: float = 1.0):
+    """(inverse frequencies float64 [rotary_dim / 2], scale of cos and sin) for rope_append; needs no GPU."""
+    out = np.zeros(max(rotary_dim // 2, 0), dtype=np.float64)
+    scale = C.c_float()
+    _ok(lib().mtb_rope_frequencies(int(rotary_dim), float(base), int(kind), float(factor), float(original_len), float(fast),
+                                   float(slow), out.ctypes.data_as(C.POINTER(C.c_double)), C.byref(scale)), "rope_frequencies")
+    return out, scale.value
+
+
+def rope_append(cache: PagedCache, cu_tokens, positions, q, k, v, inv_freq, q_out, interleaved: bool = False,
+                factor: float = 1.0, stream=None):
+    """Rotary positions of q and k and the append of k and v to the cache (mtb_rope_append).  q [tokens][heads][dim], k and v
+    [tokens][kv_heads][dim] (views of a fused projection's rows will do), inv_freq float64 [rotary / 2], q_out of the
+    cache's type.  Token i of a sequence's n goes to slot kv_len - n + i."""
+    n, heads = q.shape[0], q.shape[1]
+    qp, qs = _rows(q, "q", None, cache.dim, cache.device)
+    kp, ks = _rows(k, "k", cache.heads, cache.dim, cache.device)
+    vp, vs = _rows(v, "v", cache.heads, cache.dim, cache.device)
+    op, os_ = _rows(q_out, "q_out", heads, cache.dim, cache.device)
+    name = _dtype(q)
+    _need(k.shape[0] == n and v.shape[0] == n and q_out.shape[0] == n and _dtype(k) == name and _dtype(v) == name
+          and _dtype(q_out) == cache.type and name in _CODES, "q, k, v and q_out must agree in tokens and types")
+    _ok(lib().mtb_rope_append(cache.ref, _flat(cu_tokens, "cu_tokens", "int32", cache.n_seq + 1, cache.device), n,
+                              _flat(positions, "positions", "int32", n, cache.device), _CODES[name], qp, qs, heads, kp, ks, vp, vs,
+                              _flat(inv_freq, "inv_freq", "float64", None, cache.device), 2 * inv_freq.numel(), int(interleaved), factor, op, os_,
+                              _stream(q, stream)), "rope_append")
+
+
+def paged_attention(cache: PagedCache, cu_tokens, q, out, workspace, lse=None, scale: float | None = None, max_tokens: int = 0,
+                    stream=None):
+    """Causal attention of the new tokens over the cache (mtb_paged_attention).  q and out [tokens][heads][dim] of the
+    cache's type, lse f32 [tokens][heads]; workspace: ATTENTION_WORKSPACE bytes, zeroed once before its first use and not
+    shared by calls that overlap."""
+    n, heads = q.shape[0], q.shape[1]
+    qp, qs = _rows(q, "q", None, cache.dim, cache.device)
+    op, os_ = _rows(out, "out", heads, cache.dim, cache.device)
+    _need(out.shape[0] == n and _dtype(q) == cache.type and _dtype(out) == cache.type, "q and out must agree, in the cache's type")
+    _ok(lib().mtb_paged_attention(cache.ref, _flat(cu_tokens, "cu_tokens", "int32", cache.n_seq + 1, cache.device), n, max_tokens, qp, qs, heads,
+                                  cache.dim ** -0.5 if scale is None else scale, op, os_, _flat(lse, "lse", "float32", n * heads, cache.device),
+                                  *_space(workspace, cache.device), _stream(q, stream)), "paged_attention")
+
+
+def attention_weights(cache: PagedCache, cu_tokens, q, lse, decay: float = 1.0, scale: float | None = None, max_tokens: int = 0,
+                      stream=None):
+    """cache weight = decay * weight + the softmax weight each position received in that attention (mtb_attention_weights)."""
+    n, heads = q.shape[0], q.shape[1]
+    qp, qs = _rows(q, "q", None, cache.dim, cache.device)
+    _need(_dtype(q) == cache.type, "q must have the cache's type")
+    _ok(lib().mtb_attention_weights(cache.ref, _flat(cu_tokens, "cu_tokens", "int32", cache.n_seq + 1, cache.device), n, max_tokens, qp, qs, heads,
+                                    cache.dim ** -0.5 if scale is None else scale, _flat(lse, "lse", "float32", n * heads, cache.device), decay,
+                                    _stream(q, stream)), "attention_weights")
+
+
+def cache_evict_workspace(n_seq: int, n_kv_heads: int, table_stride: int) -> int:
+    """Device bytes of cache_evict's workspace; needs no GPU."""
+    return lib().mtb_cache_evict_workspace(int(n_seq), int(n_kv_heads), int(table_stride))
+
+
+def cache_evict(cache: PagedCache, keep: int, new_len, workspace, sinks: int = 0, recent: int = 0, stream=None):
+    """Keep the `keep` slots of each longer sequence that rank highest, in place (mtb_cache_evict); new_len int32 [sequences]
+    gets the lengths (it may be kv_len itself)."""
+    _ok(lib().mtb_cache_evict(cache.ref, keep, sinks, recent, _flat(new_len, "new_len", "int32", cache.n_seq, cache.device), *_space(workspace, cache.device),
+                              _stream(new_len, stream)), "cache_evict")
+
+
+def logits_process(logits, out=None, choice=None, history=None, hist_begin=None, hist_end=None, repetition=None, presence=None,
+                   frequency=None, bias_ids=None, bias_values=None, bias_begin=None, bias_end=None, mask=None, mask_row=None,
+                   stream=None):
+    """Penalties, biases and masks on logits [rows][vocab], and the greedy choice (mtb_logits_process).  Row r's history is
+    history[hist_begin[r]:hist_end[r]], its biases likewise; mask int32 or uint32 [mask rows][words], bit i % 32 of word i / 32."""
+    _need(len(logits.shape) == 2 and _dtype(logits) in _CODES, "logits must be [rows][vocab] of float32, float16 or bfloat16")
+    rows, vocab = logits.shape
+    st = logits.stride()
+    _need(st[1] == 1 or vocab == 1, "a logits row must be contiguous")
+    os_ = 0
+    if out is not None:
+        _need(tuple(out.shape) == (rows, vocab) and out.dtype == logits.dtype and out.device == logits.device and (out.stride()[1] == 1 or vocab == 1),
+              "out must have the shape, type and device of logits")
+        os_ = out.stride()[0] if rows > 1 else max(out.stride()[0], vocab)
+    dev = logits.device
+    if mask is not None:
+        _need(len(mask.shape) == 2 and _dtype(mask) in ("int32", "uint32") and mask.stride()[1] == 1 and mask.device == dev
+              and mask.shape[1] * 32 >= vocab and (mask_row is not None or mask.shape[0] >= rows),
+              "mask must be int32 [mask rows][vocab / 32 words], with a row for each logits row or mask_row given")
+    n_bias = 0 if bias_ids is None else bias_ids.numel()
+    p = LogitsParams(_flat(history, "history", "int32", None, dev), 0 if history is None else history.numel(),
+                     _flat(hist_begin, "hist_begin", "int32", rows, dev),
+                     _flat(hist_end, "hist_end", "int32", rows, dev), _flat(repetition, "repetition", "float32", rows, dev),
+                     _flat(presence, "presence", "float32", rows, dev), _flat(frequency, "frequency", "float32", rows, dev),
+                     _flat(bias_ids, "bias_ids", "int32", None, dev), _flat(bias_values, "bias_values", "float32", n_bias, dev), n_bias,
+                     _flat(bias_begin, "bias_begin", "int32", rows, dev), _flat(bias_end, "bias_end", "int32", rows, dev), _ptr(mask),
+                     0 if mask is None else max(mask.stride()[0], mask.shape[1]), 0 if mask is None else mask.shape[0],
+                     _flat(mask_row, "mask_row", "int32", rows, dev))
+    _ok(lib().mtb_logits_process(logits.data_ptr(), _CODES[_dtype(logits)], rows, vocab, st[0] if rows > 1 else max(st[0], vocab),
+                                 C.byref(p), _ptr(out), os_, _flat(choice, "choice", "int32", rows, dev), _stream(logits, stream)),
+        "logits_process")
