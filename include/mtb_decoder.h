@@ -326,7 +326,9 @@ enum {
     MTB_BAD_PAGE = 1,   /* a page-table entry outside [0, n_pages): its positions count as masked, are not written,
                            and a sequence that has one is not evicted from */
     MTB_BAD_LEN = 2,    /* kv_len outside [0, 64 table_stride] (clamped to it), or smaller than the new tokens */
-    MTB_BAD_TOKENS = 4  /* cu_tokens not ascending inside [0, n_tokens]: the sequence counts as one without tokens */
+    MTB_BAD_TOKENS = 4, /* cu_tokens not ascending inside [0, n_tokens]: the sequence counts as one without tokens */
+    MTB_BAD_WAIT = 8    /* a kernel's wait for its own copies ran out (seconds): that call's results are void, its
+                           workspace must be zeroed again */
 };
 
 /* A view of one layer's paged cache in the caller's pool: 64 positions per

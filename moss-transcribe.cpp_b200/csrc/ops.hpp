@@ -7,7 +7,7 @@
 namespace mtb {
 
 enum OpType : int { OP_F32 = 0, OP_F16 = 1, OP_BF16 = 2 };
-enum OpStatus : int { BAD_PAGE = 1, BAD_LEN = 2, BAD_TOKENS = 4 };
+enum OpStatus : int { BAD_PAGE = 1, BAD_LEN = 2, BAD_TOKENS = 4, BAD_WAIT = 8 };
 
 constexpr int kMaxGroup = 64;  // query heads per KV head
 

@@ -15,7 +15,8 @@ extern "C" __attribute__((visibility("hidden"))) void mtb_set_global_error(const
 namespace {
 
 static_assert(int(MTB_T_F32) == OP_F32 && int(MTB_T_F16) == OP_F16 && int(MTB_T_BF16) == OP_BF16, "one set of type codes");
-static_assert(int(MTB_BAD_PAGE) == BAD_PAGE && int(MTB_BAD_LEN) == BAD_LEN && int(MTB_BAD_TOKENS) == BAD_TOKENS, "one set of bits");
+static_assert(int(MTB_BAD_PAGE) == BAD_PAGE && int(MTB_BAD_LEN) == BAD_LEN && int(MTB_BAD_TOKENS) == BAD_TOKENS && int(MTB_BAD_WAIT) == BAD_WAIT,
+              "one set of bits");
 static_assert((long long)MTB_ATTENTION_WORKSPACE == kAttnWorkspace, "the header's size is the kernels'");
 
 int fail(int code, const std::string& text) {
@@ -100,6 +101,8 @@ int attention_args(const char* what, const mtb_paged_cache* cache, const int32_t
     if (const int rc = view_of(what, cache, &a->c)) return rc;
     if (n_tokens < 0) return fail(-2, w + ": n_tokens must not be negative");
     if (const int rc = heads_of(w, n_heads, cache->n_kv_heads)) return rc;
+    // Rows and their tiles are counted in int32.
+    if (int64_t(n_tokens) * (n_heads / cache->n_kv_heads) > (1 << 30)) return fail(-2, w + ": n_tokens * n_heads / n_kv_heads must be at most 2^30");
     if (n_tokens == 0 || cache->n_seq == 0) return 0;
     if (!cu || !q) return fail(-1, w + ": null pointer");
     if (!aligned(q, 16) || q_stride % 8 || q_stride < int64_t(n_heads) * cache->head_dim || q_stride >= (1ll << 38))

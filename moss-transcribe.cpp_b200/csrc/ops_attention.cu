@@ -1,73 +1,467 @@
 // mtb_paged_attention and mtb_attention_weights.
 //
-// One CTA per (token, head), the cache in chunks of 128 slots: a thread forms
-// one slot's score, the chunk's maximum and sum rescale the running ones
-// (softmax in one pass), then a thread owns one dim of the row and adds the chunk's V.
-#include "ops_common.cuh"
+// o = sum_j exp(s_j - lse) v_j with s = scale q.k, one pass over the cache: a
+// running maximum m and sum l of exp2(s log2 e - m), the sums of p v rescaled when m
+// has grown by more than 8 (p then stays below 2^8, which 16 bits hold as exactly as
+// values below 1; l and the sums are f32).  p is rounded to the cache's type for
+// the product with v, as the tensor cores want it; l adds it unrounded.
+#include "ops_attention.cuh"
 
 #include <algorithm>
+#include <climits>
 
 namespace mtb {
 namespace {
 
 using namespace ops;
 
-constexpr int kSimpleThreads = 128;
+constexpr int kRowsMinUnits = 2;  // pages of a CTA's interval at least
+constexpr int kMaxSms = 160;      // CTAs whose parts fit the workspace
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 template <class T>
-__global__ void __launch_bounds__(kSimpleThreads) k_attention_simple(AttnArgs a) {
-    __shared__ float s_q[128], s_p[kSimpleThreads], s_red[4];
-    const PagedView& c = a.c;
-    const int t = blockIdx.x, h = blockIdx.y, D = c.head_dim, g = h / (a.n_heads / c.n_kv);
-    const int seq = seq_of_token(a.cu, c.n_seq, t);
-    if (seq < 0) return;
-    const int2 tok = seq_tokens(c, a.cu, a.n_tokens, seq);
-    if (t - tok.x >= tok.y) return;
-    const int len = seq_len(c, seq);
-    const int sees = len - tok.y + (t - tok.x) + 1;
-    if (len < tok.y && threadIdx.x == 0) flag(c, BAD_LEN);
-    const T* q = reinterpret_cast<const T*>(a.q) + t * a.q_stride + (long long)h * D;
-    if (threadIdx.x < D) s_q[threadIdx.x] = to_f32<T>(q[threadIdx.x]);
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (int j0 = 0; j0 < sees; j0 += kSimpleThreads) {
-        const int j = j0 + threadIdx.x;
-        float s = -INFINITY;
-        if (j < sees) {
-            const int page = page_of(c, seq, j / kPage);
-            if (page >= 0) {
-                const T* k = reinterpret_cast<const T*>(c.k) + page * c.page_stride + g * c.head_stride + (long long)(j % kPage) * D;
-                s = 0.f;
-                for (int d = 0; d < D; ++d) s = fmaf(s_q[d], to_f32<T>(k[d]), s);
-                s *= a.scale;
-            }
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// ---- few rows ------------------------------------------------------------------------------------------------------
+//
+// A step or a verify pass: a tile of 16, 32 or 64 rows, so each K and V byte
+// serves few products and the cache's bytes bound the kernel.  One CTA per SM
+// walks its interval of 64-slot pages; a producer warp brings a page's K and V
+// (TMA boxes of 64 slots x 64 dims, 128-byte swizzle: the ldmatrix reads below
+// are free of bank conflicts) into a ring of as many pages as shared memory
+// holds, across tile borders.  Each of four warps takes 16 of the page's 64
+// slots, with a maximum, sum and f32 result of its own (m16n8k16, scores stay in
+// registers as the second product's operand), so that no page costs a barrier among them;
+// the four are joined when the tile's part ends.  64 rows: two such groups of
+// four warps, 32 rows each.
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+template <class T>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// MW: 16-row tiles of a warp; WM: groups of four warps.
+template <int kD, int MW, int WM>
+struct RowsShape {
+    static constexpr int kRows = 16 * MW * WM;
+    static constexpr int kThreads = (4 * WM + 1) * 32;
+    static constexpr int kHalf = kPage * 128;                  // bytes of 64 slots x 64 dims
+    static constexpr int kStage = 2 * (kD / 64) * kHalf;       // a page's K, then its V
+    static constexpr int kQ = kRows * kD * 2;
+    static constexpr int kPad = kD + 8;                        // floats of a joined row: no two rows on the same banks
+    static constexpr int kJoin = 2 * kRows * kPad * 4;
+    static constexpr int kRoom = 227 * 1024 - 1024 - 4096;     // alignment, static
+    static constexpr int kFit = (kRoom - kQ - kJoin) / kStage;
+    static constexpr int kStages = kFit > 12 ? 12 : kFit;
+    static constexpr int kSmem = 1024 + kStages * kStage + kQ + kJoin;
+};
+
+template <class T, int kD, int MW, int WM>
+__global__ void __launch_bounds__(RowsShape<kD, MW, WM>::kThreads, 1)
+    k_attention_rows(const AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+    using S = RowsShape<kD, MW, WM>;
+    constexpr int kParts = kD / 64;  // 64-dim halves of a row
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t full[S::kStages], empty[S::kStages];
+    __shared__ int s_page[S::kStages];          // the stage's page, negative: masked
+    __shared__ long long s_scan[16];
+    __shared__ float s_m[WM][4][16 * MW], s_l[WM][4][16 * MW];
+    __shared__ int s_gave_up, s_last, s_go;
+    const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;
+    uint8_t* q_at = smem_raw + (ring - smem_u32(smem_raw)) + S::kStages * S::kStage;
+    float* join = reinterpret_cast<float*>(q_at + S::kQ);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Geometry ge{a.n_heads / a.c.n_kv, S::kRows, kPage};
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::kStages; ++i) {
+            bar_init(&full[i], 1);
+            bar_init(&empty[i], 4 * WM);
         }
-        float mx = s;
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-        if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = mx;
-        __syncthreads();
-        mx = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-        const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.f : mn;
-        const float p = expf(s - base), keep = expf(m - base);
-        s_p[threadIdx.x] = p;
-        __syncthreads();
-        o *= keep;
-        l *= keep;
-        m = mn;
-        for (int i = 0; i < min(kSimpleThreads, sees - j0); ++i) {
-            l += s_p[i];
-            if (threadIdx.x < D && s_p[i] != 0.f) {
-                const int page = c.table[(long long)seq * c.table_stride + (j0 + i) / kPage];
-                const T* v = reinterpret_cast<const T*>(c.v) + page * c.page_stride + g * c.head_stride + (long long)((j0 + i) % kPage) * D;
-                o = fmaf(s_p[i], to_f32<T>(v[threadIdx.x]), o);
-            }
-        }
-        __syncthreads();
+        s_gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    T* out = reinterpret_cast<T*>(a.out) + t * a.out_stride + (long long)h * D;
-    if (threadIdx.x < D) out[threadIdx.x] = from_f32<T>(l == 0.f ? 0.f : o / l);
-    if (threadIdx.x == 0 && a.lse) a.lse[(long long)t * a.n_heads + h] = l == 0.f ? -INFINITY : m + logf(l);
+    const Line line = find_line<S::kThreads>(a, ge, kRowsMinUnits, s_scan);
+    __syncthreads();
+    if (line.lo >= line.hi) return;
+    Walk walk(a, ge, line);
+    Part p;
+
+    if (warp == 4 * WM) {
+        // Producer: table entries 32 at a time, one a lane.
+        int st = 0, round = 0;
+        while (walk.next(&p)) {
+            for (int b0 = p.b0; b0 < p.b1; b0 += 32) {
+                int mine = 0;
+                const SeqWork w = seq_work(a, ge, p.seq);
+                if (b0 + lane < p.b1) mine = (b0 + lane) * kPage < w.len ? page_of(a.c, p.seq, b0 + lane) : -1;
+                for (int b = b0; b < min(p.b1, b0 + 32); ++b) {
+                    const int page = __shfl_sync(0xffffffffu, mine, b - b0);
+                    if (round > 0 && !bar_wait(&empty[st], (round - 1) & 1, &s_gave_up)) goto drained;
+                    if (lane == 0) {
+                        s_page[st] = page;
+                        if (page < 0) {
+                            bar_arrive(&full[st]);
+                        } else {
+                            bar_expect(&full[st], S::kStage);
+                            const uint32_t dst = ring + st * S::kStage;
+#pragma unroll
+                            for (int h = 0; h < kParts; ++h) {
+                                tma_load_4d(dst + h * S::kHalf, &k_map, h * 64, 0, p.head, page, &full[st]);
+                                tma_load_4d(dst + (kParts + h) * S::kHalf, &v_map, h * 64, 0, p.head, page, &full[st]);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    if (++st == S::kStages) st = 0, ++round;
+                }
+            }
+        }
+    drained:
+        // No copy is left in flight when the CTA ends: each stage's last fill has landed.
+        for (int i = 0; i < S::kStages; ++i) {
+            const int fills = round + (i < st ? 1 : 0);
+            if (fills > 0) {
+                volatile int none = 0;
+                bar_wait(&full[i], (fills - 1) & 1, &none);
+            }
+        }
+        if (s_gave_up) flag(a.c, BAD_WAIT);
+        return;
+    }
+
+    const int group = warp >> 2, sw = warp & 3;
+    const int tid = threadIdx.x;                   // of the 128 WM consumers
+    const int gt = tid - group * 128;              // of the group's 128
+    const float to_log2 = a.scale * kLog2e;
+    int st = 0;
+    unsigned phase = 0;
+    while (walk.next(&p)) {
+        const SeqWork w = seq_work(a, ge, p.seq);
+        const int base = w.len - w.n_new;  // the first new token's slot
+        bool ok = true;
+        // The groups share q's place: both are through with the last tile's.
+        if (WM > 1) asm volatile("bar.sync 3, %0;" ::"n"(128 * WM) : "memory");
+        if (tid == 0) s_go = !s_gave_up;
+        // The tile's q rows, swizzled like K; rows that are none are 0.
+        for (int i = tid; i < S::kRows * (kD / 8); i += 128 * WM) {
+            const int r = i / (kD / 8), ch = i % (kD / 8);
+            long long token;
+            int head;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (row_place(a, ge, w, p, r, &token, &head))
+                x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + token * a.q_stride + (long long)head * kD + ch * 8);
+            *reinterpret_cast<uint4*>(q_at + (ch / 8) * (S::kRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) * 16)) = x;
+        }
+        asm volatile("bar.sync 3, %0;" ::"n"(128 * WM) : "memory");
+        if (!s_go) break;  // the same for all of them: none waits at a barrier that another has left
+        const uint32_t qa = smem_u32(q_at);
+        // Slots that row r of the tile sees: [0, base + token(r) + 1).
+        int sees[MW][2];
+        int least = INT_MAX, most = 0;
+#pragma unroll
+        for (int mt = 0; mt < MW; ++mt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = p.tile * S::kRows + group * 16 * MW + mt * 16 + e * 8 + lane / 4;
+                sees[mt][e] = r < w.n_new * ge.G ? base + r / ge.G + 1 : 0;
+            }
+        {
+            const int r0 = p.tile * S::kRows + group * 16 * MW, r1 = min(r0 + 16 * MW, w.n_new * ge.G) - 1;
+            least = r0 + 16 * MW <= w.n_new * ge.G ? base + r0 / ge.G + 1 : 0;
+            most = r1 >= r0 ? base + r1 / ge.G + 1 : 0;
+        }
+        uint32_t q[MW == 1 ? kD / 16 : 1][4];
+        if constexpr (MW == 1) {
+#pragma unroll
+            for (int kk = 0; kk < kD / 16; ++kk) {
+                const int r = group * 16 + (lane & 15), ch = kk * 2 + (lane >> 4);
+                ldsm4(q[kk], qa + (ch / 8) * (S::kRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) * 16));
+            }
+        }
+        float o[MW][kD / 8][4], m[MW][2], l[MW][2];
+#pragma unroll
+        for (int mt = 0; mt < MW; ++mt) {
+#pragma unroll
+            for (int n = 0; n < kD / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
+            m[mt][0] = m[mt][1] = -INFINITY;
+            l[mt][0] = l[mt][1] = 0.f;
+        }
+        for (int b = p.b0; b < p.b1; ++b) {
+            if (!bar_wait(&full[st], phase, &s_gave_up)) {
+                ok = false;
+                break;
+            }
+            const int s0 = b * kPage + sw * 16;  // the warp's first slot
+            if (s_page[st] >= 0 && s0 < most) {
+                const uint32_t kb = ring + st * S::kStage, vb = kb + kParts * S::kHalf;
+                float s[MW][2][4];
+#pragma unroll
+                for (int mt = 0; mt < MW; ++mt)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.f;
+#pragma unroll
+                for (int kk = 0; kk < kD / 16; ++kk) {
+                    uint32_t kf[4];
+                    const int slot = sw * 16 + ((lane >> 4) << 3) + (lane & 7), ch = kk * 2 + ((lane >> 3) & 1);
+                    ldsm4(kf, kb + (ch / 8) * S::kHalf + slot * 128 + (((ch & 7) ^ (slot & 7)) * 16));
+#pragma unroll
+                    for (int mt = 0; mt < MW; ++mt) {
+                        uint32_t qf[4];
+                        if constexpr (MW == 1) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) qf[e] = q[kk][e];
+                        } else {
+                            const int r = group * 16 * MW + mt * 16 + (lane & 15), qc = kk * 2 + (lane >> 4);
+                            ldsm4(qf, qa + (qc / 8) * (S::kRows * 128) + r * 128 + (((qc & 7) ^ (r & 7)) * 16));
+                        }
+                        mma16<T>(s[mt][0], qf, kf[0], kf[1]);
+                        mma16<T>(s[mt][1], qf, kf[2], kf[3]);
+                    }
+                }
+                uint32_t pa[MW][4];
+                const bool mask = s0 + 16 > least;
+#pragma unroll
+                for (int mt = 0; mt < MW; ++mt) {
+                    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float x = s[mt][n][e] * to_log2;
+                            if (mask && s0 + n * 8 + (lane & 3) * 2 + (e & 1) >= sees[mt][e >> 1]) x = -INFINITY;
+                            s[mt][n][e] = x;
+                            top[e >> 1] = fmaxf(top[e >> 1], x);
+                        }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
+                        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
+                    }
+                    // The maximum follows only when it has grown by more than 8.
+                    const bool grown = top[0] > m[mt][0] + 8.f || top[1] > m[mt][1] + 8.f;
+                    if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float to = fmaxf(m[mt][e], top[e]);
+                            const float f = to == -INFINITY ? 1.f : exp2_fast(m[mt][e] - to);
+                            m[mt][e] = to;
+                            l[mt][e] *= f;
+#pragma unroll
+                            for (int n = 0; n < kD / 8; ++n) {
+                                o[mt][n][2 * e] *= f;
+                                o[mt][n][2 * e + 1] *= f;
+                            }
+                        }
+                    }
+                    const float b0 = m[mt][0] == -INFINITY ? 0.f : m[mt][0], b1 = m[mt][1] == -INFINITY ? 0.f : m[mt][1];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            s[mt][n][e] = exp2_fast(s[mt][n][e] - (e < 2 ? b0 : b1));
+                            l[mt][e >> 1] += s[mt][n][e];
+                        }
+                        pa[mt][2 * n] = pack2<T>(s[mt][n][0], s[mt][n][1]);
+                        pa[mt][2 * n + 1] = pack2<T>(s[mt][n][2], s[mt][n][3]);
+                    }
+                }
+                // V at or behind the sequence's end may hold anything: 0 there, since 0 * NaN is NaN.
+                const bool tail = s0 + 16 > w.len;
+                uint32_t lo_on = 0xffffffffu, hi_on = 0xffffffffu;
+                if (tail) {
+                    const int first = s0 + (lane & 3) * 2;
+                    lo_on = (first < w.len ? 0xffffu : 0u) | (first + 1 < w.len ? 0xffff0000u : 0u);
+                    hi_on = (first + 8 < w.len ? 0xffffu : 0u) | (first + 9 < w.len ? 0xffff0000u : 0u);
+                }
+#pragma unroll
+                for (int nd = 0; nd < kD / 16; ++nd) {
+                    uint32_t vf[4];
+                    const int slot = sw * 16 + (lane & 15), ch = nd * 2 + (lane >> 4);
+                    ldsm4t(vf, vb + (ch / 8) * S::kHalf + slot * 128 + (((ch & 7) ^ (slot & 7)) * 16));
+                    if (tail) {
+                        vf[0] &= lo_on;
+                        vf[1] &= hi_on;
+                        vf[2] &= lo_on;
+                        vf[3] &= hi_on;
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < MW; ++mt) {
+                        mma16<T>(o[mt][2 * nd], pa[mt], vf[0], vf[1]);
+                        mma16<T>(o[mt][2 * nd + 1], pa[mt], vf[2], vf[3]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) bar_arrive(&empty[st]);
+            if (++st == S::kStages) st = 0, phase ^= 1;
+        }
+        // The group's four warps joined: maxima, then the scaled results in two buffers.
+#pragma unroll
+        for (int mt = 0; mt < MW; ++mt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 1);
+                l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 2);
+                if ((lane & 3) == 0) {
+                    s_m[group][sw][mt * 16 + e * 8 + lane / 4] = m[mt][e];
+                    s_l[group][sw][mt * 16 + e * 8 + lane / 4] = l[mt][e];
+                }
+            }
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+        float* buf = join + ((sw & 1) * S::kRows + group * 16 * MW) * S::kPad;
+#pragma unroll
+        for (int turn = 0; turn < 2; ++turn) {  // warps 2 and 3 store, then 0 and 1 add theirs
+            if ((sw < 2) == (turn == 1)) {
+#pragma unroll
+                for (int mt = 0; mt < MW; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int r = mt * 16 + e * 8 + lane / 4;
+                        const float top = fmaxf(fmaxf(s_m[group][0][r], s_m[group][1][r]), fmaxf(s_m[group][2][r], s_m[group][3][r]));
+                        const float f = m[mt][e] == -INFINITY ? 0.f : exp2f(m[mt][e] - top);
+#pragma unroll
+                        for (int n = 0; n < kD / 8; ++n) {
+                            float2* at = reinterpret_cast<float2*>(buf + r * S::kPad + n * 8 + (lane & 3) * 2);
+                            float2 x = make_float2(o[mt][n][2 * e] * f, o[mt][n][2 * e + 1] * f);
+                            if (turn == 1) {
+                                const float2 y = *at;
+                                x.x += y.x;
+                                x.y += y.y;
+                            }
+                            *at = x;
+                        }
+                    }
+            }
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+        }
+        const bool whole = p.b0 == 0 && p.b1 == p.n;
+        float* part = whole ? nullptr : part_at<S::kRows, kD>(a, blockIdx.x, p.b0 == 0);
+        for (int i = gt; i < 16 * MW * (kD / 4); i += 128) {
+            const int gr = i / (kD / 4), col = i % (kD / 4) * 4, r = group * 16 * MW + gr;
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) top = fmaxf(top, s_m[group][x][gr]);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const float mx = s_m[group][x][gr];
+                sum += s_l[group][x][gr] * (mx == -INFINITY ? 0.f : exp2f(mx - top));
+            }
+            const float4 x = *reinterpret_cast<const float4*>(join + r * S::kPad + col);
+            const float4 y = *reinterpret_cast<const float4*>(join + (S::kRows + r) * S::kPad + col);
+            const float4 z = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+            long long token;
+            int head;
+            if (!ok || !row_place(a, ge, w, p, r, &token, &head)) continue;
+            if (whole) {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                store4<T>(reinterpret_cast<T*>(a.out) + token * a.out_stride + (long long)head * kD + col,
+                          make_float4(z.x * inv, z.y * inv, z.z * inv, z.w * inv));
+                if (col == 0 && a.lse) a.lse[token * a.n_heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+            } else {
+                *reinterpret_cast<float4*>(part + 2 * S::kRows + r * kD + col) = z;
+                if (col == 0) {
+                    part[r] = top;
+                    part[S::kRows + r] = sum;
+                }
+            }
+        }
+        if (!whole) {
+            __threadfence();
+            asm volatile("bar.sync 3, %0;" ::"n"(128 * WM) : "memory");
+            if (tid == 0) {
+                const int c0 = cta_of(line, p.u0), c1 = cta_of(line, p.u0 + p.n - 1);
+                int* count = reinterpret_cast<int*>(a.workspace) + c0;
+                const int before = atomicAdd(count, 1);
+                s_last = before == c1 - c0;
+                if (s_last) *count = 0;
+                __threadfence();
+            }
+            asm volatile("bar.sync 3, %0;" ::"n"(128 * WM) : "memory");
+            if (s_last) join_parts<T, S::kRows, kD, 128 * WM>(a, ge, line, w, p, tid);
+        }
+    }
+}
+
+template <class T, int kD, int MW, int WM>
+cudaError_t launch_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int sms, cudaStream_t s) {
+    using S = RowsShape<kD, MW, WM>;
+    auto* kernel = k_attention_rows<T, kD, MW, WM>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    if (e != cudaSuccess) return e;
+    kernel<<<sms, S::kThreads, S::kSmem, s>>>(a, km, vm);
+    return cudaGetLastError();
+}
+
+template <class T, int kD>
+cudaError_t launch_by_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int sms, cudaStream_t s) {
+    const long long rows = (long long)a.max_tokens * (a.n_heads / a.c.n_kv);
+    if (rows <= 16) return launch_rows<T, kD, 1, 1>(a, km, vm, sms, s);
+    if (rows <= 32) return launch_rows<T, kD, 2, 1>(a, km, vm, sms, s);
+    return launch_rows<T, kD, 2, 2>(a, km, vm, sms, s);
+}
+
+// One of the cache's two maps: dims (dim, row of the page, KV head, page), boxes
+// of 64 dims x 64 rows.
+bool encode_map(CUtensorMap* map, const PagedView& c, void* base) {
+    using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const EncodeFn encode = [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return reinterpret_cast<EncodeFn>(fn);
+    }();
+    if (!encode) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, kPage, (cuuint64_t)c.n_kv, (cuuint64_t)c.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.head_dim * 2, (cuuint64_t)c.head_stride * 2, (cuuint64_t)c.page_stride * 2};
+    const cuuint32_t box[4] = {64, kPage, 1, 1}, steps[4] = {1, 1, 1, 1};
+    return encode(map, c.type == OP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, box,
+                  steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int sm_count() {
+    int device = 0, n = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
+    return std::min(n, kMaxSms);
 }
 
 // One CTA of 64 threads per (sequence, KV head, page): a thread owns a slot.
@@ -104,10 +498,12 @@ __global__ void __launch_bounds__(kPage) k_weights_simple(AttnArgs a, int pages)
 }  // namespace
 
 cudaError_t launch_paged_attention(const AttnArgs& a, cudaStream_t s) {
-    const dim3 grid(a.n_tokens, a.n_heads);
-    if (a.c.type == OP_F16) k_attention_simple<__half><<<grid, kSimpleThreads, 0, s>>>(a);
-    else k_attention_simple<__nv_bfloat16><<<grid, kSimpleThreads, 0, s>>>(a);
-    return cudaGetLastError();
+    CUtensorMap km, vm;
+    const int sms = sm_count();
+    if (sms == 0 || !encode_map(&km, a.c, a.c.k) || !encode_map(&vm, a.c, a.c.v)) return cudaErrorInvalidValue;
+    if (a.c.type == OP_F16)
+        return a.c.head_dim == 64 ? launch_by_rows<__half, 64>(a, km, vm, sms, s) : launch_by_rows<__half, 128>(a, km, vm, sms, s);
+    return a.c.head_dim == 64 ? launch_by_rows<__nv_bfloat16, 64>(a, km, vm, sms, s) : launch_by_rows<__nv_bfloat16, 128>(a, km, vm, sms, s);
 }
 
 cudaError_t launch_attention_weights(const AttnArgs& a, cudaStream_t s) {

@@ -1,0 +1,287 @@
+// What the attention kernels over a paged cache share: how the work is cut,
+// how parts of a row tile are joined, barriers and copies.
+//
+// Rows: the new tokens of a sequence times the query heads of one KV head,
+// row r = (token r / G, head r % G); a tile is kRows consecutive rows.  Units: a
+// tile's visible cache in blocks of kBlock slots (at least one).  All units of
+// all (sequence, KV head, tile) stand in one line, and CTA c of g takes the
+// c-th of g equal intervals of it, whatever the lengths are.  A tile that lies in
+// one interval is finished there.  One that spans several leaves its parts (f32
+// sums, row maxima and row sums) in the workspace, and whichever CTA comes last
+// joins them in the order of the intervals: no order of arrival changes a bit,
+// and no CTA waits for another.
+#pragma once
+
+#include "ops_common.cuh"
+
+#include <cuda.h>
+
+namespace mtb {
+namespace ops {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// ---- barriers and copies -------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint64_t* b, unsigned count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t* b, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ unsigned long long now_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+constexpr unsigned long long kWaitNs = 4000000000ull;
+
+// Waits for a phase; false once the wait ran out or another wait of this CTA
+// did (`gave_up`, shared memory), so that every role leaves its loop.
+__device__ __forceinline__ bool bar_wait(uint64_t* b, unsigned parity, volatile int* gave_up) {
+    const uint32_t at = smem_u32(b);
+    unsigned long long t0 = 0;
+    for (unsigned it = 0;; ++it) {
+        uint32_t ok;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+                     : "=r"(ok)
+                     : "r"(at), "r"(parity), "r"(20000u)
+                     : "memory");
+        if (ok) return true;
+        if (it == 0) t0 = now_ns();
+        if (*gave_up) return false;
+        if (now_ns() - t0 > kWaitNs) {
+            *gave_up = 1;
+            return false;
+        }
+    }
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// ---- the line of units ---------------------------------------------------------------------------------------------
+
+struct SeqWork {
+    int len, tok0, n_new, tiles;
+};
+
+struct Geometry {
+    int G, rows, block;  // query heads per KV head, rows per tile, slots per block
+};
+
+__device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, const Geometry& ge, int s) {
+    const int2 tok = seq_tokens(a.c, a.cu, a.n_tokens, s);
+    SeqWork w{0, tok.x, tok.y, 0};
+    if (tok.y == 0) return w;
+    w.len = seq_len(a.c, s);
+    w.tiles = (tok.y * ge.G + ge.rows - 1) / ge.rows;
+    return w;
+}
+// Blocks that the rows of a tile see, at least 1.
+__device__ __forceinline__ int tile_blocks(const SeqWork& w, const Geometry& ge, int tile) {
+    const int last = min(w.n_new - 1, ((tile + 1) * ge.rows - 1) / ge.G);
+    const int sees = w.len - w.n_new + last + 1;
+    return max(1, (sees + ge.block - 1) / ge.block);
+}
+__device__ __forceinline__ long long head_units(const SeqWork& w, const Geometry& ge) {
+    long long u = 0;
+    for (int t = 0; t < w.tiles; ++t) u += tile_blocks(w, ge, t);
+    return u;
+}
+
+// The CTA's interval of the line, and where it begins.
+struct Line {
+    long long total, lo, hi;
+    int ctas;         // CTAs that have an interval
+    int seq;          // sequence of unit lo
+    long long off;    // of lo in that sequence's units
+};
+
+// All threads of the CTA; s_scan: one long long a warp + 4.
+template <int kThreads>
+__device__ Line find_line(const AttnArgs& a, const Geometry& ge, int min_units, long long* s_scan) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int kWarps = kThreads / 32;
+    long long mine = 0, sum = 0;
+    for (int s = threadIdx.x; s < a.c.n_seq; s += kThreads) {
+        const SeqWork w = seq_work(a, ge, s);
+        if (w.n_new > w.len && blockIdx.x == 0) flag(a.c, BAD_LEN);
+        mine = head_units(w, ge) * a.c.n_kv;
+        sum += mine;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) s_scan[warp] = sum;
+    __syncthreads();
+    Line l{};
+    for (int w = 0; w < kWarps; ++w) l.total += s_scan[w];
+    const long long fit = max(1ll, l.total / min_units);
+    l.ctas = (int)min((long long)gridDim.x, fit);
+    if (l.total == 0) l.ctas = 0;
+    if ((int)blockIdx.x < l.ctas) {
+        l.lo = l.total * blockIdx.x / l.ctas;
+        l.hi = l.total * (blockIdx.x + 1) / l.ctas;
+    }
+    long long base = 0;
+    for (int s0 = 0; s0 < a.c.n_seq; s0 += kThreads) {
+        const int s = s0 + threadIdx.x;
+        long long v = a.c.n_seq <= kThreads ? mine : s < a.c.n_seq ? head_units(seq_work(a, ge, s), ge) * a.c.n_kv : 0;
+        if (s >= a.c.n_seq) v = 0;
+        long long x = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) s_scan[warp] = x;
+        __syncthreads();
+        long long before = base;
+        for (int w = 0; w < warp; ++w) before += s_scan[w];
+        for (int w = 0; w < kWarps; ++w) base += s_scan[w];
+        const long long first = before + x - v;
+        if (v > 0 && first <= l.lo && l.lo < first + v) {
+            s_scan[kWarps] = s;
+            s_scan[kWarps + 1] = l.lo - first;
+        }
+    }
+    __syncthreads();
+    l.seq = (int)s_scan[kWarps];
+    l.off = s_scan[kWarps + 1];
+    return l;
+}
+
+// The CTA whose interval holds unit u.
+__device__ __forceinline__ int cta_of(const Line& l, long long u) { return (int)(((u + 1) * l.ctas - 1) / l.total); }
+
+// A CTA's part of one tile: blocks [b0, b1) of its n.
+struct Part {
+    int seq, head, tile, b0, b1, n;
+    long long u0;  // the tile's first unit
+};
+
+// Walks the CTA's interval; every role of the CTA walks it by itself.
+struct Walk {
+    const AttnArgs& a;
+    const Geometry ge;
+    long long at, hi;  // next unit, end of the interval
+    SeqWork w{};
+    int seq, head = 0, tile = 0, block = 0;
+
+    __device__ Walk(const AttnArgs& args, const Geometry& g, const Line& l) : a(args), ge(g), at(l.lo), hi(l.hi), seq(l.seq) {
+        if (at >= hi) return;
+        w = seq_work(a, ge, seq);
+        const long long per = head_units(w, ge);
+        long long off = l.off % per;
+        head = (int)(l.off / per);
+        for (;;) {
+            const int n = tile_blocks(w, ge, tile);
+            if (off < n) break;
+            off -= n;
+            ++tile;
+        }
+        block = (int)off;
+    }
+    __device__ bool next(Part* p) {
+        if (at >= hi) return false;
+        const int n = tile_blocks(w, ge, tile);
+        const int take = (int)min((long long)(n - block), hi - at);
+        *p = Part{seq, head, tile, block, block + take, n, at - block};
+        at += take;
+        block += take;
+        if (block == n) {
+            block = 0;
+            if (++tile == w.tiles) {
+                tile = 0;
+                if (++head == a.c.n_kv) {
+                    head = 0;
+                    if (at < hi) {
+                        do w = seq_work(a, ge, ++seq);
+                        while (w.n_new == 0);
+                    }
+                }
+            }
+        }
+        return true;
+    }
+    // The sequence of the part that next() returned last may differ from w.
+};
+
+// ---- parts in the workspace ----------------------------------------------------------------------------------------
+
+// Counters (one for each CTA that begins a split tile), then two parts for each
+// CTA: of the tile that reached into its interval, and of the one that begins
+// there.  A part: row maxima (log2), row sums, f32 sums of p v.
+constexpr size_t kPartsAt = 8192;
+constexpr int kMaxCtas = 1024;  // counters that fit
+
+template <int kRows, int kD>
+__device__ __forceinline__ float* part_at(const AttnArgs& a, int cta, bool begins) {
+    return reinterpret_cast<float*>(a.workspace + kPartsAt) + (size_t)(2 * cta + (begins ? 1 : 0)) * (kRows * (kD + 2));
+}
+
+template <class T>
+__device__ __forceinline__ void store4(T* p, float4 x) {
+    uint2 u;
+    T* t = reinterpret_cast<T*>(&u);
+    t[0] = from_f32<T>(x.x);
+    t[1] = from_f32<T>(x.y);
+    t[2] = from_f32<T>(x.z);
+    t[3] = from_f32<T>(x.w);
+    *reinterpret_cast<uint2*>(p) = u;
+}
+
+// Where row r of a part's tile goes; false: not a row of the sequence.
+__device__ __forceinline__ bool row_place(const AttnArgs& a, const Geometry& ge, const SeqWork& w, const Part& p, int r, long long* token,
+                                          int* head) {
+    const int row = p.tile * ge.rows + r;
+    if (row >= w.n_new * ge.G) return false;
+    *token = w.tok0 + row / ge.G;
+    *head = p.head * ge.G + row % ge.G;
+    return true;
+}
+
+// Joins a split tile's parts, by kThreads threads numbered t.
+template <class T, int kRows, int kD, int kThreads>
+__device__ void join_parts(const AttnArgs& a, const Geometry& ge, const Line& l, const SeqWork& w, const Part& p, int t) {
+    const int c0 = cta_of(l, p.u0), c1 = cta_of(l, p.u0 + p.n - 1);
+    constexpr int kCols = kD / 4;
+    for (int i = t; i < kRows * kCols; i += kThreads) {
+        const int r = i / kCols, col = i % kCols * 4;
+        long long token;
+        int head;
+        if (!row_place(a, ge, w, p, r, &token, &head)) continue;
+        float m = -INFINITY;
+        for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(part_at<kRows, kD>(a, c, c == c0) + r));
+        const float base = m == -INFINITY ? 0.f : m;
+        float sum = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int c = c0; c <= c1; ++c) {
+            const float* q = part_at<kRows, kD>(a, c, c == c0);
+            const float f = exp2f(__ldcg(q + r) - base);
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(q + 2 * kRows + r * kD + col));
+            sum = fmaf(f, __ldcg(q + kRows + r), sum);
+            o.x = fmaf(f, x.x, o.x);
+            o.y = fmaf(f, x.y, o.y);
+            o.z = fmaf(f, x.z, o.z);
+            o.w = fmaf(f, x.w, o.w);
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        store4<T>(reinterpret_cast<T*>(a.out) + token * a.out_stride + (long long)head * kD + col,
+                  make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+        if (col == 0 && a.lse) a.lse[token * a.n_heads + head] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+    }
+}
+
+}  // namespace ops
+}  // namespace mtb

@@ -50,7 +50,7 @@ DRAFT_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.POINTER(C.c_int32), C.c_int, C.c_i
 COMMIT_FN = C.CFUNCTYPE(None, C.c_void_p, C.POINTER(C.c_int32), C.c_int, C.c_int, C.c_int)
 
 T_F32, T_F16, T_BF16 = 0, 1, 2
-BAD_PAGE, BAD_LEN, BAD_TOKENS = 1, 2, 4
+BAD_PAGE, BAD_LEN, BAD_TOKENS, BAD_WAIT = 1, 2, 4, 8
 ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN, ROPE_BANDS = range(5)
 ATTENTION_WORKSPACE = 64 << 20
 PAGE = 64
