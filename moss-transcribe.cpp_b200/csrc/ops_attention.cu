@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 namespace mtb {
 namespace {
@@ -16,6 +17,7 @@ namespace {
 using namespace ops;
 
 constexpr int kRowsMinUnits = 2;  // pages of a CTA's interval at least
+constexpr int kTilesMinUnits = 1; // blocks of 128 slots
 constexpr int kMaxSms = 160;      // CTAs whose parts fit the workspace
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -427,12 +429,386 @@ cudaError_t launch_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensor
     return cudaGetLastError();
 }
 
+// ---- many rows -----------------------------------------------------------------------------------------------------
+//
+// A chunk of new tokens: 256 rows a tile as two halves of 128, blocks of 128
+// slots; the products bound the kernel, with the exponentials next to them
+// (both take 1024 clocks of an SM for a half's block).  tcgen05 products,
+// issued by one thread: S = Q K^T into tensor memory, and O += P V with P
+// read from there.  The halves alternate: while a half's four warps (a row a thread,
+// so maxima and sums need no other thread) turn S into P, the tensor cores work for the
+// other.  P takes the place of S.  A half's products run in order, so S of block
+// j + 1 is issued behind P V of block j without a wait, and once S is there O is
+// free to be rescaled.
+constexpr int kTileRows2 = 256;
+constexpr int kTileBlock = 128;
+constexpr int kTileThreads = 384;  // warps 0-3 and 4-7: the halves; 8: products; 9: copies; 10, 11: none
+// Registers: 168 a thread at launch; a half's threads hold a row of 128 scores,
+// so the other four warps give theirs up: 256 x 224 + 128 x 56 = 384 x 168.
+constexpr int kHalfRegs = 224, kOtherRegs = 56;
+constexpr int kTileEntries = 4;    // ring of K and V blocks, in turn
+constexpr int kBadRing = 16;       // blocks whose bad-page bits are kept
+
+template <int kD>
+struct TileShape {
+    static constexpr int kPart = kTileBlock * 128;        // bytes of 128 rows x 64 dims
+    static constexpr int kEntry = (kD / 64) * kPart;      // one K or V block, or one half's q
+    static constexpr int kSmem = 1024 + (kTileEntries + 2) * kEntry;
+};
+
+template <class T, int kD>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    k_attention_tiles(const AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+    using S = TileShape<kD>;
+    constexpr int kParts = kD / 64;
+    constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t full[kTileEntries], empty[kTileEntries], q_full[2], s_full[2], p_full[2], o_full[2], drained;
+    __shared__ long long s_scan[16];
+    __shared__ int s_bad[kBadRing];  // bit 0, 1: the block's pages that are masked
+    __shared__ int s_gave_up, s_last;
+    __shared__ uint32_t s_tmem;
+    const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;
+    const uint32_t q_at = ring + kTileEntries * S::kEntry;
+    uint8_t* q_ptr = smem_raw + (q_at - smem_u32(smem_raw));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Geometry ge{a.n_heads / a.c.n_kv, kTileRows2, kTileBlock};
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kTileEntries; ++i) {
+            bar_init(&full[i], 1);
+            bar_init(&empty[i], 1);
+        }
+        for (int h = 0; h < 2; ++h) {
+            bar_init(&q_full[h], 128);
+            bar_init(&s_full[h], 1);
+            bar_init(&p_full[h], 128);
+            bar_init(&o_full[h], 1);
+        }
+        bar_init(&drained, 1);
+        s_gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    const Line line = find_line<kTileThreads>(a, ge, kTilesMinUnits, s_scan);
+    __syncthreads();
+    if (line.lo >= line.hi) return;
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;  // S of the halves at 0 and 128, O at 256 and 384
+    Walk walk(a, ge, line);
+    Part p;
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+      if (warp == 9) {
+        int e = 0, round = 0, turn = 0;
+        bool ok = true;
+        while (ok && walk.next(&p)) {
+            const SeqWork w = seq_work(a, ge, p.seq);
+            for (int b0 = p.b0; ok && b0 < p.b1; b0 += 16) {
+                // 32 pages, one a lane; no page there: the box past the pool, which reads as 0.
+                const int at = b0 * 2 + lane;
+                int mine = -1;
+                if (at < p.b1 * 2 && (long long)at * kPage < w.len) mine = page_of(a.c, p.seq, at);
+                for (int b = b0; ok && b < min(p.b1, b0 + 16); ++b) {
+                    const int pg0 = __shfl_sync(0xffffffffu, mine, 2 * (b - b0)), pg1 = __shfl_sync(0xffffffffu, mine, 2 * (b - b0) + 1);
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv) {
+                        if (round > 0 && !bar_wait(&empty[e], (round - 1) & 1, &s_gave_up)) {
+                            ok = false;
+                            break;
+                        }
+                        if (lane == 0) {
+                            if (kv == 0) s_bad[turn] = (pg0 < 0 ? 1 : 0) | (pg1 < 0 ? 2 : 0);
+                            bar_expect(&full[e], S::kEntry);
+                            const uint32_t dst = ring + e * S::kEntry;
+                            const CUtensorMap* map = kv ? &v_map : &k_map;
+#pragma unroll
+                            for (int h = 0; h < kParts; ++h) {
+                                tma_load_4d(dst + h * S::kPart, map, h * 64, 0, p.head, pg0 < 0 ? a.c.n_pages : pg0, &full[e]);
+                                tma_load_4d(dst + h * S::kPart + kPage * 128, map, h * 64, 0, p.head, pg1 < 0 ? a.c.n_pages : pg1, &full[e]);
+                            }
+                        }
+                        __syncwarp();
+                        if (++e == kTileEntries) e = 0, ++round;
+                    }
+                    turn = (turn + 1) % kBadRing;
+                }
+            }
+        }
+        for (int i = 0; i < kTileEntries; ++i) {  // every copy has landed before the CTA ends
+            const int fills = round + (i < e ? 1 : 0);
+            volatile int none = 0;
+            if (fills > 0) bar_wait(&full[i], (fills - 1) & 1, &none);
+        }
+      } else if (warp == 8) {
+        constexpr uint32_t kQk = tc_instr(kBf16, kTileBlock, false), kPv = tc_instr(kBf16, kD, true);
+        int e = 0;
+        unsigned phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+        bool ok = true;
+        auto qk = [&](int h, int entry) {
+            if (lane == 0) {
+                const uint32_t qa = q_at + h * S::kEntry, kb = ring + entry * S::kEntry;
+#pragma unroll
+                for (int kk = 0; kk < kD / 16; ++kk) {
+                    const uint32_t off = (kk / 4) * S::kPart + (kk % 4) * 32;
+                    tc_mma_ss(tmem + h * 128, desc_k(qa + off), desc_k(kb + off), kQk, kk > 0);
+                }
+                tc_commit(&s_full[h]);
+            }
+        };
+        while (ok && walk.next(&p)) {
+            const SeqWork w = seq_work(a, ge, p.seq);
+            const int halves = w.n_new * ge.G - p.tile * kTileRows2 > 128 ? 2 : 1;
+            for (int h = 0; ok && h < halves; ++h) {
+                ok = bar_wait(&q_full[h], q_phase[h], &s_gave_up);
+                q_phase[h] ^= 1;
+            }
+            if (!ok) break;
+            ok = bar_wait(&full[e], phase, &s_gave_up);
+            if (!ok) break;
+            tc_fence_after();
+            for (int h = 0; h < halves; ++h) qk(h, e);
+            if (lane == 0) tc_commit(&empty[e]);
+            if (++e == kTileEntries) e = 0, phase ^= 1;
+            for (int b = p.b0; ok && b < p.b1; ++b) {
+                const int ve = e;
+                ok = bar_wait(&full[ve], phase, &s_gave_up);
+                if (!ok) break;
+                if (++e == kTileEntries) e = 0, phase ^= 1;
+                if ((b + 1) * kTileBlock > w.len) {
+                    // V at or behind the sequence's end may hold anything: 0 there, since 0 * NaN is NaN.
+                    const int from = max(0, w.len - b * kTileBlock);
+                    uint8_t* v = smem_raw + (ring - smem_u32(smem_raw)) + ve * S::kEntry;
+                    for (int i = lane; i < kParts * (kTileBlock - from) * 8; i += 32) {
+                        const int h = i / ((kTileBlock - from) * 8), j = i % ((kTileBlock - from) * 8);
+                        *reinterpret_cast<uint4*>(v + h * S::kPart + from * 128 + j * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                const bool more = b + 1 < p.b1;
+                if (more) ok = bar_wait(&full[e], phase, &s_gave_up);
+                for (int h = 0; ok && h < halves; ++h) {
+                    ok = bar_wait(&p_full[h], p_phase[h], &s_gave_up);
+                    if (!ok) break;
+                    p_phase[h] ^= 1;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        const uint32_t vb = ring + ve * S::kEntry;
+#pragma unroll
+                        for (int kk = 0; kk < kTileBlock / 16; ++kk)
+                            tc_mma_ts(tmem + 256 + h * 128, tmem + h * 128 + kk * 8, desc_mn(vb + kk * 2048, S::kPart), kPv,
+                                      b > p.b0 || kk > 0);
+                        if (!more) tc_commit(&o_full[h]);
+                    }
+                    if (more) qk(h, e);
+                }
+                if (!ok) break;
+                if (lane == 0) tc_commit(&empty[ve]);
+                if (more) {
+                    if (lane == 0) tc_commit(&empty[e]);
+                    if (++e == kTileEntries) e = 0, phase ^= 1;
+                }
+            }
+        }
+        // Nothing that was issued is left running.
+        volatile int none = 0;
+        if (lane == 0) tc_commit(&drained);
+        __syncwarp();
+        bar_wait(&drained, 0, &none);
+      }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kHalfRegs));
+        const int half = warp >> 2, r = half * 128 + (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t t_s = tmem + lanes + half * 128, t_o = tmem + lanes + 256 + half * 128;
+        const float to_log2 = fmaxf(fabsf(a.scale), 1e-37f) * kLog2e;  // above 0: a masked -inf stays -inf
+        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // a negative scale turns q's sign: maxima stay maxima
+        unsigned s_phase = 0, o_phase = 0;
+        int turn = 0;
+        while (walk.next(&p)) {
+            const SeqWork w = seq_work(a, ge, p.seq);
+            const int base = w.len - w.n_new;
+            const bool mine = half == 0 || w.n_new * ge.G - p.tile * kTileRows2 > 128;
+            bool ok = true;
+            float m = -INFINITY, l = 0.f;
+            long long token = 0;
+            int head = 0;
+            const bool row = row_place(a, ge, w, p, r, &token, &head);
+            const bool whole = p.b0 == 0 && p.b1 == p.n;
+            if (mine) {
+                // The half's q rows, swizzled; rows that are none are 0.
+                const int t = threadIdx.x & 127;
+#pragma unroll 4
+                for (int i = t; i < 128 * (kD / 8); i += 128) {
+                    const int rr = i / (kD / 8), ch = i % (kD / 8);
+                    long long tk;
+                    int hd;
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (row_place(a, ge, w, p, half * 128 + rr, &tk, &hd)) {
+                        x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + tk * a.q_stride + (long long)hd * kD + ch * 8);
+                        x.x ^= flip;
+                        x.y ^= flip;
+                        x.z ^= flip;
+                        x.w ^= flip;
+                    }
+                    *reinterpret_cast<uint4*>(q_ptr + half * S::kEntry + (ch / 8) * S::kPart + rr * 128 + (((ch & 7) ^ (rr & 7)) * 16)) = x;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                tc_fence_before();
+                bar_arrive(&q_full[half]);
+                const int sees = row ? base + (p.tile * kTileRows2 + r) / ge.G + 1 : 0;
+                // Slots that every row of the half sees.
+                const int r0 = p.tile * kTileRows2 + half * 128;
+                const int least = r0 + 128 <= w.n_new * ge.G ? base + r0 / ge.G + 1 : 0;
+                for (int b = p.b0; b < p.b1; ++b) {
+                    if (!bar_wait(&s_full[half], s_phase, &s_gave_up)) {
+                        ok = false;
+                        break;
+                    }
+                    s_phase ^= 1;
+                    tc_fence_after();
+                    float s[128];
+                    tmem_ld32<0>(s, t_s);
+                    tmem_ld32<32>(s, t_s + 32);
+                    tmem_ld32<64>(s, t_s + 64);
+                    tmem_ld32<96>(s, t_s + 96);
+                    tmem_wait_ld();
+                    const int bad = s_bad[turn];
+                    turn = (turn + 1) % kBadRing;
+                    const int s0 = b * kTileBlock;
+                    if (s0 + kTileBlock > least) {
+#pragma unroll
+                        for (int i = 0; i < 128; ++i)
+                            if (s0 + i >= sees) s[i] = -INFINITY;
+                    }
+                    if (bad) {
+#pragma unroll
+                        for (int i = 0; i < 128; ++i)
+                            if ((bad >> (i / kPage)) & 1) s[i] = -INFINITY;
+                    }
+                    float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                    for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
+                    top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    const float reach = top[0] == -INFINITY ? -INFINITY : top[0] * to_log2;
+                    if (__any_sync(0xffffffffu, reach > m + 8.f)) {
+                        const float to = fmaxf(m, reach);
+                        const float f = to == -INFINITY ? 1.f : exp2_fast(m - to);
+                        m = to;
+                        l *= f;
+                        if (b > p.b0) {
+#pragma unroll
+                            for (int c = 0; c < kD / 32; ++c) {
+                                float o[32];
+                                tmem_ld32<0>(o, t_o + c * 32);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] *= f;
+                                tmem_st32<0>(t_o + c * 32, o);
+                            }
+                        }
+                    }
+                    const float2 by = make_float2(to_log2, to_log2);
+                    const float less = m == -INFINITY ? 0.f : -m;
+                    const float2 from = make_float2(less, less);
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float2 x = __ffma2_rn(make_float2(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), by, from);
+                            x.x = exp2_fast(x.x);
+                            x.y = exp2_fast(x.y);
+                            sum[i & 1] = __fadd2_rn(sum[i & 1], x);
+                            pk[i] = pack2<T>(x.x, x.y);
+                        }
+                        tmem_st16<0>(t_s + c * 16, pk);
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    bar_arrive(&p_full[half]);
+                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                }
+                if (ok && bar_wait(&o_full[half], o_phase, &s_gave_up)) {
+                    o_phase ^= 1;
+                    tc_fence_after();
+                    float* part = whole ? nullptr : part_at<kTileRows2, kD>(a, blockIdx.x, p.b0 == 0);
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+                    for (int c = 0; c < kD / 32; ++c) {
+                        float o[32];
+                        tmem_ld32<0>(o, t_o + c * 32);
+                        tmem_wait_ld();
+                        if (!row) continue;
+                        if (whole) {
+                            T* out = reinterpret_cast<T*>(a.out) + token * a.out_stride + (long long)head * kD + c * 32;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float x[8];
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) x[k] = o[i * 8 + k] * inv;
+                                store_vec<T, 8>(out + i * 8, x);
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                *reinterpret_cast<float4*>(part + 2 * kTileRows2 + r * kD + c * 32 + i * 4) =
+                                    make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        }
+                    }
+                    if (row && whole && a.lse) a.lse[token * a.n_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+                    if (row && !whole) {
+                        part[r] = m;
+                        part[kTileRows2 + r] = l;
+                    }
+                }
+            } else {
+                turn = (turn + p.b1 - p.b0) % kBadRing;
+            }
+            if (!whole) {
+                __threadfence();
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (threadIdx.x == 0) {
+                    const int c0 = cta_of(line, p.u0), c1 = cta_of(line, p.u0 + p.n - 1);
+                    int* count = reinterpret_cast<int*>(a.workspace) + c0;
+                    s_last = atomicAdd(count, 1) == c1 - c0;
+                    if (s_last) *count = 0;
+                    __threadfence();
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (s_last) join_parts<T, kTileRows2, kD, 256>(a, ge, line, w, p, threadIdx.x);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && s_gave_up) flag(a.c, BAD_WAIT);
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <class T, int kD>
+cudaError_t launch_tiles(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int sms, cudaStream_t s) {
+    auto* kernel = k_attention_tiles<T, kD>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<kD>::kSmem);
+    if (e != cudaSuccess) return e;
+    kernel<<<sms, kTileThreads, TileShape<kD>::kSmem, s>>>(a, km, vm);
+    return cudaGetLastError();
+}
+
 template <class T, int kD>
 cudaError_t launch_by_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int sms, cudaStream_t s) {
     const long long rows = (long long)a.max_tokens * (a.n_heads / a.c.n_kv);
     if (rows <= 16) return launch_rows<T, kD, 1, 1>(a, km, vm, sms, s);
     if (rows <= 32) return launch_rows<T, kD, 2, 1>(a, km, vm, sms, s);
-    return launch_rows<T, kD, 2, 2>(a, km, vm, sms, s);
+    if (rows <= 64) return launch_rows<T, kD, 2, 2>(a, km, vm, sms, s);
+    return launch_tiles<T, kD>(a, km, vm, sms, s);
 }
 
 // One of the cache's two maps: dims (dim, row of the page, KV head, page), boxes

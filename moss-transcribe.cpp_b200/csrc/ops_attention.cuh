@@ -68,6 +68,62 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
                  : "memory");
 }
 
+// ---- tensor memory and its products --------------------------------------------------------------------------------
+
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// The barrier gets one arrival when all products that this thread has issued are done.
+__device__ __forceinline__ void tc_commit(uint64_t* b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+
+// 32 lanes (the warp's quarter), consecutive columns: a thread has one row.
+template <int kAt, int kN>
+__device__ __forceinline__ void tmem_ld32(float (&x)[kN], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=f"(x[kAt + 0]), "=f"(x[kAt + 1]), "=f"(x[kAt + 2]), "=f"(x[kAt + 3]), "=f"(x[kAt + 4]), "=f"(x[kAt + 5]), "=f"(x[kAt + 6]), "=f"(x[kAt + 7]), "=f"(x[kAt + 8]), "=f"(x[kAt + 9]), "=f"(x[kAt + 10]), "=f"(x[kAt + 11]), "=f"(x[kAt + 12]), "=f"(x[kAt + 13]), "=f"(x[kAt + 14]), "=f"(x[kAt + 15]), "=f"(x[kAt + 16]), "=f"(x[kAt + 17]), "=f"(x[kAt + 18]), "=f"(x[kAt + 19]), "=f"(x[kAt + 20]), "=f"(x[kAt + 21]), "=f"(x[kAt + 22]), "=f"(x[kAt + 23]), "=f"(x[kAt + 24]), "=f"(x[kAt + 25]), "=f"(x[kAt + 26]), "=f"(x[kAt + 27]), "=f"(x[kAt + 28]), "=f"(x[kAt + 29]), "=f"(x[kAt + 30]), "=f"(x[kAt + 31])
+                 : "r"(at));
+}
+template <int kAt, int kN>
+__device__ __forceinline__ void tmem_st32(uint32_t at, const float (&x)[kN]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+                 ::"r"(at), "f"(x[kAt + 0]), "f"(x[kAt + 1]), "f"(x[kAt + 2]), "f"(x[kAt + 3]), "f"(x[kAt + 4]), "f"(x[kAt + 5]), "f"(x[kAt + 6]), "f"(x[kAt + 7]), "f"(x[kAt + 8]), "f"(x[kAt + 9]), "f"(x[kAt + 10]), "f"(x[kAt + 11]), "f"(x[kAt + 12]), "f"(x[kAt + 13]), "f"(x[kAt + 14]), "f"(x[kAt + 15]), "f"(x[kAt + 16]), "f"(x[kAt + 17]), "f"(x[kAt + 18]), "f"(x[kAt + 19]), "f"(x[kAt + 20]), "f"(x[kAt + 21]), "f"(x[kAt + 22]), "f"(x[kAt + 23]), "f"(x[kAt + 24]), "f"(x[kAt + 25]), "f"(x[kAt + 26]), "f"(x[kAt + 27]), "f"(x[kAt + 28]), "f"(x[kAt + 29]), "f"(x[kAt + 30]), "f"(x[kAt + 31])
+                 : "memory");
+}
+template <int kAt, int kN>
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&x)[kN]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(at), "r"(x[kAt + 0]), "r"(x[kAt + 1]), "r"(x[kAt + 2]), "r"(x[kAt + 3]), "r"(x[kAt + 4]), "r"(x[kAt + 5]), "r"(x[kAt + 6]), "r"(x[kAt + 7]), "r"(x[kAt + 8]), "r"(x[kAt + 9]), "r"(x[kAt + 10]), "r"(x[kAt + 11]), "r"(x[kAt + 12]), "r"(x[kAt + 13]), "r"(x[kAt + 14]), "r"(x[kAt + 15])
+                 : "memory");
+}
+
+// Operand tiles of [dims / 64][rows][64 dims], 128-byte swizzle, 1024-byte aligned.
+// K-major (products over the dims): 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_k(uint32_t at) {
+    return (uint64_t)((at >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// MN-major (products over the rows): 64-dim parts `part` bytes apart, 8-row groups 1024.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t at, uint32_t part) {
+    return (uint64_t)((at >> 4) & 0x3FFF) | ((uint64_t)(part >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// f32 sums of 16-bit products, 128 rows x n columns.
+__device__ __forceinline__ constexpr uint32_t tc_instr(bool bf16, int n, bool b_mn) {
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add)
+                 : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t instr, bool add) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+                 ::"r"(d), "r"(a), "l"(b), "r"(instr), "r"((uint32_t)add)
+                 : "memory");
+}
+
 // ---- the line of units ---------------------------------------------------------------------------------------------
 
 struct SeqWork {
