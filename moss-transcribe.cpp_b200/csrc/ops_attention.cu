@@ -113,10 +113,10 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM>::kThreads, 1)
         s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const Line line = find_line<S::kThreads>(a, ge, kRowsMinUnits, s_scan);
+    const Line line = find_line<S::kThreads, CutRows>(a, ge, kRowsMinUnits, s_scan);
     __syncthreads();
     if (line.lo >= line.hi) return;
-    Walk walk(a, ge, line);
+    Walk<CutRows> walk(a, ge, line);
     Part p;
 
     if (warp == 4 * WM) {
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM>::kThreads, 1)
         while (walk.next(&p)) {
             for (int b0 = p.b0; b0 < p.b1; b0 += 32) {
                 int mine = 0;
-                const SeqWork w = seq_work(a, ge, p.seq);
+                const SeqWork w = seq_work(a, p.seq);
                 if (b0 + lane < p.b1) mine = (b0 + lane) * kPage < w.len ? page_of(a.c, p.seq, b0 + lane) : -1;
                 for (int b = b0; b < min(p.b1, b0 + 32); ++b) {
                     const int page = __shfl_sync(0xffffffffu, mine, b - b0);
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM>::kThreads, 1)
     int st = 0;
     unsigned phase = 0;
     while (walk.next(&p)) {
-        const SeqWork w = seq_work(a, ge, p.seq);
+        const SeqWork w = seq_work(a, p.seq);
         const int base = w.len - w.n_new;  // the first new token's slot
         bool ok = true;
         // The groups share q's place: both are through with the last tile's.
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const Line line = find_line<kTileThreads>(a, ge, kTilesMinUnits, s_scan);
+    const Line line = find_line<kTileThreads, CutRows>(a, ge, kTilesMinUnits, s_scan);
     __syncthreads();
     if (line.lo >= line.hi) return;
     if (warp == 8) {
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;  // S of the halves at 0 and 128, O at 256 and 384
-    Walk walk(a, ge, line);
+    Walk<CutRows> walk(a, ge, line);
     Part p;
 
     if (warp >= 8) {
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         int e = 0, round = 0, turn = 0;
         bool ok = true;
         while (ok && walk.next(&p)) {
-            const SeqWork w = seq_work(a, ge, p.seq);
+            const SeqWork w = seq_work(a, p.seq);
             for (int b0 = p.b0; ok && b0 < p.b1; b0 += 16) {
                 // 32 pages, one a lane; no page there: the box past the pool, which reads as 0.
                 const int at = b0 * 2 + lane;
@@ -562,7 +562,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
         };
         while (ok && walk.next(&p)) {
-            const SeqWork w = seq_work(a, ge, p.seq);
+            const SeqWork w = seq_work(a, p.seq);
             const int halves = w.n_new * ge.G - p.tile * kTileRows2 > 128 ? 2 : 1;
             for (int h = 0; ok && h < halves; ++h) {
                 ok = bar_wait(&q_full[h], q_phase[h], &s_gave_up);
@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         unsigned s_phase = 0, o_phase = 0;
         int turn = 0;
         while (walk.next(&p)) {
-            const SeqWork w = seq_work(a, ge, p.seq);
+            const SeqWork w = seq_work(a, p.seq);
             const int base = w.len - w.n_new;
             const bool mine = half == 0 || w.n_new * ge.G - p.tile * kTileRows2 > 128;
             bool ok = true;
@@ -802,6 +802,463 @@ cudaError_t launch_tiles(const AttnArgs& a, const CUtensorMap& km, const CUtenso
     return cudaGetLastError();
 }
 
+// ---- weights, few rows ---------------------------------------------------------------------------------------------
+//
+// weight[slot] += sum over rows exp2(s - lse log2 e), s formed again: K is read
+// a second time (from L2 as far as it still lies there), V is not.  As above, each of
+// four warps takes 16 slots of a page; a thread adds its rows' probabilities of
+// its columns, and eight lanes' sums make a slot's.  All rows of a (sequence, KV head)
+// pass over the part's pages 64 at a time, so nothing is joined between CTAs.
+constexpr int kWRows = 64;
+constexpr int kWThreads = 160;
+
+template <int kD>
+struct WRowsShape {
+    static constexpr int kStage = (kD / 64) * kPage * 128;
+    static constexpr int kQ = kWRows * kD * 2;
+    static constexpr int kStages = 8;
+    static constexpr int kSmem = 1024 + kStages * kStage + kQ;
+};
+
+template <class T, int kD>
+__global__ void __launch_bounds__(kWThreads, 1) k_weights_rows(const AttnArgs a, const __grid_constant__ CUtensorMap k_map) {
+    using S = WRowsShape<kD>;
+    constexpr int kParts = kD / 64, kHalf = kPage * 128;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t full[S::kStages], empty[S::kStages];
+    __shared__ int s_page[S::kStages];
+    __shared__ long long s_scan[16];
+    __shared__ float s_lse[kWRows];
+    __shared__ int s_gave_up;
+    const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;
+    uint8_t* q_at = smem_raw + (ring - smem_u32(smem_raw)) + S::kStages * S::kStage;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Geometry ge{a.n_heads / a.c.n_kv, kWRows, kPage};
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::kStages; ++i) {
+            bar_init(&full[i], 1);
+            bar_init(&empty[i], 4);
+        }
+        s_gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    const Line line = find_line<kWThreads, CutPages>(a, ge, kRowsMinUnits, s_scan);
+    __syncthreads();
+    if (line.lo >= line.hi) return;
+    Walk<CutPages> walk(a, ge, line);
+    Part p;
+    if (warp == 4) {
+        int st = 0, round = 0;
+        bool ok = true;
+        while (ok && walk.next(&p)) {
+            const SeqWork w = seq_work(a, p.seq);
+            for (int r0 = 0; ok && r0 < w.n_new * ge.G; r0 += kWRows)
+                for (int b0 = p.b0; ok && b0 < p.b1; b0 += 32) {
+                    const int mine = b0 + lane < p.b1 ? page_of(a.c, p.seq, b0 + lane) : -1;
+                    for (int b = b0; b < min(p.b1, b0 + 32); ++b) {
+                        const int page = __shfl_sync(0xffffffffu, mine, b - b0);
+                        if (round > 0 && !bar_wait(&empty[st], (round - 1) & 1, &s_gave_up)) {
+                            ok = false;
+                            break;
+                        }
+                        if (lane == 0) {
+                            s_page[st] = page;
+                            if (page < 0) {
+                                bar_arrive(&full[st]);
+                            } else {
+                                bar_expect(&full[st], S::kStage);
+#pragma unroll
+                                for (int h = 0; h < kParts; ++h)
+                                    tma_load_4d(ring + st * S::kStage + h * kHalf, &k_map, h * 64, 0, p.head, page, &full[st]);
+                            }
+                        }
+                        __syncwarp();
+                        if (++st == S::kStages) st = 0, ++round;
+                    }
+                }
+        }
+        for (int i = 0; i < S::kStages; ++i) {
+            const int fills = round + (i < st ? 1 : 0);
+            volatile int none = 0;
+            if (fills > 0) bar_wait(&full[i], (fills - 1) & 1, &none);
+        }
+        if (s_gave_up) flag(a.c, BAD_WAIT);
+        return;
+    }
+    const float to_log2 = a.scale * kLog2e;
+    int st = 0;
+    unsigned phase = 0;
+    while (walk.next(&p)) {
+        const SeqWork w = seq_work(a, p.seq);
+        const int base = w.len - w.n_new, rows = w.n_new * ge.G;
+        bool ok = true;
+        for (int r0 = 0; r0 < rows; r0 += kWRows) {
+            const Part rp{p.seq, p.head, r0 / kWRows, 0, 0, 0, 0};
+            asm volatile("bar.sync 1, 128;" ::: "memory");  // all are through with the last rows
+            for (int i = threadIdx.x; i < kWRows * (kD / 8); i += 128) {
+                const int r = i / (kD / 8), ch = i % (kD / 8);
+                long long token;
+                int head;
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (row_place(a, ge, w, rp, r, &token, &head))
+                    x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + token * a.q_stride + (long long)head * kD + ch * 8);
+                *reinterpret_cast<uint4*>(q_at + (ch / 8) * (kWRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) * 16)) = x;
+            }
+            if (threadIdx.x < kWRows) {
+                long long token;
+                int head;
+                float x = INFINITY;  // exp2(s - inf) = 0: no row, or one that sees nothing
+                if (row_place(a, ge, w, rp, threadIdx.x, &token, &head)) {
+                    x = a.lse[token * a.n_heads + head] * kLog2e;
+                    if (x == -INFINITY) x = INFINITY;
+                }
+                s_lse[threadIdx.x] = x;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            const uint32_t qa = smem_u32(q_at);
+            const int tiles = (min(rows - r0, kWRows) + 15) / 16;
+            for (int b = p.b0; b < p.b1 && ok; ++b) {
+                if (!bar_wait(&full[st], phase, &s_gave_up)) {
+                    ok = false;
+                    break;
+                }
+                const int s0 = b * kPage + warp * 16, page = s_page[st];
+                if (page >= 0 && s0 < w.len) {
+                    const uint32_t kb = ring + st * S::kStage;
+                    uint32_t kf[kD / 16][4];
+#pragma unroll
+                    for (int kk = 0; kk < kD / 16; ++kk) {
+                        const int slot = warp * 16 + ((lane >> 4) << 3) + (lane & 7), ch = kk * 2 + ((lane >> 3) & 1);
+                        ldsm4(kf[kk], kb + (ch / 8) * kHalf + slot * 128 + (((ch & 7) ^ (slot & 7)) * 16));
+                    }
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    for (int mt = 0; mt < tiles; ++mt) {
+                        float s[2][4];
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+                        for (int kk = 0; kk < kD / 16; ++kk) {
+                            uint32_t qf[4];
+                            const int r = mt * 16 + (lane & 15), qc = kk * 2 + (lane >> 4);
+                            ldsm4(qf, qa + (qc / 8) * (kWRows * 128) + r * 128 + (((qc & 7) ^ (r & 7)) * 16));
+                            mma16<T>(s[0], qf, kf[kk][0], kf[kk][1]);
+                            mma16<T>(s[1], qf, kf[kk][2], kf[kk][3]);
+                        }
+                        const int top = r0 + mt * 16;  // the tile's first row
+                        const bool mask = s0 + 16 > base + top / ge.G + 1 || top + 16 > rows;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int r = mt * 16 + (e >> 1) * 8 + lane / 4;
+                            const float less = s_lse[r];
+                            const int sees = !mask ? INT_MAX : r0 + r < rows ? base + (r0 + r) / ge.G + 1 : 0;
+#pragma unroll
+                            for (int n = 0; n < 2; ++n) {
+                                const float x = exp2_fast(__fmaf_rn(s[n][e], to_log2, -less));
+                                sum[n * 2 + (e & 1)] += s0 + n * 8 + (lane & 3) * 2 + (e & 1) < sees ? x : 0.f;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 4);
+                        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 8);
+                        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 16);
+                    }
+                    if (lane < 4) {
+                        float* at = a.c.weight + ((long long)page * a.c.n_kv + p.head) * kPage + warp * 16;
+                        const float decay = r0 == 0 ? a.decay : 1.f;  // later rows add to what the first ones left
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int off = (i >> 1) * 8 + lane * 2 + (i & 1);
+                            if (s0 + off < w.len) at[off] = decay == 0.f ? sum[i] : __fmaf_rn(decay, at[off], sum[i]);
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) bar_arrive(&empty[st]);
+                if (++st == S::kStages) st = 0, phase ^= 1;
+            }
+        }
+    }
+}
+
+// ---- weights, many rows --------------------------------------------------------------------------------------------
+//
+// S^T = K Q^T: a thread has one slot's scores against 128 rows, so a slot's sum is
+// one thread's.  A tile of 256 slots (two halves of 128, four warps each) stays in
+// shared memory while the rows that see it stream past, 128 / G whole tokens at a time
+// with their log-sums; S is double-buffered in tensor memory, so the products run
+// ahead.  The exponentials bound it: one for each product of 128 dims.
+constexpr int kWTileSlots = 256, kWTileRows = 128;
+constexpr int kWEntries = 2;  // ring of row tiles
+constexpr int kWLse = 4;      // ring of their log-sums
+
+template <int kD>
+struct WTileShape {
+    static constexpr int kPart = 128 * 128;
+    static constexpr int kEntry = (kD / 64) * kPart;
+    static constexpr int kSmem = 1024 + (4 + kWEntries) * kEntry;  // two tiles of slots (the next one arrives early)
+};
+
+template <class T, int kD>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    k_weights_tiles(const AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap q_map) {
+    using S = WTileShape<kD>;
+    constexpr int kParts = kD / 64;
+    constexpr bool kBf16 = !std::is_same<T, __half>::value;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t k_full[2], k_empty[2], q_full[kWEntries], q_empty[kWEntries], l_full[kWLse], l_empty[kWLse], s_full[2][2], s_empty[2][2],
+        drained;
+    __shared__ long long s_scan[16];
+    __shared__ __align__(16) float s_less[kWLse][kWTileRows];  // - lse log2 e
+    __shared__ int s_sees[kWLse][kWTileRows];                  // slots that the row sees
+    __shared__ int s_gave_up;
+    __shared__ uint32_t s_tmem;
+    const uint32_t k_at = (smem_u32(smem_raw) + 1023) & ~1023u;
+    const uint32_t q_at = k_at + 4 * S::kEntry;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int G = a.n_heads / a.c.n_kv, per = kWTileRows / G, live = per * G;  // tokens and rows of a row tile
+    const Geometry ge{G, kWTileRows, kWTileSlots};
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&k_full[i], 1);
+            bar_init(&k_empty[i], 1);
+            for (int j = 0; j < 2; ++j) {
+                bar_init(&s_full[i][j], 1);
+                bar_init(&s_empty[i][j], 4);
+            }
+        }
+        for (int i = 0; i < kWEntries; ++i) {
+            bar_init(&q_full[i], 1);
+            bar_init(&q_empty[i], 1);
+        }
+        for (int i = 0; i < kWLse; ++i) {
+            bar_init(&l_full[i], 32);
+            bar_init(&l_empty[i], 8);
+        }
+        bar_init(&drained, 1);
+        s_gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // Rows past live are never written by a copy: 0, once.
+    {
+        uint8_t* q = smem_raw + (q_at - smem_u32(smem_raw));
+        for (int i = threadIdx.x; i < kWEntries * S::kEntry / 16; i += kTileThreads) reinterpret_cast<uint4*>(q)[i] = make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    const Line line = find_line<kTileThreads, CutSlots>(a, ge, kTilesMinUnits, s_scan);
+    __syncthreads();
+    if (line.lo >= line.hi) return;
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    Walk<CutSlots, true> walk(a, ge, line);
+    Part p;
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == 9) {
+            // Copies: a tile of slots, then the row tiles that see it.
+            int e = 0, round = 0, kt = 0;
+            bool ok = true;
+            while (ok && walk.next(&p)) {
+                const SeqWork w = seq_work(a, p.seq);
+                const int kb = kt & 1;
+                if (kt >= 2 && !bar_wait(&k_empty[kb], ((kt >> 1) - 1) & 1, &s_gave_up)) break;
+                int page = -1;
+                if (lane < 4 && (long long)p.tile * kWTileSlots + lane * kPage < w.len) page = page_of(a.c, p.seq, p.tile * 4 + lane);
+                if (lane == 0) bar_expect(&k_full[kb], 2 * S::kEntry);
+                for (int i = 0; i < 4; ++i) {
+                    const int pg = __shfl_sync(0xffffffffu, page, i);
+                    if (lane == 0)
+#pragma unroll
+                        for (int h = 0; h < kParts; ++h)
+                            tma_load_4d(k_at + (2 * kb + i / 2) * S::kEntry + h * S::kPart + (i % 2) * kPage * 128, &k_map, h * 64, 0, p.head,
+                                        pg < 0 ? a.c.n_pages : pg, &k_full[kb]);
+                }
+                ++kt;
+                const int q0 = CutSlots::first(w, ge, p.tile);
+                for (int b = 0; b < p.n; ++b) {
+                    if (round > 0 && !bar_wait(&q_empty[e], (round - 1) & 1, &s_gave_up)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) {
+                        bar_expect(&q_full[e], live * kD * 2);
+#pragma unroll
+                        for (int h = 0; h < kParts; ++h)
+                            tma_load_3d(q_at + e * S::kEntry + h * S::kPart, &q_map, h * 64, p.head * G, w.tok0 + (q0 + b) * per, &q_full[e]);
+                    }
+                    __syncwarp();
+                    if (++e == kWEntries) e = 0, ++round;
+                }
+            }
+            volatile int none = 0;
+            for (int i = 0; i < kWEntries; ++i) {
+                const int fills = round + (i < e ? 1 : 0);
+                if (fills > 0) bar_wait(&q_full[i], (fills - 1) & 1, &none);
+            }
+            for (int i = 0; i < 2; ++i) {
+                const int fills = (kt + 1 - i) / 2;
+                if (fills > 0) bar_wait(&k_full[i], (fills - 1) & 1, &none);
+            }
+        } else if (warp == 10) {
+            // The row tiles' log-sums and limits.
+            int e = 0, round = 0;
+            bool ok = true;
+            while (ok && walk.next(&p)) {
+                const SeqWork w = seq_work(a, p.seq);
+                const int q0 = CutSlots::first(w, ge, p.tile), base = w.len - w.n_new;
+                for (int b = 0; b < p.n; ++b) {
+                    if (round > 0 && !bar_wait(&l_empty[e], (round - 1) & 1, &s_gave_up)) {
+                        ok = false;
+                        break;
+                    }
+#pragma unroll
+                    for (int i = 0; i < kWTileRows / 32; ++i) {
+                        const int r = i * 32 + lane, tok = (q0 + b) * per + r / G;
+                        float less = 0.f;
+                        int sees = 0;
+                        if (r < live && tok < w.n_new) {
+                            less = -a.lse[(long long)(w.tok0 + tok) * a.n_heads + p.head * G + r % G] * kLog2e;
+                            sees = base + tok + 1;
+                        }
+                        s_less[e][r] = less;
+                        s_sees[e][r] = sees;
+                    }
+                    bar_arrive(&l_full[e]);
+                    if (++e == kWLse) e = 0, ++round;
+                }
+            }
+        } else if (warp == 8) {
+            constexpr uint32_t kInstr = tc_instr(kBf16, kWTileRows, false);
+            int e = 0, kt = 0, buf = 0;
+            unsigned phase = 0, s_phase = 1;  // the first wait for an empty S passes
+            bool ok = true;
+            while (ok && walk.next(&p)) {
+                const int kb = kt & 1;
+                if (!bar_wait(&k_full[kb], (kt >> 1) & 1, &s_gave_up)) break;
+                for (int b = 0; ok && b < p.n; ++b) {
+                    ok = bar_wait(&q_full[e], phase, &s_gave_up);
+                    for (int h = 0; ok && h < 2; ++h) {
+                        ok = bar_wait(&s_empty[h][buf], s_phase, &s_gave_up);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (lane == 0) {
+                            const uint32_t ka = k_at + (2 * kb + h) * S::kEntry, qb = q_at + e * S::kEntry;
+#pragma unroll
+                            for (int kk = 0; kk < kD / 16; ++kk) {
+                                const uint32_t off = (kk / 4) * S::kPart + (kk % 4) * 32;
+                                tc_mma_ss(tmem + (h * 2 + buf) * 128, desc_k(ka + off), desc_k(qb + off), kInstr, kk > 0);
+                            }
+                            tc_commit(&s_full[h][buf]);
+                        }
+                    }
+                    if (!ok) break;
+                    if (lane == 0) tc_commit(&q_empty[e]);
+                    if (++e == kWEntries) e = 0, phase ^= 1;
+                    buf ^= 1;
+                    if (buf == 0) s_phase ^= 1;
+                }
+                if (ok && lane == 0) tc_commit(&k_empty[kb]);
+                ++kt;
+            }
+            volatile int none = 0;
+            if (lane == 0) tc_commit(&drained);
+            __syncwarp();
+            bar_wait(&drained, 0, &none);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kHalfRegs));
+        const int half = warp >> 2;
+        const uint32_t t_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 256;
+        const float to_log2 = a.scale * kLog2e;
+        const float2 by = make_float2(to_log2, to_log2);
+        int e = 0, buf = 0;
+        unsigned phase = 0, s_phase = 0;
+        bool ok = true;
+        while (walk.next(&p)) {
+            const SeqWork w = seq_work(a, p.seq);
+            const int q0 = CutSlots::first(w, ge, p.tile);
+            const int h0 = p.tile * kWTileSlots + half * 128, slot = h0 + (warp & 3) * 32 + lane;
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            for (int b = 0; ok && b < p.n; ++b) {
+                ok = bar_wait(&s_full[half][buf], s_phase, &s_gave_up) && bar_wait(&l_full[e], phase, &s_gave_up);
+                if (!ok) break;
+                tc_fence_after();
+                const int t0 = (q0 + b) * per;
+                // Some row is none, or does not see all of the half's slots.
+                const bool mask = live < kWTileRows || t0 + per > w.n_new || h0 + 128 > w.len - w.n_new + t0 + 1;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float s[32];
+                    tmem_ld32<0>(s, t_s + buf * 128 + c * 32);
+                    tmem_wait_ld();
+                    if (c == 3) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(&s_empty[half][buf]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float4 less = *reinterpret_cast<const float4*>(&s_less[e][c * 32 + i * 4]);
+                        float2 x = __ffma2_rn(make_float2(s[4 * i], s[4 * i + 1]), by, make_float2(less.x, less.y));
+                        float2 y = __ffma2_rn(make_float2(s[4 * i + 2], s[4 * i + 3]), by, make_float2(less.z, less.w));
+                        if (mask) {
+                            const int4 sees = *reinterpret_cast<const int4*>(&s_sees[e][c * 32 + i * 4]);
+                            x.x = slot < sees.x ? x.x : -INFINITY;
+                            x.y = slot < sees.y ? x.y : -INFINITY;
+                            y.x = slot < sees.z ? y.x : -INFINITY;
+                            y.y = slot < sees.w ? y.y : -INFINITY;
+                        }
+                        sum[0] = __fadd2_rn(sum[0], make_float2(exp2_fast(x.x), exp2_fast(x.y)));
+                        sum[1] = __fadd2_rn(sum[1], make_float2(exp2_fast(y.x), exp2_fast(y.y)));
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) bar_arrive(&l_empty[e]);
+                if (++e == kWLse) e = 0, phase ^= 1;
+                buf ^= 1;
+                if (buf == 0) s_phase ^= 1;
+            }
+            if (ok && slot < w.len) {
+                const int page = page_of(a.c, p.seq, slot / kPage);
+                if (page >= 0) {
+                    float* at = a.c.weight + ((long long)page * a.c.n_kv + p.head) * kPage + slot % kPage;
+                    const float x = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                    *at = a.decay == 0.f ? x : __fmaf_rn(a.decay, *at, x);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && s_gave_up) flag(a.c, BAD_WAIT);
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <class T, int kD>
+cudaError_t launch_weights(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& qm, int sms, cudaStream_t s) {
+    const long long rows = (long long)a.max_tokens * (a.n_heads / a.c.n_kv);
+    cudaError_t e;
+    if (rows <= kWRows) {
+        auto* kernel = k_weights_rows<T, kD>;
+        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WRowsShape<kD>::kSmem)) != cudaSuccess) return e;
+        kernel<<<sms, kWThreads, WRowsShape<kD>::kSmem, s>>>(a, km);
+    } else {
+        auto* kernel = k_weights_tiles<T, kD>;
+        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WTileShape<kD>::kSmem)) != cudaSuccess) return e;
+        kernel<<<sms, kTileThreads, WTileShape<kD>::kSmem, s>>>(a, km, qm);
+    }
+    return cudaGetLastError();
+}
+
 template <class T, int kD>
 cudaError_t launch_by_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int sms, cudaStream_t s) {
     const long long rows = (long long)a.max_tokens * (a.n_heads / a.c.n_kv);
@@ -811,27 +1268,38 @@ cudaError_t launch_by_rows(const AttnArgs& a, const CUtensorMap& km, const CUten
     return launch_tiles<T, kD>(a, km, vm, sms, s);
 }
 
-// One of the cache's two maps: dims (dim, row of the page, KV head, page), boxes
-// of 64 dims x 64 rows.
-bool encode_map(CUtensorMap* map, const PagedView& c, void* base) {
-    using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static const EncodeFn encode = [] {
-        void* fn = nullptr;
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+bool encode(CUtensorMap* map, int type, int rank, void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+    static const EncodeFn fn = [] {
+        void* f = nullptr;
         cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            fn = nullptr;
-        return reinterpret_cast<EncodeFn>(fn);
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeFn>(f);
     }();
-    if (!encode) return false;
+    const cuuint32_t steps[4] = {1, 1, 1, 1};
+    return fn && fn(map, type == OP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, base, dims, strides, box, steps,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// K or V: (dim, row of the page, KV head, page) in boxes of 64 dims x 64 rows.
+bool encode_cache(CUtensorMap* map, const PagedView& c, void* base) {
     const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, kPage, (cuuint64_t)c.n_kv, (cuuint64_t)c.n_pages};
     const cuuint64_t strides[3] = {(cuuint64_t)c.head_dim * 2, (cuuint64_t)c.head_stride * 2, (cuuint64_t)c.page_stride * 2};
-    const cuuint32_t box[4] = {64, kPage, 1, 1}, steps[4] = {1, 1, 1, 1};
-    return encode(map, c.type == OP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, box,
-                  steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint32_t box[4] = {64, kPage, 1, 1};
+    return encode(map, c.type, 4, base, dims, strides, box);
+}
+
+// q: (dim, head, token) in boxes of 64 dims x one KV head's group x as many whole tokens as 128 rows hold.
+bool encode_q(CUtensorMap* map, const AttnArgs& a) {
+    const int G = a.n_heads / a.c.n_kv;
+    const cuuint64_t dims[3] = {(cuuint64_t)a.c.head_dim, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.c.head_dim * 2, (cuuint64_t)a.q_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(kWTileRows / G)};
+    return encode(map, a.c.type, 3, const_cast<char*>(a.q), dims, strides, box);
 }
 
 int sm_count() {
@@ -840,53 +1308,28 @@ int sm_count() {
     return std::min(n, kMaxSms);
 }
 
-// One CTA of 64 threads per (sequence, KV head, page): a thread owns a slot.
-template <class T>
-__global__ void __launch_bounds__(kPage) k_weights_simple(AttnArgs a, int pages) {
-    __shared__ float s_q[128];
-    const PagedView& c = a.c;
-    const int seq = blockIdx.x / pages, p = blockIdx.x % pages, g = blockIdx.y, D = c.head_dim, G = a.n_heads / c.n_kv;
-    const int2 tok = seq_tokens(c, a.cu, a.n_tokens, seq);
-    const int len = seq_len(c, seq);
-    if (tok.y == 0 || p * kPage >= len) return;
-    const int page = page_of(c, seq, p);
-    if (page < 0) return;
-    const int slot = p * kPage + threadIdx.x;
-    const T* k = reinterpret_cast<const T*>(c.k) + page * c.page_stride + g * c.head_stride + (long long)threadIdx.x * D;
-    float w = 0.f;
-    for (int i = max(0, p * kPage - (len - tok.y)); i < tok.y; ++i)
-        for (int h = g * G; h < (g + 1) * G; ++h) {
-            __syncthreads();
-            const T* q = reinterpret_cast<const T*>(a.q) + (tok.x + i) * a.q_stride + (long long)h * D;
-            for (int d = threadIdx.x; d < D; d += kPage) s_q[d] = to_f32<T>(q[d]);
-            __syncthreads();
-            if (slot > len - tok.y + i) continue;
-            float s = 0.f;
-            for (int d = 0; d < D; ++d) s = fmaf(s_q[d], to_f32<T>(k[d]), s);
-            w += expf(s * a.scale - a.lse[(long long)(tok.x + i) * a.n_heads + h]);
-        }
-    if (slot < len) {
-        float* at = c.weight + ((long long)page * c.n_kv + g) * kPage + threadIdx.x;
-        *at = a.decay == 0.f ? w : fmaf(a.decay, *at, w);
-    }
-}
-
 }  // namespace
+
+template <class F>
+cudaError_t by_type(const PagedView& c, F&& f) {
+    using D64 = std::integral_constant<int, 64>;
+    using D128 = std::integral_constant<int, 128>;
+    if (c.type == OP_F16) return c.head_dim == 64 ? f(__half(), D64()) : f(__half(), D128());
+    return c.head_dim == 64 ? f(__nv_bfloat16(), D64()) : f(__nv_bfloat16(), D128());
+}
 
 cudaError_t launch_paged_attention(const AttnArgs& a, cudaStream_t s) {
     CUtensorMap km, vm;
     const int sms = sm_count();
-    if (sms == 0 || !encode_map(&km, a.c, a.c.k) || !encode_map(&vm, a.c, a.c.v)) return cudaErrorInvalidValue;
-    if (a.c.type == OP_F16)
-        return a.c.head_dim == 64 ? launch_by_rows<__half, 64>(a, km, vm, sms, s) : launch_by_rows<__half, 128>(a, km, vm, sms, s);
-    return a.c.head_dim == 64 ? launch_by_rows<__nv_bfloat16, 64>(a, km, vm, sms, s) : launch_by_rows<__nv_bfloat16, 128>(a, km, vm, sms, s);
+    if (sms == 0 || !encode_cache(&km, a.c, a.c.k) || !encode_cache(&vm, a.c, a.c.v)) return cudaErrorInvalidValue;
+    return by_type(a.c, [&](auto t, auto d) { return launch_by_rows<decltype(t), decltype(d)::value>(a, km, vm, sms, s); });
 }
 
 cudaError_t launch_attention_weights(const AttnArgs& a, cudaStream_t s) {
-    const dim3 grid(a.c.n_seq * a.c.table_stride, a.c.n_kv);
-    if (a.c.type == OP_F16) k_weights_simple<__half><<<grid, kPage, 0, s>>>(a, a.c.table_stride);
-    else k_weights_simple<__nv_bfloat16><<<grid, kPage, 0, s>>>(a, a.c.table_stride);
-    return cudaGetLastError();
+    CUtensorMap km, qm;
+    const int sms = sm_count();
+    if (sms == 0 || !encode_cache(&km, a.c, a.c.k) || !encode_q(&qm, a)) return cudaErrorInvalidValue;
+    return by_type(a.c, [&](auto t, auto d) { return launch_weights<decltype(t), decltype(d)::value>(a, km, qm, sms, s); });
 }
 
 }  // namespace mtb

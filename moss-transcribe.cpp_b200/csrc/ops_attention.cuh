@@ -2,8 +2,8 @@
 // how parts of a row tile are joined, barriers and copies.
 //
 // Rows: the new tokens of a sequence times the query heads of one KV head,
-// row r = (token r / G, head r % G); a tile is kRows consecutive rows.  Units: a
-// tile's visible cache in blocks of kBlock slots (at least one).  All units of
+// row r = (token r / G, head r % G); a tile is some consecutive rows.  Units: a
+// tile's visible cache in blocks of slots (at least one).  All units of
 // all (sequence, KV head, tile) stand in one line, and CTA c of g takes the
 // c-th of g equal intervals of it, whatever the lengths are.  A tile that lies in
 // one interval is finished there.  One that spans several leaves its parts (f32
@@ -68,6 +68,12 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
                  : "memory");
 }
 
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+                 : "memory");
+}
+
 // ---- tensor memory and its products --------------------------------------------------------------------------------
 
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -127,30 +133,49 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
 // ---- the line of units ---------------------------------------------------------------------------------------------
 
 struct SeqWork {
-    int len, tok0, n_new, tiles;
+    int len, tok0, n_new;
 };
 
 struct Geometry {
     int G, rows, block;  // query heads per KV head, rows per tile, slots per block
 };
 
-__device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, const Geometry& ge, int s) {
+__device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int s) {
     const int2 tok = seq_tokens(a.c, a.cu, a.n_tokens, s);
-    SeqWork w{0, tok.x, tok.y, 0};
-    if (tok.y == 0) return w;
-    w.len = seq_len(a.c, s);
-    w.tiles = (tok.y * ge.G + ge.rows - 1) / ge.rows;
+    SeqWork w{0, tok.x, tok.y};
+    if (tok.y) w.len = seq_len(a.c, s);
     return w;
 }
-// Blocks that the rows of a tile see, at least 1.
-__device__ __forceinline__ int tile_blocks(const SeqWork& w, const Geometry& ge, int tile) {
-    const int last = min(w.n_new - 1, ((tile + 1) * ge.rows - 1) / ge.G);
-    const int sees = w.len - w.n_new + last + 1;
-    return max(1, (sees + ge.block - 1) / ge.block);
-}
+
+// How a sequence's work under one KV head is cut: tiles, and units of a tile.
+struct CutRows {  // the attention: tiles of rows, in blocks of the slots that they see, at least one
+    static __device__ __forceinline__ int tiles(const SeqWork& w, const Geometry& ge) { return (w.n_new * ge.G + ge.rows - 1) / ge.rows; }
+    static __device__ __forceinline__ int units(const SeqWork& w, const Geometry& ge, int tile) {
+        const int last = min(w.n_new - 1, ((tile + 1) * ge.rows - 1) / ge.G);
+        return max(1, (w.len - w.n_new + last + ge.block) / ge.block);
+    }
+};
+struct CutPages {  // the weights of few rows: one tile, in blocks of slots
+    static __device__ __forceinline__ int tiles(const SeqWork& w, const Geometry&) { return w.n_new > 0 && w.len > 0; }
+    static __device__ __forceinline__ int units(const SeqWork& w, const Geometry& ge, int) { return (w.len + ge.block - 1) / ge.block; }
+};
+struct CutSlots {  // the weights of many: tiles of slots, in tiles of the new tokens (rows / G each) that see some of them
+    static __device__ __forceinline__ int tiles(const SeqWork& w, const Geometry& ge) {
+        return w.n_new > 0 ? (w.len + ge.block - 1) / ge.block : 0;
+    }
+    static __device__ __forceinline__ int first(const SeqWork& w, const Geometry& ge, int tile) {
+        return max(0, tile * ge.block - (w.len - w.n_new)) / (ge.rows / ge.G);
+    }
+    static __device__ __forceinline__ int units(const SeqWork& w, const Geometry& ge, int tile) {
+        const int per = ge.rows / ge.G;
+        return (w.n_new + per - 1) / per - first(w, ge, tile);
+    }
+};
+template <class Cut>
 __device__ __forceinline__ long long head_units(const SeqWork& w, const Geometry& ge) {
     long long u = 0;
-    for (int t = 0; t < w.tiles; ++t) u += tile_blocks(w, ge, t);
+    const int tiles = Cut::tiles(w, ge);
+    for (int t = 0; t < tiles; ++t) u += Cut::units(w, ge, t);
     return u;
 }
 
@@ -163,15 +188,15 @@ struct Line {
 };
 
 // All threads of the CTA; s_scan: one long long a warp + 4.
-template <int kThreads>
+template <int kThreads, class Cut>
 __device__ Line find_line(const AttnArgs& a, const Geometry& ge, int min_units, long long* s_scan) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     constexpr int kWarps = kThreads / 32;
     long long mine = 0, sum = 0;
     for (int s = threadIdx.x; s < a.c.n_seq; s += kThreads) {
-        const SeqWork w = seq_work(a, ge, s);
+        const SeqWork w = seq_work(a, s);
         if (w.n_new > w.len && blockIdx.x == 0) flag(a.c, BAD_LEN);
-        mine = head_units(w, ge) * a.c.n_kv;
+        mine = head_units<Cut>(w, ge) * a.c.n_kv;
         sum += mine;
     }
 #pragma unroll
@@ -190,7 +215,7 @@ __device__ Line find_line(const AttnArgs& a, const Geometry& ge, int min_units, 
     long long base = 0;
     for (int s0 = 0; s0 < a.c.n_seq; s0 += kThreads) {
         const int s = s0 + threadIdx.x;
-        long long v = a.c.n_seq <= kThreads ? mine : s < a.c.n_seq ? head_units(seq_work(a, ge, s), ge) * a.c.n_kv : 0;
+        long long v = a.c.n_seq <= kThreads ? mine : s < a.c.n_seq ? head_units<Cut>(seq_work(a, s), ge) * a.c.n_kv : 0;
         if (s >= a.c.n_seq) v = 0;
         long long x = v;
 #pragma unroll
@@ -225,51 +250,57 @@ struct Part {
     long long u0;  // the tile's first unit
 };
 
-// Walks the CTA's interval; every role of the CTA walks it by itself.
+// Walks the CTA's interval; every role of the CTA walks it by itself.  Whole: a
+// tile goes undivided to the interval that holds its first unit.
+template <class Cut, bool kWhole = false>
 struct Walk {
     const AttnArgs& a;
     const Geometry ge;
     long long at, hi;  // next unit, end of the interval
     SeqWork w{};
-    int seq, head = 0, tile = 0, block = 0;
+    int seq, head = 0, tile = 0, block = 0, tiles = 0;
 
     __device__ Walk(const AttnArgs& args, const Geometry& g, const Line& l) : a(args), ge(g), at(l.lo), hi(l.hi), seq(l.seq) {
         if (at >= hi) return;
-        w = seq_work(a, ge, seq);
-        const long long per = head_units(w, ge);
+        w = seq_work(a, seq);
+        tiles = Cut::tiles(w, ge);
+        const long long per = head_units<Cut>(w, ge);
         long long off = l.off % per;
         head = (int)(l.off / per);
         for (;;) {
-            const int n = tile_blocks(w, ge, tile);
+            const int n = Cut::units(w, ge, tile);
             if (off < n) break;
             off -= n;
             ++tile;
         }
         block = (int)off;
+        if (kWhole && block > 0) {
+            at += Cut::units(w, ge, tile) - block;
+            step();
+        }
+    }
+    __device__ void step() {
+        block = 0;
+        if (++tile < tiles) return;
+        tile = 0;
+        if (++head < a.c.n_kv) return;
+        head = 0;
+        while (at < hi) {
+            w = seq_work(a, ++seq);
+            tiles = Cut::tiles(w, ge);
+            if (tiles > 0) break;
+        }
     }
     __device__ bool next(Part* p) {
         if (at >= hi) return false;
-        const int n = tile_blocks(w, ge, tile);
-        const int take = (int)min((long long)(n - block), hi - at);
+        const int n = Cut::units(w, ge, tile);
+        const int take = kWhole ? n : (int)min((long long)(n - block), hi - at);
         *p = Part{seq, head, tile, block, block + take, n, at - block};
         at += take;
         block += take;
-        if (block == n) {
-            block = 0;
-            if (++tile == w.tiles) {
-                tile = 0;
-                if (++head == a.c.n_kv) {
-                    head = 0;
-                    if (at < hi) {
-                        do w = seq_work(a, ge, ++seq);
-                        while (w.n_new == 0);
-                    }
-                }
-            }
-        }
+        if (block == n) step();
         return true;
     }
-    // The sequence of the part that next() returned last may differ from w.
 };
 
 // ---- parts in the workspace ----------------------------------------------------------------------------------------
