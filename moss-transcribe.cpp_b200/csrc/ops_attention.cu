@@ -39,6 +39,40 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+bool encode(CUtensorMap* map, int type, int rank, void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+    static const EncodeFn fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeFn>(f);
+    }();
+    const cuuint32_t steps[4] = {1, 1, 1, 1};
+    return fn && fn(map, type == OP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, base, dims, strides, box, steps,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// K or V: (dim, row of the page, KV head, page) in boxes of 64 dims x 64 rows.
+bool encode_cache(CUtensorMap* map, const PagedView& c, void* base) {
+    const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, kPage, (cuuint64_t)c.n_kv, (cuuint64_t)c.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.head_dim * 2, (cuuint64_t)c.head_stride * 2, (cuuint64_t)c.page_stride * 2};
+    const cuuint32_t box[4] = {64, kPage, 1, 1};
+    return encode(map, c.type, 4, base, dims, strides, box);
+}
+
+// q: (dim, head, token) in boxes of 64 dims x one KV head's group x as many whole tokens as 128 rows hold.
+bool encode_q(CUtensorMap* map, const AttnArgs& a) {
+    const int G = a.n_heads / a.c.n_kv;
+    const cuuint64_t dims[3] = {(cuuint64_t)a.c.head_dim, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.c.head_dim * 2, (cuuint64_t)a.q_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(128 / G)};
+    return encode(map, a.c.type, 3, const_cast<char*>(a.q), dims, strides, box);
+}
+
 // ---- few rows ------------------------------------------------------------------------------------------------------
 //
 // A step or a verify pass: a tile of 16, 32 or 64 rows, so each K and V byte
@@ -46,11 +80,12 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
 // walks its interval of 64-slot pages; a producer warp brings a page's K and V
 // (TMA boxes of 64 slots x 64 dims, 128-byte swizzle: the ldmatrix reads below
 // are free of bank conflicts) into a ring of as many pages as shared memory
-// holds, across tile borders.  Each of four warps takes 16 of the page's 64
+// holds, across tile borders.  Each of four warps takes 16 of a page's 64
 // slots, with a maximum, sum and f32 result of its own (m16n8k16, scores stay in
 // registers as the second product's operand), so that no page costs a barrier among them;
-// the four are joined when the tile's part ends.  64 rows: two such groups of
-// four warps, 32 rows each.
+// they are joined when the tile's part ends.  Up to 32 rows two such sets of
+// four warps take the pages in turn (a page is a chain of dependent steps, two
+// chains fill each other's gaps); 64 rows are two sets of 32 on the same page.
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -73,33 +108,40 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&d)[4], const uint32
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// MW: 16-row tiles of a warp; WM: groups of four warps.
-template <int kD, int MW, int WM>
+// MW: 16-row tiles of a warp; WM: sets of four warps by rows; WP: by pages.
+template <int kD, int MW, int WM, int WP>
 struct RowsShape {
     static constexpr int kRows = 16 * MW * WM;
-    static constexpr int kThreads = (4 * WM + 1) * 32;
+    static constexpr int kWarps = 4 * WM * WP;                 // consumers
+    static constexpr int kThreads = (kWarps + 1) * 32;
     static constexpr int kHalf = kPage * 128;                  // bytes of 64 slots x 64 dims
     static constexpr int kStage = 2 * (kD / 64) * kHalf;       // a page's K, then its V
     static constexpr int kQ = kRows * kD * 2;
     static constexpr int kPad = kD + 8;                        // floats of a joined row: no two rows on the same banks
-    static constexpr int kJoin = 2 * kRows * kPad * 4;
-    static constexpr int kRoom = 227 * 1024 - 1024 - 4096;     // alignment, static
+    static constexpr int kBufs = 2 * WP;                       // half of the warps that share a row
+    static constexpr int kJoin = kBufs * kRows * kPad * 4;
+    static constexpr int kRoom = 227 * 1024 - 1024 - 6144;     // alignment, static
     static constexpr int kFit = (kRoom - kQ - kJoin) / kStage;
-    static constexpr int kStages = kFit > 12 ? 12 : kFit;
+    // A stage always falls to the same set of warps: each waits for every fill
+    // of its stages, or a barrier's parity would say nothing.
+    static constexpr int kStages = (kFit > 12 ? 12 : kFit) / WP * WP;
     static constexpr int kSmem = 1024 + kStages * kStage + kQ + kJoin;
 };
+constexpr int kPartRing = 8;
 
-template <class T, int kD, int MW, int WM>
-__global__ void __launch_bounds__(RowsShape<kD, MW, WM>::kThreads, 1)
+template <class T, int kD, int MW, int WM, int WP>
+__global__ void __launch_bounds__(RowsShape<kD, MW, WM, WP>::kThreads, 1)
     k_attention_rows(const AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
-    using S = RowsShape<kD, MW, WM>;
-    constexpr int kParts = kD / 64;  // 64-dim halves of a row
+    using S = RowsShape<kD, MW, WM, WP>;
+    constexpr int kParts = kD / 64;  // 64-dim parts of a row
+    constexpr int kSplit = 4 * WP;   // warps that share a row
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full[S::kStages], empty[S::kStages];
-    __shared__ int s_page[S::kStages];          // the stage's page, negative: masked
+    __shared__ uint64_t full[S::kStages], empty[S::kStages], all_bar;
+    __shared__ PartRing<kPartRing> parts;
+    __shared__ int s_page[S::kStages];  // the stage's page, negative: masked
     __shared__ long long s_scan[16];
-    __shared__ float s_m[WM][4][16 * MW], s_l[WM][4][16 * MW];
-    __shared__ int s_gave_up, s_last, s_go;
+    __shared__ float s_m[WM][kSplit][16 * MW], s_l[WM][kSplit][16 * MW];
+    __shared__ int s_gave_up, s_last;
     const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;
     uint8_t* q_at = smem_raw + (ring - smem_u32(smem_raw)) + S::kStages * S::kStage;
     float* join = reinterpret_cast<float*>(q_at + S::kQ);
@@ -110,26 +152,34 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM>::kThreads, 1)
             bar_init(&full[i], 1);
             bar_init(&empty[i], 4 * WM);
         }
+        bar_init(&all_bar, S::kWarps * 32);
+        parts.init(S::kWarps);
         s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     const Line line = find_line<S::kThreads, CutRows>(a, ge, kRowsMinUnits, s_scan);
     __syncthreads();
     if (line.lo >= line.hi) return;
-    Walk<CutRows> walk(a, ge, line);
     Part p;
 
-    if (warp == 4 * WM) {
+    if (warp == S::kWarps) {
         // Producer: table entries 32 at a time, one a lane.
+        Walk<CutRows> walk(a, ge, line);
         int st = 0, round = 0;
-        while (walk.next(&p)) {
-            for (int b0 = p.b0; b0 < p.b1; b0 += 32) {
-                int mine = 0;
-                const SeqWork w = seq_work(a, p.seq);
-                if (b0 + lane < p.b1) mine = (b0 + lane) * kPage < w.len ? page_of(a.c, p.seq, b0 + lane) : -1;
+        unsigned turn = 0;
+        bool ok = true;
+        while (ok && walk.next(&p)) {
+            if (!parts.put(turn, p, &s_gave_up)) break;
+            ++turn;
+            for (int b0 = p.b0; ok && b0 < p.b1; b0 += 32) {
+                int mine = -1;
+                if (b0 + lane < p.b1 && (long long)(b0 + lane) * kPage < p.len) mine = page_of(a.c, p.seq, b0 + lane);
                 for (int b = b0; b < min(p.b1, b0 + 32); ++b) {
                     const int page = __shfl_sync(0xffffffffu, mine, b - b0);
-                    if (round > 0 && !bar_wait(&empty[st], (round - 1) & 1, &s_gave_up)) goto drained;
+                    if (round > 0 && !bar_wait(&empty[st], (round - 1) & 1, &s_gave_up)) {
+                        ok = false;
+                        break;
+                    }
                     if (lane == 0) {
                         s_page[st] = page;
                         if (page < 0) {
@@ -138,10 +188,11 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM>::kThreads, 1)
                             bar_expect(&full[st], S::kStage);
                             const uint32_t dst = ring + st * S::kStage;
 #pragma unroll
-                            for (int h = 0; h < kParts; ++h) {
+                            for (int h = 0; h < kParts; ++h)
                                 tma_load_4d(dst + h * S::kHalf, &k_map, h * 64, 0, p.head, page, &full[st]);
+#pragma unroll
+                            for (int h = 0; h < kParts; ++h)
                                 tma_load_4d(dst + (kParts + h) * S::kHalf, &v_map, h * 64, 0, p.head, page, &full[st]);
-                            }
                         }
                     }
                     __syncwarp();
@@ -149,60 +200,53 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM>::kThreads, 1)
                 }
             }
         }
-    drained:
+        p.n = 0;
+        parts.put(turn, p, &s_gave_up);
         // No copy is left in flight when the CTA ends: each stage's last fill has landed.
         for (int i = 0; i < S::kStages; ++i) {
             const int fills = round + (i < st ? 1 : 0);
-            if (fills > 0) {
-                volatile int none = 0;
-                bar_wait(&full[i], (fills - 1) & 1, &none);
-            }
+            volatile int none = 0;
+            if (fills > 0) bar_wait(&full[i], (fills - 1) & 1, &none);
         }
-        if (s_gave_up) flag(a.c, BAD_WAIT);
+        if (lane == 0 && s_gave_up) flag(a.c, BAD_WAIT);
         return;
     }
 
-    const int group = warp >> 2, sw = warp & 3;
-    const int tid = threadIdx.x;                   // of the 128 WM consumers
-    const int gt = tid - group * 128;              // of the group's 128
+    const int wp = warp / (4 * WM), group = (warp / 4) % WM, sw = warp & 3;
+    const int share = wp * 4 + sw;                 // of the warps that share its rows
+    const int tid = threadIdx.x;                   // of the consumers
     const float to_log2 = a.scale * kLog2e;
-    int st = 0;
+    SyncPoint all{&all_bar, 0, &s_gave_up};
+    int st = 0, mine = 0;                          // mine: whose turn the stage is
     unsigned phase = 0;
-    while (walk.next(&p)) {
-        const SeqWork w = seq_work(a, p.seq);
-        const int base = w.len - w.n_new;  // the first new token's slot
+    for (unsigned turn = 0; parts.get(turn, &p, &s_gave_up); ++turn) {
+        const int base = p.len - p.n_new;  // the first new token's slot
+        const int rows = min(S::kRows, p.n_new * ge.G - p.tile * S::kRows);
         bool ok = true;
-        // The groups share q's place: both are through with the last tile's.
-        if (WM > 1) asm volatile("bar.sync 3, %0;" ::"n"(128 * WM) : "memory");
-        if (tid == 0) s_go = !s_gave_up;
         // The tile's q rows, swizzled like K; rows that are none are 0.
-        for (int i = tid; i < S::kRows * (kD / 8); i += 128 * WM) {
+        for (int i = tid; i < S::kRows * (kD / 8); i += S::kWarps * 32) {
             const int r = i / (kD / 8), ch = i % (kD / 8);
             long long token;
             int head;
             uint4 x = make_uint4(0, 0, 0, 0);
-            if (row_place(a, ge, w, p, r, &token, &head))
+            if (r < rows && row_place(ge, p, r, &token, &head))
                 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + token * a.q_stride + (long long)head * kD + ch * 8);
             *reinterpret_cast<uint4*>(q_at + (ch / 8) * (S::kRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) * 16)) = x;
         }
-        asm volatile("bar.sync 3, %0;" ::"n"(128 * WM) : "memory");
-        if (!s_go) break;  // the same for all of them: none waits at a barrier that another has left
-        const uint32_t qa = smem_u32(q_at);
-        // Slots that row r of the tile sees: [0, base + token(r) + 1).
+        // Slots that the thread's rows see: [0, base + token(r) + 1); least, most: of the warp's rows.
         int sees[MW][2];
-        int least = INT_MAX, most = 0;
 #pragma unroll
         for (int mt = 0; mt < MW; ++mt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int r = p.tile * S::kRows + group * 16 * MW + mt * 16 + e * 8 + lane / 4;
-                sees[mt][e] = r < w.n_new * ge.G ? base + r / ge.G + 1 : 0;
+                const int r = group * 16 * MW + mt * 16 + e * 8 + lane / 4;
+                sees[mt][e] = r < rows ? base + (p.tile * S::kRows + r) / ge.G + 1 : 0;
             }
-        {
-            const int r0 = p.tile * S::kRows + group * 16 * MW, r1 = min(r0 + 16 * MW, w.n_new * ge.G) - 1;
-            least = r0 + 16 * MW <= w.n_new * ge.G ? base + r0 / ge.G + 1 : 0;
-            most = r1 >= r0 ? base + r1 / ge.G + 1 : 0;
-        }
+        const int r0 = group * 16 * MW, r1 = min(r0 + 16 * MW, rows) - 1;
+        const int least = r1 == r0 + 16 * MW - 1 ? base + (p.tile * S::kRows + r0) / ge.G + 1 : 0;
+        const int most = r1 >= r0 ? base + (p.tile * S::kRows + r1) / ge.G + 1 : 0;
+        all.sync();
+        const uint32_t qa = smem_u32(q_at);
         uint32_t q[MW == 1 ? kD / 16 : 1][4];
         if constexpr (MW == 1) {
 #pragma unroll
@@ -222,13 +266,19 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM>::kThreads, 1)
             l[mt][0] = l[mt][1] = 0.f;
         }
         for (int b = p.b0; b < p.b1; ++b) {
-            if (!bar_wait(&full[st], phase, &s_gave_up)) {
+            const bool here = mine == wp;
+            const int at = st;
+            const unsigned parity = phase;
+            if (++st == S::kStages) st = 0, phase ^= 1;
+            if (++mine == WP) mine = 0;
+            if (!here) continue;
+            if (!bar_wait(&full[at], parity, &s_gave_up)) {
                 ok = false;
                 break;
             }
             const int s0 = b * kPage + sw * 16;  // the warp's first slot
-            if (s_page[st] >= 0 && s0 < most) {
-                const uint32_t kb = ring + st * S::kStage, vb = kb + kParts * S::kHalf;
+            if (s_page[at] >= 0 && s0 < most) {
+                const uint32_t kb = ring + at * S::kStage, vb = kb + kParts * S::kHalf;
                 float s[MW][2][4];
 #pragma unroll
                 for (int mt = 0; mt < MW; ++mt)
@@ -303,12 +353,12 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM>::kThreads, 1)
                     }
                 }
                 // V at or behind the sequence's end may hold anything: 0 there, since 0 * NaN is NaN.
-                const bool tail = s0 + 16 > w.len;
+                const bool tail = s0 + 16 > p.len;
                 uint32_t lo_on = 0xffffffffu, hi_on = 0xffffffffu;
                 if (tail) {
                     const int first = s0 + (lane & 3) * 2;
-                    lo_on = (first < w.len ? 0xffffu : 0u) | (first + 1 < w.len ? 0xffff0000u : 0u);
-                    hi_on = (first + 8 < w.len ? 0xffffu : 0u) | (first + 9 < w.len ? 0xffff0000u : 0u);
+                    lo_on = (first < p.len ? 0xffffu : 0u) | (first + 1 < p.len ? 0xffff0000u : 0u);
+                    hi_on = (first + 8 < p.len ? 0xffffu : 0u) | (first + 9 < p.len ? 0xffff0000u : 0u);
                 }
 #pragma unroll
                 for (int nd = 0; nd < kD / 16; ++nd) {
@@ -329,10 +379,9 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM>::kThreads, 1)
                 }
             }
             __syncwarp();
-            if (lane == 0) bar_arrive(&empty[st]);
-            if (++st == S::kStages) st = 0, phase ^= 1;
+            if (lane == 0) bar_arrive(&empty[at]);
         }
-        // The group's four warps joined: maxima, then the scaled results in two buffers.
+        // The warps that share a row joined: maxima, then the scaled results, half of them stored, half added.
 #pragma unroll
         for (int mt = 0; mt < MW; ++mt)
 #pragma unroll
@@ -340,55 +389,64 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM>::kThreads, 1)
                 l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 1);
                 l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 2);
                 if ((lane & 3) == 0) {
-                    s_m[group][sw][mt * 16 + e * 8 + lane / 4] = m[mt][e];
-                    s_l[group][sw][mt * 16 + e * 8 + lane / 4] = l[mt][e];
+                    s_m[group][share][mt * 16 + e * 8 + lane / 4] = m[mt][e];
+                    s_l[group][share][mt * 16 + e * 8 + lane / 4] = l[mt][e];
                 }
             }
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
-        float* buf = join + ((sw & 1) * S::kRows + group * 16 * MW) * S::kPad;
+        all.sync();
+        float* buf = join + ((share % S::kBufs) * S::kRows + group * 16 * MW) * S::kPad;
 #pragma unroll
-        for (int turn = 0; turn < 2; ++turn) {  // warps 2 and 3 store, then 0 and 1 add theirs
-            if ((sw < 2) == (turn == 1)) {
+        for (int add = 0; add < 2; ++add) {
+            if ((share < S::kBufs) == (add == 1)) {
 #pragma unroll
                 for (int mt = 0; mt < MW; ++mt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int r = mt * 16 + e * 8 + lane / 4;
-                        const float top = fmaxf(fmaxf(s_m[group][0][r], s_m[group][1][r]), fmaxf(s_m[group][2][r], s_m[group][3][r]));
+                        if (group * 16 * MW + r >= rows) continue;
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int x = 0; x < kSplit; ++x) top = fmaxf(top, s_m[group][x][r]);
                         const float f = m[mt][e] == -INFINITY ? 0.f : exp2f(m[mt][e] - top);
 #pragma unroll
                         for (int n = 0; n < kD / 8; ++n) {
-                            float2* at = reinterpret_cast<float2*>(buf + r * S::kPad + n * 8 + (lane & 3) * 2);
+                            float2* to = reinterpret_cast<float2*>(buf + r * S::kPad + n * 8 + (lane & 3) * 2);
                             float2 x = make_float2(o[mt][n][2 * e] * f, o[mt][n][2 * e + 1] * f);
-                            if (turn == 1) {
-                                const float2 y = *at;
+                            if (add == 1) {
+                                const float2 y = *to;
                                 x.x += y.x;
                                 x.y += y.y;
                             }
-                            *at = x;
+                            *to = x;
                         }
                     }
             }
-            asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+            all.sync();
         }
-        const bool whole = p.b0 == 0 && p.b1 == p.n;
+        const bool whole = p.b1 - p.b0 == p.n;
         float* part = whole ? nullptr : part_at<S::kRows, kD>(a, blockIdx.x, p.b0 == 0);
-        for (int i = gt; i < 16 * MW * (kD / 4); i += 128) {
-            const int gr = i / (kD / 4), col = i % (kD / 4) * 4, r = group * 16 * MW + gr;
+        for (int i = tid; ok && i < rows * (kD / 4); i += S::kWarps * 32) {
+            const int r = i / (kD / 4), col = i % (kD / 4) * 4, g = r / (16 * MW), gr = r % (16 * MW);
             float top = -INFINITY, sum = 0.f;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) top = fmaxf(top, s_m[group][x][gr]);
+            for (int x = 0; x < kSplit; ++x) top = fmaxf(top, s_m[g][x][gr]);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const float mx = s_m[group][x][gr];
-                sum += s_l[group][x][gr] * (mx == -INFINITY ? 0.f : exp2f(mx - top));
+            for (int x = 0; x < kSplit; ++x) {
+                const float mx = s_m[g][x][gr];
+                sum += s_l[g][x][gr] * (mx == -INFINITY ? 0.f : exp2f(mx - top));
             }
-            const float4 x = *reinterpret_cast<const float4*>(join + r * S::kPad + col);
-            const float4 y = *reinterpret_cast<const float4*>(join + (S::kRows + r) * S::kPad + col);
-            const float4 z = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+            float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int x = 0; x < S::kBufs; ++x) {
+                const float4 y = *reinterpret_cast<const float4*>(join + (x * S::kRows + r) * S::kPad + col);
+                z.x += y.x;
+                z.y += y.y;
+                z.z += y.z;
+                z.w += y.w;
+            }
             long long token;
             int head;
-            if (!ok || !row_place(a, ge, w, p, r, &token, &head)) continue;
+            row_place(ge, p, r, &token, &head);
             if (whole) {
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
                 store4<T>(reinterpret_cast<T*>(a.out) + token * a.out_stride + (long long)head * kD + col,
@@ -404,25 +462,18 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM>::kThreads, 1)
         }
         if (!whole) {
             __threadfence();
-            asm volatile("bar.sync 3, %0;" ::"n"(128 * WM) : "memory");
-            if (tid == 0) {
-                const int c0 = cta_of(line, p.u0), c1 = cta_of(line, p.u0 + p.n - 1);
-                int* count = reinterpret_cast<int*>(a.workspace) + c0;
-                const int before = atomicAdd(count, 1);
-                s_last = before == c1 - c0;
-                if (s_last) *count = 0;
-                __threadfence();
-            }
-            asm volatile("bar.sync 3, %0;" ::"n"(128 * WM) : "memory");
-            if (s_last) join_parts<T, S::kRows, kD, 128 * WM>(a, ge, line, w, p, tid);
+            all.sync();
+            if (tid == 0) s_last = part_is_last(a, p);
+            all.sync();
+            if (s_last) join_parts<T, S::kRows, kD, S::kWarps * 32>(a, ge, p, tid, all);
         }
     }
 }
 
-template <class T, int kD, int MW, int WM>
+template <class T, int kD, int MW, int WM, int WP>
 cudaError_t launch_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int sms, cudaStream_t s) {
-    using S = RowsShape<kD, MW, WM>;
-    auto* kernel = k_attention_rows<T, kD, MW, WM>;
+    using S = RowsShape<kD, MW, WM, WP>;
+    auto* kernel = k_attention_rows<T, kD, MW, WM, WP>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     if (e != cudaSuccess) return e;
     kernel<<<sms, S::kThreads, S::kSmem, s>>>(a, km, vm);
@@ -442,7 +493,7 @@ cudaError_t launch_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensor
 // free to be rescaled.
 constexpr int kTileRows2 = 256;
 constexpr int kTileBlock = 128;
-constexpr int kTileThreads = 384;  // warps 0-3 and 4-7: the halves; 8: products; 9: copies; 10, 11: none
+constexpr int kTileThreads = 384;  // warps 0-3 and 4-7: the halves; 8: products; 9, 10: copies; 11: none
 // Registers: 168 a thread at launch; a half's threads hold a row of 128 scores,
 // so the other four warps give theirs up: 256 x 224 + 128 x 56 = 384 x 168.
 constexpr int kHalfRegs = 224, kOtherRegs = 56;
@@ -458,33 +509,39 @@ struct TileShape {
 
 template <class T, int kD>
 __global__ void __launch_bounds__(kTileThreads, 1)
-    k_attention_tiles(const AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+    k_attention_tiles(const AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                      const __grid_constant__ CUtensorMap q_map) {
     using S = TileShape<kD>;
     constexpr int kParts = kD / 64;
-    constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+    constexpr bool kBf16 = !std::is_same<T, __half>::value;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full[kTileEntries], empty[kTileEntries], q_full[2], s_full[2], p_full[2], o_full[2], drained;
+    __shared__ uint64_t full[kTileEntries], empty[kTileEntries], q_full[2], q_empty, s_full[2], p_full[2], o_full[2], all_bar, drained;
+    __shared__ PartRing<kPartRing> parts;
     __shared__ long long s_scan[16];
     __shared__ int s_bad[kBadRing];  // bit 0, 1: the block's pages that are masked
     __shared__ int s_gave_up, s_last;
     __shared__ uint32_t s_tmem;
     const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;
     const uint32_t q_at = ring + kTileEntries * S::kEntry;
-    uint8_t* q_ptr = smem_raw + (q_at - smem_u32(smem_raw));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Geometry ge{a.n_heads / a.c.n_kv, kTileRows2, kTileBlock};
+    // A half has as many whole tokens as 128 rows hold.
+    const int G = a.n_heads / a.c.n_kv, per = 128 / G, live = per * G;
+    const Geometry ge{G, 2 * live, kTileBlock};
     if (threadIdx.x == 0) {
         for (int i = 0; i < kTileEntries; ++i) {
             bar_init(&full[i], 1);
             bar_init(&empty[i], 1);
         }
         for (int h = 0; h < 2; ++h) {
-            bar_init(&q_full[h], 128);
+            bar_init(&q_full[h], 1);
             bar_init(&s_full[h], 1);
             bar_init(&p_full[h], 128);
             bar_init(&o_full[h], 1);
         }
+        bar_init(&q_empty, 1);
+        bar_init(&all_bar, 256);
         bar_init(&drained, 1);
+        parts.init(10);
         s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -499,173 +556,179 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;  // S of the halves at 0 and 128, O at 256 and 384
-    Walk<CutRows> walk(a, ge, line);
-    Part p;
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-      if (warp == 9) {
-        int e = 0, round = 0, turn = 0;
-        bool ok = true;
-        while (ok && walk.next(&p)) {
-            const SeqWork w = seq_work(a, p.seq);
-            for (int b0 = p.b0; ok && b0 < p.b1; b0 += 16) {
-                // 32 pages, one a lane; no page there: the box past the pool, which reads as 0.
-                const int at = b0 * 2 + lane;
-                int mine = -1;
-                if (at < p.b1 * 2 && (long long)at * kPage < w.len) mine = page_of(a.c, p.seq, at);
-                for (int b = b0; ok && b < min(p.b1, b0 + 16); ++b) {
-                    const int pg0 = __shfl_sync(0xffffffffu, mine, 2 * (b - b0)), pg1 = __shfl_sync(0xffffffffu, mine, 2 * (b - b0) + 1);
+        Part p;
+        if (warp == 9) {
+            // K and V blocks, in turn.
+            Walk<CutRows> walk(a, ge, line);
+            int e = 0, round = 0, slot = 0;
+            unsigned turn = 0;
+            bool ok = true;
+            while (ok && walk.next(&p)) {
+                if (!parts.put(turn, p, &s_gave_up)) break;
+                ++turn;
+                for (int b0 = p.b0; ok && b0 < p.b1; b0 += 16) {
+                    // 32 pages, one a lane; no page there: the box past the pool, which reads as 0.
+                    const int at = b0 * 2 + lane;
+                    int mine = -1;
+                    if (at < p.b1 * 2 && (long long)at * kPage < p.len) mine = page_of(a.c, p.seq, at);
+                    for (int b = b0; ok && b < min(p.b1, b0 + 16); ++b) {
+                        const int pg0 = __shfl_sync(0xffffffffu, mine, 2 * (b - b0)), pg1 = __shfl_sync(0xffffffffu, mine, 2 * (b - b0) + 1);
 #pragma unroll
-                    for (int kv = 0; kv < 2; ++kv) {
-                        if (round > 0 && !bar_wait(&empty[e], (round - 1) & 1, &s_gave_up)) {
-                            ok = false;
-                            break;
-                        }
-                        if (lane == 0) {
-                            if (kv == 0) s_bad[turn] = (pg0 < 0 ? 1 : 0) | (pg1 < 0 ? 2 : 0);
-                            bar_expect(&full[e], S::kEntry);
-                            const uint32_t dst = ring + e * S::kEntry;
-                            const CUtensorMap* map = kv ? &v_map : &k_map;
-#pragma unroll
-                            for (int h = 0; h < kParts; ++h) {
-                                tma_load_4d(dst + h * S::kPart, map, h * 64, 0, p.head, pg0 < 0 ? a.c.n_pages : pg0, &full[e]);
-                                tma_load_4d(dst + h * S::kPart + kPage * 128, map, h * 64, 0, p.head, pg1 < 0 ? a.c.n_pages : pg1, &full[e]);
+                        for (int kv = 0; kv < 2; ++kv) {
+                            if (round > 0 && !bar_wait(&empty[e], (round - 1) & 1, &s_gave_up)) {
+                                ok = false;
+                                break;
                             }
+                            if (lane == 0) {
+                                if (kv == 0) s_bad[slot] = (pg0 < 0 ? 1 : 0) | (pg1 < 0 ? 2 : 0);
+                                bar_expect(&full[e], S::kEntry);
+                                const uint32_t dst = ring + e * S::kEntry;
+                                const CUtensorMap* map = kv ? &v_map : &k_map;
+#pragma unroll
+                                for (int h = 0; h < kParts; ++h) {
+                                    tma_load_4d(dst + h * S::kPart, map, h * 64, 0, p.head, pg0 < 0 ? a.c.n_pages : pg0, &full[e]);
+                                    tma_load_4d(dst + h * S::kPart + kPage * 128, map, h * 64, 0, p.head, pg1 < 0 ? a.c.n_pages : pg1, &full[e]);
+                                }
+                            }
+                            __syncwarp();
+                            if (++e == kTileEntries) e = 0, ++round;
                         }
-                        __syncwarp();
-                        if (++e == kTileEntries) e = 0, ++round;
+                        slot = (slot + 1) % kBadRing;
                     }
-                    turn = (turn + 1) % kBadRing;
                 }
             }
-        }
-        for (int i = 0; i < kTileEntries; ++i) {  // every copy has landed before the CTA ends
-            const int fills = round + (i < e ? 1 : 0);
-            volatile int none = 0;
-            if (fills > 0) bar_wait(&full[i], (fills - 1) & 1, &none);
-        }
-      } else if (warp == 8) {
-        constexpr uint32_t kQk = tc_instr(kBf16, kTileBlock, false), kPv = tc_instr(kBf16, kD, true);
-        int e = 0;
-        unsigned phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-        bool ok = true;
-        auto qk = [&](int h, int entry) {
-            if (lane == 0) {
-                const uint32_t qa = q_at + h * S::kEntry, kb = ring + entry * S::kEntry;
-#pragma unroll
-                for (int kk = 0; kk < kD / 16; ++kk) {
-                    const uint32_t off = (kk / 4) * S::kPart + (kk % 4) * 32;
-                    tc_mma_ss(tmem + h * 128, desc_k(qa + off), desc_k(kb + off), kQk, kk > 0);
-                }
-                tc_commit(&s_full[h]);
+            p.n = 0;
+            parts.put(turn, p, &s_gave_up);
+            for (int i = 0; i < kTileEntries; ++i) {  // every copy has landed before the CTA ends
+                const int fills = round + (i < e ? 1 : 0);
+                volatile int none = 0;
+                if (fills > 0) bar_wait(&full[i], (fills - 1) & 1, &none);
             }
-        };
-        while (ok && walk.next(&p)) {
-            const SeqWork w = seq_work(a, p.seq);
-            const int halves = w.n_new * ge.G - p.tile * kTileRows2 > 128 ? 2 : 1;
-            for (int h = 0; ok && h < halves; ++h) {
-                ok = bar_wait(&q_full[h], q_phase[h], &s_gave_up);
-                q_phase[h] ^= 1;
-            }
-            if (!ok) break;
-            ok = bar_wait(&full[e], phase, &s_gave_up);
-            if (!ok) break;
-            tc_fence_after();
-            for (int h = 0; h < halves; ++h) qk(h, e);
-            if (lane == 0) tc_commit(&empty[e]);
-            if (++e == kTileEntries) e = 0, phase ^= 1;
-            for (int b = p.b0; ok && b < p.b1; ++b) {
-                const int ve = e;
-                ok = bar_wait(&full[ve], phase, &s_gave_up);
-                if (!ok) break;
-                if (++e == kTileEntries) e = 0, phase ^= 1;
-                if ((b + 1) * kTileBlock > w.len) {
-                    // V at or behind the sequence's end may hold anything: 0 there, since 0 * NaN is NaN.
-                    const int from = max(0, w.len - b * kTileBlock);
-                    uint8_t* v = smem_raw + (ring - smem_u32(smem_raw)) + ve * S::kEntry;
-                    for (int i = lane; i < kParts * (kTileBlock - from) * 8; i += 32) {
-                        const int h = i / ((kTileBlock - from) * 8), j = i % ((kTileBlock - from) * 8);
-                        *reinterpret_cast<uint4*>(v + h * S::kPart + from * 128 + j * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                }
-                const bool more = b + 1 < p.b1;
-                if (more) ok = bar_wait(&full[e], phase, &s_gave_up);
-                for (int h = 0; ok && h < halves; ++h) {
-                    ok = bar_wait(&p_full[h], p_phase[h], &s_gave_up);
-                    if (!ok) break;
-                    p_phase[h] ^= 1;
-                    tc_fence_after();
+        } else if (warp == 10) {
+            // q rows: the next tile's as soon as the last product with this one's is done.
+            int fills[2] = {0, 0};
+            for (unsigned turn = 0; parts.get(turn, &p, &s_gave_up); ++turn) {
+                if (turn > 0 && !bar_wait(&q_empty, (turn - 1) & 1, &s_gave_up)) break;
+                const int halves = p.n_new > (2 * p.tile + 1) * per ? 2 : 1;
+                for (int h = 0; h < halves; ++h) {
                     if (lane == 0) {
-                        const uint32_t vb = ring + ve * S::kEntry;
+                        bar_expect(&q_full[h], live * kD * 2);
 #pragma unroll
-                        for (int kk = 0; kk < kTileBlock / 16; ++kk)
-                            tc_mma_ts(tmem + 256 + h * 128, tmem + h * 128 + kk * 8, desc_mn(vb + kk * 2048, S::kPart), kPv,
-                                      b > p.b0 || kk > 0);
-                        if (!more) tc_commit(&o_full[h]);
+                        for (int i = 0; i < kParts; ++i)
+                            tma_load_3d(q_at + h * S::kEntry + i * S::kPart, &q_map, i * 64, p.head * G, p.tok0 + (2 * p.tile + h) * per, &q_full[h]);
                     }
-                    if (more) qk(h, e);
-                }
-                if (!ok) break;
-                if (lane == 0) tc_commit(&empty[ve]);
-                if (more) {
-                    if (lane == 0) tc_commit(&empty[e]);
-                    if (++e == kTileEntries) e = 0, phase ^= 1;
+                    ++fills[h];
                 }
             }
+            volatile int none = 0;
+            for (int h = 0; h < 2; ++h)
+                if (fills[h] > 0) bar_wait(&q_full[h], (fills[h] - 1) & 1, &none);
+        } else if (warp == 8) {
+            const uint32_t kQk = tc_instr(kBf16, kTileBlock, false) | (a.scale < 0.f ? kNegateA : 0u);
+            constexpr uint32_t kPv = tc_instr(kBf16, kD, true);
+            int e = 0;
+            unsigned phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+            bool ok = true;
+            auto qk = [&](int h, int entry) {
+                if (lane == 0) {
+                    const uint32_t qa = q_at + h * S::kEntry, kb = ring + entry * S::kEntry;
+#pragma unroll
+                    for (int kk = 0; kk < kD / 16; ++kk) {
+                        const uint32_t off = (kk / 4) * S::kPart + (kk % 4) * 32;
+                        tc_mma_ss(tmem + h * 128, desc_k(qa + off), desc_k(kb + off), kQk, kk > 0);
+                    }
+                    tc_commit(&s_full[h]);
+                }
+            };
+            for (unsigned turn = 0; ok && parts.get(turn, &p, &s_gave_up); ++turn) {
+                const int halves = p.n_new > (2 * p.tile + 1) * per ? 2 : 1;
+                for (int h = 0; ok && h < halves; ++h) {
+                    ok = bar_wait(&q_full[h], q_phase[h], &s_gave_up);
+                    q_phase[h] ^= 1;
+                }
+                ok = ok && bar_wait(&full[e], phase, &s_gave_up);
+                if (!ok) break;
+                tc_fence_after();
+                for (int h = 0; h < halves; ++h) qk(h, e);
+                if (lane == 0) {
+                    tc_commit(&empty[e]);
+                    if (p.b1 - p.b0 == 1) tc_commit(&q_empty);
+                }
+                if (++e == kTileEntries) e = 0, phase ^= 1;
+                for (int b = p.b0; ok && b < p.b1; ++b) {
+                    const int ve = e;
+                    ok = bar_wait(&full[ve], phase, &s_gave_up);
+                    if (!ok) break;
+                    if (++e == kTileEntries) e = 0, phase ^= 1;
+                    if ((b + 1) * kTileBlock > p.len) {
+                        // V at or behind the sequence's end may hold anything: 0 there, since 0 * NaN is NaN.
+                        const int from = max(0, p.len - b * kTileBlock);
+                        uint8_t* v = smem_raw + (ring - smem_u32(smem_raw)) + ve * S::kEntry;
+                        for (int i = lane; i < kParts * (kTileBlock - from) * 8; i += 32) {
+                            const int h = i / ((kTileBlock - from) * 8), j = i % ((kTileBlock - from) * 8);
+                            *reinterpret_cast<uint4*>(v + h * S::kPart + from * 128 + j * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+                    const bool more = b + 1 < p.b1;
+                    if (more) ok = bar_wait(&full[e], phase, &s_gave_up);
+                    for (int h = 0; ok && h < halves; ++h) {
+                        ok = bar_wait(&p_full[h], p_phase[h], &s_gave_up);
+                        if (!ok) break;
+                        p_phase[h] ^= 1;
+                        tc_fence_after();
+                        if (lane == 0) {
+                            const uint32_t vb = ring + ve * S::kEntry;
+#pragma unroll
+                            for (int kk = 0; kk < kTileBlock / 16; ++kk)
+                                tc_mma_ts(tmem + 256 + h * 128, tmem + h * 128 + kk * 8, desc_mn(vb + kk * 2048, S::kPart), kPv,
+                                          b > p.b0 || kk > 0);
+                            if (!more) tc_commit(&o_full[h]);
+                        }
+                        if (more) qk(h, e);
+                    }
+                    if (!ok) break;
+                    if (lane == 0) tc_commit(&empty[ve]);
+                    if (more) {
+                        if (lane == 0) {
+                            tc_commit(&empty[e]);
+                            if (b + 2 == p.b1) tc_commit(&q_empty);
+                        }
+                        if (++e == kTileEntries) e = 0, phase ^= 1;
+                    }
+                }
+            }
+            // Nothing that was issued is left running.
+            volatile int none = 0;
+            if (lane == 0) tc_commit(&drained);
+            __syncwarp();
+            bar_wait(&drained, 0, &none);
         }
-        // Nothing that was issued is left running.
-        volatile int none = 0;
-        if (lane == 0) tc_commit(&drained);
-        __syncwarp();
-        bar_wait(&drained, 0, &none);
-      }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kHalfRegs));
-        const int half = warp >> 2, r = half * 128 + (warp & 3) * 32 + lane;
+        const int half = warp >> 2, in_half = (warp & 3) * 32 + lane;
+        const int r = in_half < live ? half * live + in_half : kTileRows2;  // the tile's row, or none
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_s = tmem + lanes + half * 128, t_o = tmem + lanes + 256 + half * 128;
         const float to_log2 = fmaxf(fabsf(a.scale), 1e-37f) * kLog2e;  // above 0: a masked -inf stays -inf
-        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // a negative scale turns q's sign: maxima stay maxima
+        SyncPoint all{&all_bar, 0, &s_gave_up};
         unsigned s_phase = 0, o_phase = 0;
-        int turn = 0;
-        while (walk.next(&p)) {
-            const SeqWork w = seq_work(a, p.seq);
-            const int base = w.len - w.n_new;
-            const bool mine = half == 0 || w.n_new * ge.G - p.tile * kTileRows2 > 128;
-            bool ok = true;
-            float m = -INFINITY, l = 0.f;
-            long long token = 0;
-            int head = 0;
-            const bool row = row_place(a, ge, w, p, r, &token, &head);
-            const bool whole = p.b0 == 0 && p.b1 == p.n;
+        int slot = 0;
+        Part p;
+        for (unsigned turn = 0; parts.get(turn, &p, &s_gave_up); ++turn) {
+            const int base = p.len - p.n_new;
+            const bool mine = half == 0 || p.n_new > (2 * p.tile + 1) * per;
+            const bool whole = p.b1 - p.b0 == p.n;
             if (mine) {
-                // The half's q rows, swizzled; rows that are none are 0.
-                const int t = threadIdx.x & 127;
-#pragma unroll 4
-                for (int i = t; i < 128 * (kD / 8); i += 128) {
-                    const int rr = i / (kD / 8), ch = i % (kD / 8);
-                    long long tk;
-                    int hd;
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (row_place(a, ge, w, p, half * 128 + rr, &tk, &hd)) {
-                        x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + tk * a.q_stride + (long long)hd * kD + ch * 8);
-                        x.x ^= flip;
-                        x.y ^= flip;
-                        x.z ^= flip;
-                        x.w ^= flip;
-                    }
-                    *reinterpret_cast<uint4*>(q_ptr + half * S::kEntry + (ch / 8) * S::kPart + rr * 128 + (((ch & 7) ^ (rr & 7)) * 16)) = x;
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                tc_fence_before();
-                bar_arrive(&q_full[half]);
-                const int sees = row ? base + (p.tile * kTileRows2 + r) / ge.G + 1 : 0;
-                // Slots that every row of the half sees.
-                const int r0 = p.tile * kTileRows2 + half * 128;
-                const int least = r0 + 128 <= w.n_new * ge.G ? base + r0 / ge.G + 1 : 0;
+                bool ok = true;
+                float m = -INFINITY, l = 0.f;
+                const int first = (2 * p.tile + half) * per;  // the half's first token
+                const int sees = min(first + in_half / G, p.n_new - 1) + base + 1;
+                const int least = first + base + 1;           // slots that every row of the half sees
                 for (int b = p.b0; b < p.b1; ++b) {
                     if (!bar_wait(&s_full[half], s_phase, &s_gave_up)) {
                         ok = false;
@@ -679,8 +742,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     tmem_ld32<64>(s, t_s + 64);
                     tmem_ld32<96>(s, t_s + 96);
                     tmem_wait_ld();
-                    const int bad = s_bad[turn];
-                    turn = (turn + 1) % kBadRing;
+                    const int bad = s_bad[slot];
+                    slot = (slot + 1) % kBadRing;
                     const int s0 = b * kTileBlock;
                     if (s0 + kTileBlock > least) {
 #pragma unroll
@@ -694,9 +757,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                     float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
+                    for (int i = 4; i < 128; i += 8)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            top[j] = i + 4 + j < 128 ? fmaxf(fmaxf(top[j], s[i + j]), s[i + 4 + j]) : fmaxf(top[j], s[i + j]);
                     top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                    const float reach = top[0] == -INFINITY ? -INFINITY : top[0] * to_log2;
+                    const float reach = top[0] * to_log2;
                     if (__any_sync(0xffffffffu, reach > m + 8.f)) {
                         const float to = fmaxf(m, reach);
                         const float f = to == -INFINITY ? 1.f : exp2_fast(m - to);
@@ -739,6 +805,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 if (ok && bar_wait(&o_full[half], o_phase, &s_gave_up)) {
                     o_phase ^= 1;
                     tc_fence_after();
+                    long long token = 0;
+                    int head = 0;
+                    const bool row = row_place(ge, p, r, &token, &head);
                     float* part = whole ? nullptr : part_at<kTileRows2, kD>(a, blockIdx.x, p.b0 == 0);
                     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
@@ -770,20 +839,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                 }
             } else {
-                turn = (turn + p.b1 - p.b0) % kBadRing;
+                slot = (slot + p.b1 - p.b0) % kBadRing;
             }
             if (!whole) {
                 __threadfence();
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (threadIdx.x == 0) {
-                    const int c0 = cta_of(line, p.u0), c1 = cta_of(line, p.u0 + p.n - 1);
-                    int* count = reinterpret_cast<int*>(a.workspace) + c0;
-                    s_last = atomicAdd(count, 1) == c1 - c0;
-                    if (s_last) *count = 0;
-                    __threadfence();
-                }
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (s_last) join_parts<T, kTileRows2, kD, 256>(a, ge, line, w, p, threadIdx.x);
+                all.sync();
+                if (threadIdx.x == 0) s_last = part_is_last(a, p);
+                all.sync();
+                if (s_last) join_parts<T, kTileRows2, kD, 256>(a, ge, p, threadIdx.x, all);
             }
         }
     }
@@ -795,10 +858,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
 template <class T, int kD>
 cudaError_t launch_tiles(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int sms, cudaStream_t s) {
+    CUtensorMap qm;
+    if (!encode_q(&qm, a)) return cudaErrorInvalidValue;
     auto* kernel = k_attention_tiles<T, kD>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<kD>::kSmem);
     if (e != cudaSuccess) return e;
-    kernel<<<sms, kTileThreads, TileShape<kD>::kSmem, s>>>(a, km, vm);
+    kernel<<<sms, kTileThreads, TileShape<kD>::kSmem, s>>>(a, km, vm, qm);
     return cudaGetLastError();
 }
 
@@ -825,7 +890,8 @@ __global__ void __launch_bounds__(kWThreads, 1) k_weights_rows(const AttnArgs a,
     using S = WRowsShape<kD>;
     constexpr int kParts = kD / 64, kHalf = kPage * 128;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full[S::kStages], empty[S::kStages];
+    __shared__ uint64_t full[S::kStages], empty[S::kStages], all_bar;
+    __shared__ PartRing<kPartRing> parts;
     __shared__ int s_page[S::kStages];
     __shared__ long long s_scan[16];
     __shared__ float s_lse[kWRows];
@@ -839,20 +905,24 @@ __global__ void __launch_bounds__(kWThreads, 1) k_weights_rows(const AttnArgs a,
             bar_init(&full[i], 1);
             bar_init(&empty[i], 4);
         }
+        bar_init(&all_bar, 128);
+        parts.init(4);
         s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     const Line line = find_line<kWThreads, CutPages>(a, ge, kRowsMinUnits, s_scan);
     __syncthreads();
     if (line.lo >= line.hi) return;
-    Walk<CutPages> walk(a, ge, line);
     Part p;
     if (warp == 4) {
+        Walk<CutPages> walk(a, ge, line);
         int st = 0, round = 0;
+        unsigned turn = 0;
         bool ok = true;
         while (ok && walk.next(&p)) {
-            const SeqWork w = seq_work(a, p.seq);
-            for (int r0 = 0; ok && r0 < w.n_new * ge.G; r0 += kWRows)
+            if (!parts.put(turn, p, &s_gave_up)) break;
+            ++turn;
+            for (int r0 = 0; ok && r0 < p.n_new * ge.G; r0 += kWRows)
                 for (int b0 = p.b0; ok && b0 < p.b1; b0 += 32) {
                     const int mine = b0 + lane < p.b1 ? page_of(a.c, p.seq, b0 + lane) : -1;
                     for (int b = b0; b < min(p.b1, b0 + 32); ++b) {
@@ -877,30 +947,32 @@ __global__ void __launch_bounds__(kWThreads, 1) k_weights_rows(const AttnArgs a,
                     }
                 }
         }
+        p.n = 0;
+        parts.put(turn, p, &s_gave_up);
         for (int i = 0; i < S::kStages; ++i) {
             const int fills = round + (i < st ? 1 : 0);
             volatile int none = 0;
             if (fills > 0) bar_wait(&full[i], (fills - 1) & 1, &none);
         }
-        if (s_gave_up) flag(a.c, BAD_WAIT);
+        if (lane == 0 && s_gave_up) flag(a.c, BAD_WAIT);
         return;
     }
     const float to_log2 = a.scale * kLog2e;
     int st = 0;
     unsigned phase = 0;
-    while (walk.next(&p)) {
-        const SeqWork w = seq_work(a, p.seq);
-        const int base = w.len - w.n_new, rows = w.n_new * ge.G;
+    SyncPoint all{&all_bar, 0, &s_gave_up};
+    for (unsigned turn = 0; parts.get(turn, &p, &s_gave_up); ++turn) {
+        const int base = p.len - p.n_new, rows = p.n_new * ge.G;
         bool ok = true;
         for (int r0 = 0; r0 < rows; r0 += kWRows) {
-            const Part rp{p.seq, p.head, r0 / kWRows, 0, 0, 0, 0};
-            asm volatile("bar.sync 1, 128;" ::: "memory");  // all are through with the last rows
+            p.tile = r0 / kWRows;  // row_place() below goes by it
+            all.sync();            // all are through with the last rows
             for (int i = threadIdx.x; i < kWRows * (kD / 8); i += 128) {
                 const int r = i / (kD / 8), ch = i % (kD / 8);
                 long long token;
                 int head;
                 uint4 x = make_uint4(0, 0, 0, 0);
-                if (row_place(a, ge, w, rp, r, &token, &head))
+                if (row_place(ge, p, r, &token, &head))
                     x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + token * a.q_stride + (long long)head * kD + ch * 8);
                 *reinterpret_cast<uint4*>(q_at + (ch / 8) * (kWRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) * 16)) = x;
             }
@@ -908,13 +980,13 @@ __global__ void __launch_bounds__(kWThreads, 1) k_weights_rows(const AttnArgs a,
                 long long token;
                 int head;
                 float x = INFINITY;  // exp2(s - inf) = 0: no row, or one that sees nothing
-                if (row_place(a, ge, w, rp, threadIdx.x, &token, &head)) {
+                if (row_place(ge, p, threadIdx.x, &token, &head)) {
                     x = a.lse[token * a.n_heads + head] * kLog2e;
                     if (x == -INFINITY) x = INFINITY;
                 }
                 s_lse[threadIdx.x] = x;
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            all.sync();
             const uint32_t qa = smem_u32(q_at);
             const int tiles = (min(rows - r0, kWRows) + 15) / 16;
             for (int b = p.b0; b < p.b1 && ok; ++b) {
@@ -923,7 +995,7 @@ __global__ void __launch_bounds__(kWThreads, 1) k_weights_rows(const AttnArgs a,
                     break;
                 }
                 const int s0 = b * kPage + warp * 16, page = s_page[st];
-                if (page >= 0 && s0 < w.len) {
+                if (page >= 0 && s0 < p.len) {
                     const uint32_t kb = ring + st * S::kStage;
                     uint32_t kf[kD / 16][4];
 #pragma unroll
@@ -972,7 +1044,7 @@ __global__ void __launch_bounds__(kWThreads, 1) k_weights_rows(const AttnArgs a,
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int off = (i >> 1) * 8 + lane * 2 + (i & 1);
-                            if (s0 + off < w.len) at[off] = decay == 0.f ? sum[i] : __fmaf_rn(decay, at[off], sum[i]);
+                            if (s0 + off < p.len) at[off] = decay == 0.f ? sum[i] : __fmaf_rn(decay, at[off], sum[i]);
                         }
                     }
                 }
@@ -1011,6 +1083,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t k_full[2], k_empty[2], q_full[kWEntries], q_empty[kWEntries], l_full[kWLse], l_empty[kWLse], s_full[2][2], s_empty[2][2],
         drained;
+    __shared__ PartRing<kPartRing> parts;
     __shared__ long long s_scan[16];
     __shared__ __align__(16) float s_less[kWLse][kWTileRows];  // - lse log2 e
     __shared__ int s_sees[kWLse][kWTileRows];                  // slots that the row sees
@@ -1039,6 +1112,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             bar_init(&l_empty[i], 8);
         }
         bar_init(&drained, 1);
+        parts.init(10);
         s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -1059,20 +1133,22 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    Walk<CutSlots, true> walk(a, ge, line);
     Part p;
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == 9) {
             // Copies: a tile of slots, then the row tiles that see it.
+            Walk<CutSlots, true> walk(a, ge, line);
             int e = 0, round = 0, kt = 0;
+            unsigned turn = 0;
             bool ok = true;
             while (ok && walk.next(&p)) {
-                const SeqWork w = seq_work(a, p.seq);
+                if (!parts.put(turn, p, &s_gave_up)) break;
+                ++turn;
                 const int kb = kt & 1;
                 if (kt >= 2 && !bar_wait(&k_empty[kb], ((kt >> 1) - 1) & 1, &s_gave_up)) break;
                 int page = -1;
-                if (lane < 4 && (long long)p.tile * kWTileSlots + lane * kPage < w.len) page = page_of(a.c, p.seq, p.tile * 4 + lane);
+                if (lane < 4 && (long long)p.tile * kWTileSlots + lane * kPage < p.len) page = page_of(a.c, p.seq, p.tile * 4 + lane);
                 if (lane == 0) bar_expect(&k_full[kb], 2 * S::kEntry);
                 for (int i = 0; i < 4; ++i) {
                     const int pg = __shfl_sync(0xffffffffu, page, i);
@@ -1083,7 +1159,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                         pg < 0 ? a.c.n_pages : pg, &k_full[kb]);
                 }
                 ++kt;
-                const int q0 = CutSlots::first(w, ge, p.tile);
+                const int q0 = CutSlots::first(SeqWork{p.len, 0, p.n_new}, ge, p.tile);
                 for (int b = 0; b < p.n; ++b) {
                     if (round > 0 && !bar_wait(&q_empty[e], (round - 1) & 1, &s_gave_up)) {
                         ok = false;
@@ -1093,12 +1169,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         bar_expect(&q_full[e], live * kD * 2);
 #pragma unroll
                         for (int h = 0; h < kParts; ++h)
-                            tma_load_3d(q_at + e * S::kEntry + h * S::kPart, &q_map, h * 64, p.head * G, w.tok0 + (q0 + b) * per, &q_full[e]);
+                            tma_load_3d(q_at + e * S::kEntry + h * S::kPart, &q_map, h * 64, p.head * G, p.tok0 + (q0 + b) * per, &q_full[e]);
                     }
                     __syncwarp();
                     if (++e == kWEntries) e = 0, ++round;
                 }
             }
+            p.n = 0;
+            parts.put(turn, p, &s_gave_up);
             volatile int none = 0;
             for (int i = 0; i < kWEntries; ++i) {
                 const int fills = round + (i < e ? 1 : 0);
@@ -1112,9 +1190,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             // The row tiles' log-sums and limits.
             int e = 0, round = 0;
             bool ok = true;
-            while (ok && walk.next(&p)) {
-                const SeqWork w = seq_work(a, p.seq);
-                const int q0 = CutSlots::first(w, ge, p.tile), base = w.len - w.n_new;
+            for (unsigned turn = 0; ok && parts.get(turn, &p, &s_gave_up); ++turn) {
+                const int q0 = CutSlots::first(SeqWork{p.len, 0, p.n_new}, ge, p.tile), base = p.len - p.n_new;
                 for (int b = 0; b < p.n; ++b) {
                     if (round > 0 && !bar_wait(&l_empty[e], (round - 1) & 1, &s_gave_up)) {
                         ok = false;
@@ -1125,8 +1202,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         const int r = i * 32 + lane, tok = (q0 + b) * per + r / G;
                         float less = 0.f;
                         int sees = 0;
-                        if (r < live && tok < w.n_new) {
-                            less = -a.lse[(long long)(w.tok0 + tok) * a.n_heads + p.head * G + r % G] * kLog2e;
+                        if (r < live && tok < p.n_new) {
+                            less = -a.lse[(long long)(p.tok0 + tok) * a.n_heads + p.head * G + r % G] * kLog2e;
                             sees = base + tok + 1;
                         }
                         s_less[e][r] = less;
@@ -1141,7 +1218,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             int e = 0, kt = 0, buf = 0;
             unsigned phase = 0, s_phase = 1;  // the first wait for an empty S passes
             bool ok = true;
-            while (ok && walk.next(&p)) {
+            for (unsigned turn = 0; ok && parts.get(turn, &p, &s_gave_up); ++turn) {
                 const int kb = kt & 1;
                 if (!bar_wait(&k_full[kb], (kt >> 1) & 1, &s_gave_up)) break;
                 for (int b = 0; ok && b < p.n; ++b) {
@@ -1183,9 +1260,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         int e = 0, buf = 0;
         unsigned phase = 0, s_phase = 0;
         bool ok = true;
-        while (walk.next(&p)) {
-            const SeqWork w = seq_work(a, p.seq);
-            const int q0 = CutSlots::first(w, ge, p.tile);
+        for (unsigned turn = 0; ok && parts.get(turn, &p, &s_gave_up); ++turn) {
+            const int q0 = CutSlots::first(SeqWork{p.len, 0, p.n_new}, ge, p.tile);
             const int h0 = p.tile * kWTileSlots + half * 128, slot = h0 + (warp & 3) * 32 + lane;
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             for (int b = 0; ok && b < p.n; ++b) {
@@ -1194,7 +1270,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 tc_fence_after();
                 const int t0 = (q0 + b) * per;
                 // Some row is none, or does not see all of the half's slots.
-                const bool mask = live < kWTileRows || t0 + per > w.n_new || h0 + 128 > w.len - w.n_new + t0 + 1;
+                const bool mask = live < kWTileRows || t0 + per > p.n_new || h0 + 128 > p.len - p.n_new + t0 + 1;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     float s[32];
@@ -1227,7 +1303,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 buf ^= 1;
                 if (buf == 0) s_phase ^= 1;
             }
-            if (ok && slot < w.len) {
+            if (ok && slot < p.len) {
                 const int page = page_of(a.c, p.seq, slot / kPage);
                 if (page >= 0) {
                     float* at = a.c.weight + ((long long)page * a.c.n_kv + p.head) * kPage + slot % kPage;
@@ -1262,44 +1338,10 @@ cudaError_t launch_weights(const AttnArgs& a, const CUtensorMap& km, const CUten
 template <class T, int kD>
 cudaError_t launch_by_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int sms, cudaStream_t s) {
     const long long rows = (long long)a.max_tokens * (a.n_heads / a.c.n_kv);
-    if (rows <= 16) return launch_rows<T, kD, 1, 1>(a, km, vm, sms, s);
-    if (rows <= 32) return launch_rows<T, kD, 2, 1>(a, km, vm, sms, s);
-    if (rows <= 64) return launch_rows<T, kD, 2, 2>(a, km, vm, sms, s);
+    if (rows <= 16) return launch_rows<T, kD, 1, 1, 2>(a, km, vm, sms, s);
+    if (rows <= 32) return launch_rows<T, kD, 2, 1, 2>(a, km, vm, sms, s);
+    if (rows <= 64) return launch_rows<T, kD, 2, 2, 1>(a, km, vm, sms, s);
     return launch_tiles<T, kD>(a, km, vm, sms, s);
-}
-
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-bool encode(CUtensorMap* map, int type, int rank, void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
-    static const EncodeFn fn = [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
-            f = nullptr;
-        return reinterpret_cast<EncodeFn>(f);
-    }();
-    const cuuint32_t steps[4] = {1, 1, 1, 1};
-    return fn && fn(map, type == OP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, base, dims, strides, box, steps,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// K or V: (dim, row of the page, KV head, page) in boxes of 64 dims x 64 rows.
-bool encode_cache(CUtensorMap* map, const PagedView& c, void* base) {
-    const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, kPage, (cuuint64_t)c.n_kv, (cuuint64_t)c.n_pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)c.head_dim * 2, (cuuint64_t)c.head_stride * 2, (cuuint64_t)c.page_stride * 2};
-    const cuuint32_t box[4] = {64, kPage, 1, 1};
-    return encode(map, c.type, 4, base, dims, strides, box);
-}
-
-// q: (dim, head, token) in boxes of 64 dims x one KV head's group x as many whole tokens as 128 rows hold.
-bool encode_q(CUtensorMap* map, const AttnArgs& a) {
-    const int G = a.n_heads / a.c.n_kv;
-    const cuuint64_t dims[3] = {(cuuint64_t)a.c.head_dim, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_tokens};
-    const cuuint64_t strides[2] = {(cuuint64_t)a.c.head_dim * 2, (cuuint64_t)a.q_stride * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(kWTileRows / G)};
-    return encode(map, a.c.type, 3, const_cast<char*>(a.q), dims, strides, box);
 }
 
 int sm_count() {

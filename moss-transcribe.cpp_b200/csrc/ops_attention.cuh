@@ -62,6 +62,19 @@ __device__ __forceinline__ bool bar_wait(uint64_t* b, unsigned parity, volatile 
     }
 }
 
+// A barrier among some threads of the CTA whose wait is bounded: a role that
+// has left its loop leaves nobody waiting for good.
+struct SyncPoint {
+    uint64_t* bar;
+    unsigned phase = 0;
+    volatile int* gave_up;
+    __device__ __forceinline__ void sync() {
+        bar_arrive(bar);
+        bar_wait(bar, phase, gave_up);
+        phase ^= 1;
+    }
+};
+
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
@@ -115,6 +128,7 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t at, uint32_t part) {
     return (uint64_t)((at >> 4) & 0x3FFF) | ((uint64_t)(part >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 // f32 sums of 16-bit products, 128 rows x n columns.
+constexpr uint32_t kNegateA = 1u << 13;
 __device__ __forceinline__ constexpr uint32_t tc_instr(bool bf16, int n, bool b_mn) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(128 >> 4) << 24);
@@ -171,32 +185,52 @@ struct CutSlots {  // the weights of many: tiles of slots, in tiles of the new t
         return (w.n_new + per - 1) / per - first(w, ge, tile);
     }
 };
+// Units of a sequence under one KV head, one sequence a lane: few tiles by
+// the lane itself, many by the whole warp.
 template <class Cut>
 __device__ __forceinline__ long long head_units(const SeqWork& w, const Geometry& ge) {
-    long long u = 0;
+    const int lane = threadIdx.x & 31;
     const int tiles = Cut::tiles(w, ge);
-    for (int t = 0; t < tiles; ++t) u += Cut::units(w, ge, t);
+    long long u = 0;
+    if (tiles <= 4)
+        for (int t = 0; t < tiles; ++t) u += Cut::units(w, ge, t);
+    for (unsigned many = __ballot_sync(0xffffffffu, tiles > 4); many; many &= many - 1) {
+        const int from = __ffs(many) - 1;
+        const SeqWork x{__shfl_sync(0xffffffffu, w.len, from), 0, __shfl_sync(0xffffffffu, w.n_new, from)};
+        const int n = __shfl_sync(0xffffffffu, tiles, from);
+        long long sum = 0;
+        for (int t = lane; t < n; t += 32) sum += Cut::units(x, ge, t);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == from) u = sum;
+    }
     return u;
 }
 
 // The CTA's interval of the line, and where it begins.
 struct Line {
     long long total, lo, hi;
-    int ctas;         // CTAs that have an interval
-    int seq;          // sequence of unit lo
-    long long off;    // of lo in that sequence's units
+    int ctas;               // CTAs that have an interval
+    int seq;                // sequence of unit lo
+    long long off, per;     // of lo in that sequence's units; those of one KV head
 };
 
-// All threads of the CTA; s_scan: one long long a warp + 4.
+// All threads of the CTA, in whole warps; s_scan: one long long a warp + 3.
 template <int kThreads, class Cut>
 __device__ Line find_line(const AttnArgs& a, const Geometry& ge, int min_units, long long* s_scan) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     constexpr int kWarps = kThreads / 32;
+    auto units_of = [&](int s, bool report) {
+        SeqWork w{0, 0, 0};
+        if (s < a.c.n_seq) {
+            w = seq_work(a, s);
+            if (report && w.n_new > w.len && blockIdx.x == 0) flag(a.c, BAD_LEN);
+        }
+        return head_units<Cut>(w, ge) * a.c.n_kv;
+    };
     long long mine = 0, sum = 0;
-    for (int s = threadIdx.x; s < a.c.n_seq; s += kThreads) {
-        const SeqWork w = seq_work(a, s);
-        if (w.n_new > w.len && blockIdx.x == 0) flag(a.c, BAD_LEN);
-        mine = head_units<Cut>(w, ge) * a.c.n_kv;
+    for (int s0 = 0; s0 < a.c.n_seq; s0 += kThreads) {
+        mine = units_of(s0 + threadIdx.x, true);
         sum += mine;
     }
 #pragma unroll
@@ -206,17 +240,14 @@ __device__ Line find_line(const AttnArgs& a, const Geometry& ge, int min_units, 
     Line l{};
     for (int w = 0; w < kWarps; ++w) l.total += s_scan[w];
     const long long fit = max(1ll, l.total / min_units);
-    l.ctas = (int)min((long long)gridDim.x, fit);
-    if (l.total == 0) l.ctas = 0;
+    l.ctas = l.total ? (int)min((long long)gridDim.x, fit) : 0;
     if ((int)blockIdx.x < l.ctas) {
         l.lo = l.total * blockIdx.x / l.ctas;
         l.hi = l.total * (blockIdx.x + 1) / l.ctas;
     }
     long long base = 0;
     for (int s0 = 0; s0 < a.c.n_seq; s0 += kThreads) {
-        const int s = s0 + threadIdx.x;
-        long long v = a.c.n_seq <= kThreads ? mine : s < a.c.n_seq ? head_units<Cut>(seq_work(a, s), ge) * a.c.n_kv : 0;
-        if (s >= a.c.n_seq) v = 0;
+        const long long v = a.c.n_seq <= kThreads ? mine : units_of(s0 + threadIdx.x, false);
         long long x = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -227,53 +258,69 @@ __device__ Line find_line(const AttnArgs& a, const Geometry& ge, int min_units, 
         if (lane == 31) s_scan[warp] = x;
         __syncthreads();
         long long before = base;
-        for (int w = 0; w < warp; ++w) before += s_scan[w];
-        for (int w = 0; w < kWarps; ++w) base += s_scan[w];
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += s_scan[w];
+            base += s_scan[w];
+        }
         const long long first = before + x - v;
         if (v > 0 && first <= l.lo && l.lo < first + v) {
-            s_scan[kWarps] = s;
+            s_scan[kWarps] = s0 + threadIdx.x;
             s_scan[kWarps + 1] = l.lo - first;
+            s_scan[kWarps + 2] = v / a.c.n_kv;
         }
     }
     __syncthreads();
     l.seq = (int)s_scan[kWarps];
     l.off = s_scan[kWarps + 1];
+    l.per = s_scan[kWarps + 2];
     return l;
 }
 
 // The CTA whose interval holds unit u.
 __device__ __forceinline__ int cta_of(const Line& l, long long u) { return (int)(((u + 1) * l.ctas - 1) / l.total); }
 
-// A CTA's part of one tile: blocks [b0, b1) of its n.
+// A CTA's part of one tile: blocks [b0, b1) of its n, with what the roles need
+// of its sequence.  n == 0: there are no more parts.
 struct Part {
     int seq, head, tile, b0, b1, n;
-    long long u0;  // the tile's first unit
+    int len, tok0, n_new;
+    int c0, c1;  // the CTAs that have parts of the tile
 };
 
-// Walks the CTA's interval; every role of the CTA walks it by itself.  Whole: a
-// tile goes undivided to the interval that holds its first unit.
+// Walks the CTA's interval, one warp.  Whole: a tile goes undivided to the
+// interval that holds its first unit.
 template <class Cut, bool kWhole = false>
 struct Walk {
     const AttnArgs& a;
     const Geometry ge;
-    long long at, hi;  // next unit, end of the interval
+    const Line& line;
+    long long at;  // next unit
     SeqWork w{};
     int seq, head = 0, tile = 0, block = 0, tiles = 0;
 
-    __device__ Walk(const AttnArgs& args, const Geometry& g, const Line& l) : a(args), ge(g), at(l.lo), hi(l.hi), seq(l.seq) {
-        if (at >= hi) return;
+    __device__ Walk(const AttnArgs& args, const Geometry& g, const Line& l) : a(args), ge(g), line(l), at(l.lo), seq(l.seq) {
         w = seq_work(a, seq);
         tiles = Cut::tiles(w, ge);
-        const long long per = head_units<Cut>(w, ge);
-        long long off = l.off % per;
-        head = (int)(l.off / per);
-        for (;;) {
-            const int n = Cut::units(w, ge, tile);
-            if (off < n) break;
-            off -= n;
-            ++tile;
+        head = (int)(l.off / l.per);
+        long long off = l.off % l.per;
+        const int lane = threadIdx.x & 31;
+        for (;; tile += 32) {  // 32 tiles at a time
+            long long x = tile + lane < tiles ? Cut::units(w, ge, tile + lane) : 0;
+            const long long v = x;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, off < x);
+            if (past) {
+                const int i = __ffs(past) - 1;
+                tile += i;
+                block = (int)(off - __shfl_sync(0xffffffffu, x - v, i));
+                break;
+            }
+            off -= __shfl_sync(0xffffffffu, x, 31);
         }
-        block = (int)off;
         if (kWhole && block > 0) {
             at += Cut::units(w, ge, tile) - block;
             step();
@@ -285,21 +332,55 @@ struct Walk {
         tile = 0;
         if (++head < a.c.n_kv) return;
         head = 0;
-        while (at < hi) {
+        while (at < line.hi) {
             w = seq_work(a, ++seq);
             tiles = Cut::tiles(w, ge);
             if (tiles > 0) break;
         }
     }
     __device__ bool next(Part* p) {
-        if (at >= hi) return false;
+        if (at >= line.hi) return false;
         const int n = Cut::units(w, ge, tile);
-        const int take = kWhole ? n : (int)min((long long)(n - block), hi - at);
-        *p = Part{seq, head, tile, block, block + take, n, at - block};
+        const int take = kWhole ? n : (int)min((long long)(n - block), line.hi - at);
+        const long long u0 = at - block;
+        const bool cut = !kWhole && take < n;
+        *p = Part{seq, head, tile, block, block + take, n, w.len, w.tok0, w.n_new, cut ? cta_of(line, u0) : 0, cut ? cta_of(line, u0 + n - 1) : 0};
         at += take;
         block += take;
         if (block == n) step();
         return true;
+    }
+};
+
+// The producer warp walks and hands the parts to the other roles' warps
+// through a ring in shared memory.
+template <int kRing>
+struct PartRing {
+    Part part[kRing];
+    uint64_t full[kRing], taken[kRing];
+    __device__ void init(int warps) {
+        for (int i = 0; i < kRing; ++i) {
+            bar_init(&full[i], 1);
+            bar_init(&taken[i], warps);
+        }
+    }
+    // The producer warp, the i-th part; false: the wait for room ran out.
+    __device__ bool put(unsigned i, const Part& p, volatile int* gave_up) {
+        if (i >= kRing && !bar_wait(&taken[i % kRing], (i / kRing - 1) & 1, gave_up)) return false;
+        if ((threadIdx.x & 31) == 0) {
+            part[i % kRing] = p;
+            bar_arrive(&full[i % kRing]);
+        }
+        __syncwarp();
+        return true;
+    }
+    // A warp; false: there are no more.
+    __device__ bool get(unsigned i, Part* p, volatile int* gave_up) {
+        if (!bar_wait(&full[i % kRing], (i / kRing) & 1, gave_up)) return false;
+        *p = part[i % kRing];
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) bar_arrive(&taken[i % kRing]);
+        return p->n > 0;
     }
 };
 
@@ -316,6 +397,18 @@ __device__ __forceinline__ float* part_at(const AttnArgs& a, int cta, bool begin
     return reinterpret_cast<float*>(a.workspace + kPartsAt) + (size_t)(2 * cta + (begins ? 1 : 0)) * (kRows * (kD + 2));
 }
 
+// Loads of what other CTAs wrote in this launch: from L2, and kept in order with the barriers.
+__device__ __forceinline__ float ld_cg(const float* p) {
+    float x;
+    asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(x) : "l"(p));
+    return x;
+}
+__device__ __forceinline__ float4 ld_cg4(const float* p) {
+    float4 x;
+    asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "l"(p));
+    return x;
+}
+
 template <class T>
 __device__ __forceinline__ void store4(T* p, float4 x) {
     uint2 u;
@@ -328,45 +421,76 @@ __device__ __forceinline__ void store4(T* p, float4 x) {
 }
 
 // Where row r of a part's tile goes; false: not a row of the sequence.
-__device__ __forceinline__ bool row_place(const AttnArgs& a, const Geometry& ge, const SeqWork& w, const Part& p, int r, long long* token,
-                                          int* head) {
+__device__ __forceinline__ bool row_place(const Geometry& ge, const Part& p, int r, long long* token, int* head) {
     const int row = p.tile * ge.rows + r;
-    if (row >= w.n_new * ge.G) return false;
-    *token = w.tok0 + row / ge.G;
+    if (r >= ge.rows || row >= p.n_new * ge.G) return false;
+    *token = p.tok0 + row / ge.G;
     *head = p.head * ge.G + row % ge.G;
     return true;
 }
 
+// Counts a part of a split tile as written; true for whom it was the last.
+// By one thread, after a barrier behind everyone's writes and fences.
+__device__ __forceinline__ bool part_is_last(const AttnArgs& a, const Part& p) {
+    int* count = reinterpret_cast<int*>(a.workspace) + p.c0;
+    __threadfence();
+    const bool last = atomicAdd(count, 1) == p.c1 - p.c0;
+    if (last) *count = 0;
+    __threadfence();
+    return last;
+}
+
 // Joins a split tile's parts, by kThreads threads numbered t.
+// First each row's factors, a warp a row and a lane a part; they take the maxima's
+// place.  Then the sums, whose loads depend on nothing.
 template <class T, int kRows, int kD, int kThreads>
-__device__ void join_parts(const AttnArgs& a, const Geometry& ge, const Line& l, const SeqWork& w, const Part& p, int t) {
-    const int c0 = cta_of(l, p.u0), c1 = cta_of(l, p.u0 + p.n - 1);
+__device__ void join_parts(const AttnArgs& a, const Geometry& ge, const Part& p, int t, SyncPoint& all) {
+    const int rows = min(ge.rows, p.n_new * ge.G - p.tile * ge.rows);
+    const int lane = t & 31;
+    const int parts = p.c1 - p.c0 + 1;
+#pragma unroll 4
+    for (int r = t >> 5; r < rows; r += kThreads / 32) {
+        float m = -INFINITY, sum = 0.f;
+        for (int i = lane; i < parts; i += 32) m = fmaxf(m, ld_cg(part_at<kRows, kD>(a, p.c0 + i, i == 0) + r));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float base = m == -INFINITY ? 0.f : m;
+        for (int i = lane; i < parts; i += 32) {
+            const float* q = part_at<kRows, kD>(a, p.c0 + i, i == 0) + r;
+            sum += exp2f(ld_cg(q) - base) * ld_cg(q + kRows);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        for (int i = lane; i < parts; i += 32) {
+            float* q = part_at<kRows, kD>(a, p.c0 + i, i == 0) + r;
+            __stcg(q, exp2f(ld_cg(q) - base) * inv);
+        }
+        long long token;
+        int head;
+        if (lane == 0 && a.lse && row_place(ge, p, r, &token, &head))
+            a.lse[token * a.n_heads + head] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+    }
+    all.sync();
     constexpr int kCols = kD / 4;
-    for (int i = t; i < kRows * kCols; i += kThreads) {
+#pragma unroll 2
+    for (int i = t; i < rows * kCols; i += kThreads) {
         const int r = i / kCols, col = i % kCols * 4;
         long long token;
         int head;
-        if (!row_place(a, ge, w, p, r, &token, &head)) continue;
-        float m = -INFINITY;
-        for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(part_at<kRows, kD>(a, c, c == c0) + r));
-        const float base = m == -INFINITY ? 0.f : m;
-        float sum = 0.f;
+        if (!row_place(ge, p, r, &token, &head)) continue;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int c = c0; c <= c1; ++c) {
-            const float* q = part_at<kRows, kD>(a, c, c == c0);
-            const float f = exp2f(__ldcg(q + r) - base);
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(q + 2 * kRows + r * kD + col));
-            sum = fmaf(f, __ldcg(q + kRows + r), sum);
-            o.x = fmaf(f, x.x, o.x);
-            o.y = fmaf(f, x.y, o.y);
-            o.z = fmaf(f, x.z, o.z);
-            o.w = fmaf(f, x.w, o.w);
+        for (int c = 0; c < parts; ++c) {
+            const float* q = part_at<kRows, kD>(a, p.c0 + c, c == 0);
+            const float f = ld_cg(q + r);
+            const float4 x = ld_cg4(q + 2 * kRows + r * kD + col);
+            o.x = __fmaf_rn(f, x.x, o.x);
+            o.y = __fmaf_rn(f, x.y, o.y);
+            o.z = __fmaf_rn(f, x.z, o.z);
+            o.w = __fmaf_rn(f, x.w, o.w);
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        store4<T>(reinterpret_cast<T*>(a.out) + token * a.out_stride + (long long)head * kD + col,
-                  make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-        if (col == 0 && a.lse) a.lse[token * a.n_heads + head] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+        store4<T>(reinterpret_cast<T*>(a.out) + token * a.out_stride + (long long)head * kD + col, o);
     }
 }
 
