@@ -131,7 +131,7 @@ constexpr int kPartRing = 8;
 
 template <class T, int kD, int MW, int WM, int WP>
 __global__ void __launch_bounds__(RowsShape<kD, MW, WM, WP>::kThreads, 1)
-    k_attention_rows(const AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+    k_attention_rows(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using S = RowsShape<kD, MW, WM, WP>;
     constexpr int kParts = kD / 64;  // 64-dim parts of a row
     constexpr int kSplit = 4 * WP;   // warps that share a row
@@ -152,14 +152,17 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM, WP>::kThreads, 1)
             bar_init(&full[i], 1);
             bar_init(&empty[i], 4 * WM);
         }
-        bar_init(&all_bar, S::kWarps * 32);
+        bar_init(&all_bar, S::kWarps);
         parts.init(S::kWarps);
         s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const Line line = find_line<S::kThreads, CutRows>(a, ge, kRowsMinUnits, s_scan);
+    if (threadIdx.x == S::kWarps * 32) {
+        tma_prefetch(&k_map);
+        tma_prefetch(&v_map);
+    }
     __syncthreads();
-    if (line.lo >= line.hi) return;
+    const Line line = find_line<S::kThreads, CutRows>(a, ge, kRowsMinUnits, s_scan, warp == S::kWarps);
     Part p;
 
     if (warp == S::kWarps) {
@@ -461,11 +464,10 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM, WP>::kThreads, 1)
             }
         }
         if (!whole) {
-            __threadfence();
             all.sync();
             if (tid == 0) s_last = part_is_last(a, p);
             all.sync();
-            if (s_last) join_parts<T, S::kRows, kD, S::kWarps * 32>(a, ge, p, tid, all);
+            if (s_last) join_parts<T, S::kRows, kD, S::kWarps>(a, ge, p, warp);
         }
     }
 }
@@ -509,7 +511,7 @@ struct TileShape {
 
 template <class T, int kD>
 __global__ void __launch_bounds__(kTileThreads, 1)
-    k_attention_tiles(const AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+    k_attention_tiles(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                       const __grid_constant__ CUtensorMap q_map) {
     using S = TileShape<kD>;
     constexpr int kParts = kD / 64;
@@ -535,19 +537,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int h = 0; h < 2; ++h) {
             bar_init(&q_full[h], 1);
             bar_init(&s_full[h], 1);
-            bar_init(&p_full[h], 128);
+            bar_init(&p_full[h], 4);
             bar_init(&o_full[h], 1);
         }
         bar_init(&q_empty, 1);
-        bar_init(&all_bar, 256);
+        bar_init(&all_bar, 8);
         bar_init(&drained, 1);
         parts.init(10);
         s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const Line line = find_line<kTileThreads, CutRows>(a, ge, kTilesMinUnits, s_scan);
-    __syncthreads();
-    if (line.lo >= line.hi) return;
+    if (threadIdx.x == 9 * 32) {
+        tma_prefetch(&k_map);
+        tma_prefetch(&v_map);
+        tma_prefetch(&q_map);
+    }
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -556,6 +560,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;  // S of the halves at 0 and 128, O at 256 and 384
+    const Line line = find_line<kTileThreads, CutRows>(a, ge, kTilesMinUnits, s_scan, warp == 9);
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -799,7 +804,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                     tmem_wait_st();
                     tc_fence_before();
-                    bar_arrive(&p_full[half]);
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&p_full[half]);
                     l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 }
                 if (ok && bar_wait(&o_full[half], o_phase, &s_gave_up)) {
@@ -842,11 +848,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 slot = (slot + p.b1 - p.b0) % kBadRing;
             }
             if (!whole) {
-                __threadfence();
                 all.sync();
                 if (threadIdx.x == 0) s_last = part_is_last(a, p);
                 all.sync();
-                if (s_last) join_parts<T, kTileRows2, kD, 256>(a, ge, p, threadIdx.x, all);
+                if (s_last) join_parts<T, kTileRows2, kD, 8>(a, ge, p, warp);
             }
         }
     }
@@ -886,7 +891,7 @@ struct WRowsShape {
 };
 
 template <class T, int kD>
-__global__ void __launch_bounds__(kWThreads, 1) k_weights_rows(const AttnArgs a, const __grid_constant__ CUtensorMap k_map) {
+__global__ void __launch_bounds__(kWThreads, 1) k_weights_rows(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map) {
     using S = WRowsShape<kD>;
     constexpr int kParts = kD / 64, kHalf = kPage * 128;
     extern __shared__ uint8_t smem_raw[];
@@ -905,14 +910,14 @@ __global__ void __launch_bounds__(kWThreads, 1) k_weights_rows(const AttnArgs a,
             bar_init(&full[i], 1);
             bar_init(&empty[i], 4);
         }
-        bar_init(&all_bar, 128);
+        bar_init(&all_bar, 4);
         parts.init(4);
         s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const Line line = find_line<kWThreads, CutPages>(a, ge, kRowsMinUnits, s_scan);
+    if (threadIdx.x == 128) tma_prefetch(&k_map);
     __syncthreads();
-    if (line.lo >= line.hi) return;
+    const Line line = find_line<kWThreads, CutPages>(a, ge, kRowsMinUnits, s_scan, warp == 4);
     Part p;
     if (warp == 4) {
         Walk<CutPages> walk(a, ge, line);
@@ -1076,7 +1081,7 @@ struct WTileShape {
 
 template <class T, int kD>
 __global__ void __launch_bounds__(kTileThreads, 1)
-    k_weights_tiles(const AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap q_map) {
+    k_weights_tiles(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap q_map) {
     using S = WTileShape<kD>;
     constexpr int kParts = kD / 64;
     constexpr bool kBf16 = !std::is_same<T, __half>::value;
@@ -1122,9 +1127,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int i = threadIdx.x; i < kWEntries * S::kEntry / 16; i += kTileThreads) reinterpret_cast<uint4*>(q)[i] = make_uint4(0, 0, 0, 0);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    const Line line = find_line<kTileThreads, CutSlots>(a, ge, kTilesMinUnits, s_scan);
-    __syncthreads();
-    if (line.lo >= line.hi) return;
+    if (threadIdx.x == 9 * 32) {
+        tma_prefetch(&k_map);
+        tma_prefetch(&q_map);
+    }
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -1133,6 +1139,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
+    const Line line = find_line<kTileThreads, CutSlots>(a, ge, kTilesMinUnits, s_scan, warp == 9);
     Part p;
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));

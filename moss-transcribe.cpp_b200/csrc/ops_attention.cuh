@@ -48,12 +48,13 @@ __device__ __forceinline__ bool bar_wait(uint64_t* b, unsigned parity, volatile 
     unsigned long long t0 = 0;
     for (unsigned it = 0;; ++it) {
         uint32_t ok;
-        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
                      : "=r"(ok)
-                     : "r"(at), "r"(parity), "r"(20000u)
+                     : "r"(at), "r"(parity)
                      : "memory");
         if (ok) return true;
-        if (it == 0) t0 = now_ns();
+        if (it < 64) continue;  // the time is looked at once it has become long
+        if (it == 64) t0 = now_ns();
         if (*gave_up) return false;
         if (now_ns() - t0 > kWaitNs) {
             *gave_up = 1;
@@ -68,13 +69,17 @@ struct SyncPoint {
     uint64_t* bar;
     unsigned phase = 0;
     volatile int* gave_up;
-    __device__ __forceinline__ void sync() {
-        bar_arrive(bar);
+    __device__ __forceinline__ void sync() {  // counts warps
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) bar_arrive(bar);
         bar_wait(bar, phase, gave_up);
         phase ^= 1;
     }
 };
 
+__device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
@@ -155,10 +160,14 @@ struct Geometry {
 };
 
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int s) {
-    const int2 tok = seq_tokens(a.c, a.cu, a.n_tokens, s);
-    SeqWork w{0, tok.x, tok.y};
-    if (tok.y) w.len = seq_len(a.c, s);
-    return w;
+    const int b = a.cu[s], e = a.cu[s + 1], n = a.c.kv_len[s];  // together: none waits for another
+    if (b < 0 || e < b || e > a.n_tokens) {
+        flag(a.c, BAD_TOKENS);
+        return SeqWork{0, 0, 0};
+    }
+    const int len = (int)min(max((long long)n, 0ll), (long long)a.c.table_stride * kPage);
+    if (e > b && len != n) flag(a.c, BAD_LEN);
+    return SeqWork{len, b, e - b};
 }
 
 // How a sequence's work under one KV head is cut: tiles, and units of a tile.
@@ -207,17 +216,63 @@ __device__ __forceinline__ long long head_units(const SeqWork& w, const Geometry
     return u;
 }
 
+// x * y / z of values that are mostly small: 32-bit division where it does.
+__device__ __forceinline__ long long mul_div(long long x, int y, long long z) {
+    if (x < (1 << 20) && y <= 1024 && z < (1ll << 31)) return (long long)((unsigned)x * (unsigned)y / (unsigned)z);
+    return x * y / z;
+}
+__device__ __forceinline__ long long div_small(long long x, long long z) {
+    return x < (1ll << 31) && z < (1ll << 31) ? (long long)((unsigned)x / (unsigned)z) : x / z;
+}
+
 // The CTA's interval of the line, and where it begins.
 struct Line {
     long long total, lo, hi;
-    int ctas;               // CTAs that have an interval
-    int seq;                // sequence of unit lo
-    long long off, per;     // of lo in that sequence's units; those of one KV head
+    int ctas;       // CTAs that have an interval
+    int seq;        // sequence of unit lo
+    long long off;  // of lo in that sequence's units
+    long long per;  // that sequence's units under one KV head
 };
 
-// All threads of the CTA, in whole warps; s_scan: one long long a warp + 3.
+__device__ __forceinline__ void cut_line(Line* l, int min_units) {
+    const long long fit = max(1ll, div_small(l->total, min_units));
+    l->ctas = l->total ? (int)min((long long)gridDim.x, fit) : 0;
+    l->lo = l->hi = 0;
+    if ((int)blockIdx.x < l->ctas) {
+        l->lo = mul_div(l->total, blockIdx.x, l->ctas);
+        l->hi = mul_div(l->total, blockIdx.x + 1, l->ctas);
+    }
+}
+
+// Up to 32 sequences: one warp by itself.
+template <class Cut>
+__device__ Line find_line_warp(const AttnArgs& a, const Geometry& ge, int min_units) {
+    const int lane = threadIdx.x & 31;
+    SeqWork w{0, 0, 0};
+    if (lane < a.c.n_seq) {
+        w = seq_work(a, lane);
+        if (w.n_new > w.len && blockIdx.x == 0) flag(a.c, BAD_LEN);
+    }
+    const long long per = head_units<Cut>(w, ge), v = per * a.c.n_kv;
+    long long x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    Line l{};
+    l.total = __shfl_sync(0xffffffffu, x, 31);
+    cut_line(&l, min_units);
+    const unsigned at = __ballot_sync(0xffffffffu, v > 0 && x - v <= l.lo && l.lo < x);
+    l.seq = max(0, __ffs(at) - 1);
+    l.off = l.lo - __shfl_sync(0xffffffffu, x - v, l.seq);
+    l.per = __shfl_sync(0xffffffffu, per, l.seq);
+    return l;
+}
+
+// Any number: all threads of the CTA; s_scan: one long long a warp + 3.
 template <int kThreads, class Cut>
-__device__ Line find_line(const AttnArgs& a, const Geometry& ge, int min_units, long long* s_scan) {
+__device__ Line find_line_cta(const AttnArgs& a, const Geometry& ge, int min_units, long long* s_scan) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     constexpr int kWarps = kThreads / 32;
     auto units_of = [&](int s, bool report) {
@@ -239,12 +294,7 @@ __device__ Line find_line(const AttnArgs& a, const Geometry& ge, int min_units, 
     __syncthreads();
     Line l{};
     for (int w = 0; w < kWarps; ++w) l.total += s_scan[w];
-    const long long fit = max(1ll, l.total / min_units);
-    l.ctas = l.total ? (int)min((long long)gridDim.x, fit) : 0;
-    if ((int)blockIdx.x < l.ctas) {
-        l.lo = l.total * blockIdx.x / l.ctas;
-        l.hi = l.total * (blockIdx.x + 1) / l.ctas;
-    }
+    cut_line(&l, min_units);
     long long base = 0;
     for (int s0 = 0; s0 < a.c.n_seq; s0 += kThreads) {
         const long long v = a.c.n_seq <= kThreads ? mine : units_of(s0 + threadIdx.x, false);
@@ -266,7 +316,7 @@ __device__ Line find_line(const AttnArgs& a, const Geometry& ge, int min_units, 
         if (v > 0 && first <= l.lo && l.lo < first + v) {
             s_scan[kWarps] = s0 + threadIdx.x;
             s_scan[kWarps + 1] = l.lo - first;
-            s_scan[kWarps + 2] = v / a.c.n_kv;
+            s_scan[kWarps + 2] = div_small(v, a.c.n_kv);
         }
     }
     __syncthreads();
@@ -276,8 +326,20 @@ __device__ Line find_line(const AttnArgs& a, const Geometry& ge, int min_units, 
     return l;
 }
 
+// The interval, for the producer warp; all threads call, and with few
+// sequences nobody waits.
+template <int kThreads, class Cut>
+__device__ __forceinline__ Line find_line(const AttnArgs& a, const Geometry& ge, int min_units, long long* s_scan, bool producer) {
+    if (a.c.n_seq > 32) return find_line_cta<kThreads, Cut>(a, ge, min_units, s_scan);
+    if (!producer) return Line{};
+    return find_line_warp<Cut>(a, ge, min_units);
+}
+
 // The CTA whose interval holds unit u.
-__device__ __forceinline__ int cta_of(const Line& l, long long u) { return (int)(((u + 1) * l.ctas - 1) / l.total); }
+__device__ __forceinline__ int cta_of(const Line& l, long long u) {
+    if (u < (1 << 20) && l.ctas <= 1024) return (int)(((unsigned)(u + 1) * (unsigned)l.ctas - 1) / (unsigned)l.total);
+    return (int)(((u + 1) * l.ctas - 1) / l.total);
+}
 
 // A CTA's part of one tile: blocks [b0, b1) of its n, with what the roles need
 // of its sequence.  n == 0: there are no more parts.
@@ -299,10 +361,11 @@ struct Walk {
     int seq, head = 0, tile = 0, block = 0, tiles = 0;
 
     __device__ Walk(const AttnArgs& args, const Geometry& g, const Line& l) : a(args), ge(g), line(l), at(l.lo), seq(l.seq) {
+        if (l.lo >= l.hi) return;
         w = seq_work(a, seq);
         tiles = Cut::tiles(w, ge);
-        head = (int)(l.off / l.per);
-        long long off = l.off % l.per;
+        head = a.c.n_kv == 1 ? 0 : (int)div_small(l.off, l.per);
+        long long off = l.off - head * l.per;
         const int lane = threadIdx.x & 31;
         for (;; tile += 32) {  // 32 tiles at a time
             long long x = tile + lane < tiles ? Cut::units(w, ge, tile + lane) : 0;
@@ -403,6 +466,11 @@ __device__ __forceinline__ float ld_cg(const float* p) {
     asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(x) : "l"(p));
     return x;
 }
+__device__ __forceinline__ float2 ld_cg2(const float* p) {
+    float2 x;
+    asm volatile("ld.global.cg.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "l"(p));
+    return x;
+}
 __device__ __forceinline__ float4 ld_cg4(const float* p) {
     float4 x;
     asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "l"(p));
@@ -430,67 +498,94 @@ __device__ __forceinline__ bool row_place(const Geometry& ge, const Part& p, int
 }
 
 // Counts a part of a split tile as written; true for whom it was the last.
-// By one thread, after a barrier behind everyone's writes and fences.
+// By one thread, between two barriers of the CTA: its release covers what the
+// others wrote before the first, its acquire what they read behind the second.
 __device__ __forceinline__ bool part_is_last(const AttnArgs& a, const Part& p) {
     int* count = reinterpret_cast<int*>(a.workspace) + p.c0;
-    __threadfence();
-    const bool last = atomicAdd(count, 1) == p.c1 - p.c0;
+    int before;
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
+    const bool last = before == p.c1 - p.c0;
     if (last) *count = 0;
-    __threadfence();
     return last;
 }
 
-// Joins a split tile's parts, by kThreads threads numbered t.
-// First each row's factors, a warp a row and a lane a part; they take the maxima's
-// place.  Then the sums, whose loads depend on nothing.
-template <class T, int kRows, int kD, int kThreads>
-__device__ void join_parts(const AttnArgs& a, const Geometry& ge, const Part& p, int t, SyncPoint& all) {
+// Joins a split tile's parts, by kWarps warps: a warp a row, a lane a part's
+// maximum and sum and some columns; the columns' loads wait for nothing.
+template <class T, int kRows, int kD, int kWarps>
+__device__ __forceinline__ void join_parts(const AttnArgs& a, const Geometry& ge, const Part& p, int warp) {
+    constexpr int kCols = kD / 32, kBatch = 8;
     const int rows = min(ge.rows, p.n_new * ge.G - p.tile * ge.rows);
-    const int lane = t & 31;
+    const int lane = threadIdx.x & 31;
     const int parts = p.c1 - p.c0 + 1;
-#pragma unroll 4
-    for (int r = t >> 5; r < rows; r += kThreads / 32) {
-        float m = -INFINITY, sum = 0.f;
-        for (int i = lane; i < parts; i += 32) m = fmaxf(m, ld_cg(part_at<kRows, kD>(a, p.c0 + i, i == 0) + r));
+    int c_first = p.c0;
+    asm volatile("" : "+r"(c_first));  // addresses are formed here, not kept through the loops above
+    auto at = [&](int i) { return part_at<kRows, kD>(a, c_first + i, i == 0); };
+#pragma unroll 1
+    for (int r = warp; r < rows; r += kWarps) {
+        float x[kBatch][kCols];
+        auto load = [&](int c0) {
+            const float* from = part_at<kRows, kD>(a, c_first + c0, false) + 2 * kRows + r * kD + lane * kCols;
+#pragma unroll
+            for (int c = 0; c < kBatch; ++c)
+                if (c0 + c < parts) {
+                    const float* q = from + c * (2 * kRows * (kD + 2)) + (c == 0 && c0 == 0 ? kRows * (kD + 2) : 0);
+                    if constexpr (kCols == 4) {
+                        const float4 y = ld_cg4(q);
+                        x[c][0] = y.x, x[c][1] = y.y, x[c][2] = y.z, x[c][3] = y.w;
+                    } else {
+                        const float2 y = ld_cg2(q);
+                        x[c][0] = y.x, x[c][1] = y.y;
+                    }
+                }
+        };
+        load(0);
+        float mi = -INFINITY, li = 0.f;
+        if (lane < parts) {
+            mi = ld_cg(at(lane) + r);
+            li = ld_cg(at(lane) + kRows + r);
+        }
+        float m = mi;
+        for (int i = 32 + lane; i < parts; i += 32) m = fmaxf(m, ld_cg(at(i) + r));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         const float base = m == -INFINITY ? 0.f : m;
-        for (int i = lane; i < parts; i += 32) {
-            const float* q = part_at<kRows, kD>(a, p.c0 + i, i == 0) + r;
-            sum += exp2f(ld_cg(q) - base) * ld_cg(q + kRows);
+        float o[kCols], sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) o[k] = 0.f;
+#pragma unroll 1
+        for (int c0 = 0; c0 < parts; c0 += 32) {
+            if (c0 > 0 && c0 + lane < parts) {
+                mi = ld_cg(at(c0 + lane) + r);
+                li = ld_cg(at(c0 + lane) + kRows + r);
+            }
+            const float f = c0 + lane < parts ? exp2f(mi - base) : 0.f;
+            sum += c0 + lane < parts ? f * li : 0.f;
+#pragma unroll 1
+            for (int h = 0; h < 32 && c0 + h < parts; h += kBatch) {
+                if (c0 + h > 0) load(c0 + h);
+#pragma unroll
+                for (int c = 0; c < kBatch; ++c) {
+                    const float fc = __shfl_sync(0xffffffffu, f, h + c);
+                    if (c0 + h + c < parts)
+#pragma unroll
+                        for (int k = 0; k < kCols; ++k) o[k] = __fmaf_rn(fc, x[c][k], o[k]);
+                }
+            }
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        for (int i = lane; i < parts; i += 32) {
-            float* q = part_at<kRows, kD>(a, p.c0 + i, i == 0) + r;
-            __stcg(q, exp2f(ld_cg(q) - base) * inv);
-        }
         long long token;
         int head;
-        if (lane == 0 && a.lse && row_place(ge, p, r, &token, &head))
-            a.lse[token * a.n_heads + head] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
-    }
-    all.sync();
-    constexpr int kCols = kD / 4;
-#pragma unroll 2
-    for (int i = t; i < rows * kCols; i += kThreads) {
-        const int r = i / kCols, col = i % kCols * 4;
-        long long token;
-        int head;
-        if (!row_place(ge, p, r, &token, &head)) continue;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int c = 0; c < parts; ++c) {
-            const float* q = part_at<kRows, kD>(a, p.c0 + c, c == 0);
-            const float f = ld_cg(q + r);
-            const float4 x = ld_cg4(q + 2 * kRows + r * kD + col);
-            o.x = __fmaf_rn(f, x.x, o.x);
-            o.y = __fmaf_rn(f, x.y, o.y);
-            o.z = __fmaf_rn(f, x.z, o.z);
-            o.w = __fmaf_rn(f, x.w, o.w);
+        row_place(ge, p, r, &token, &head);
+        T* out = reinterpret_cast<T*>(a.out) + token * a.out_stride + (long long)head * kD + lane * kCols;
+        if constexpr (kCols == 4) {
+            store4<T>(out, make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv));
+        } else {
+            out[0] = from_f32<T>(o[0] * inv);
+            out[1] = from_f32<T>(o[1] * inv);
         }
-        store4<T>(reinterpret_cast<T*>(a.out) + token * a.out_stride + (long long)head * kD + col, o);
+        if (lane == 0 && a.lse) a.lse[token * a.n_heads + head] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
     }
 }
 
