@@ -634,43 +634,47 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         } else if (warp == 8) {
             const uint32_t kQk = tc_instr(kBf16, kTileBlock, false) | (a.scale < 0.f ? kNegateA : 0u);
             constexpr uint32_t kPv = tc_instr(kBf16, kD, true);
+            const uint32_t t_at = uniform(tmem), q_lo = uniform(desc_lo_k(q_at)), k_lo = uniform(desc_lo_k(ring)),
+                           v_lo = uniform(desc_lo_mn(ring, S::kPart));
             int e = 0;
             unsigned phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
             bool ok = true;
             auto qk = [&](int h, int entry) {
-                if (lane == 0) {
-                    const uint32_t qa = q_at + h * S::kEntry, kb = ring + entry * S::kEntry;
+                if (elect_one()) {
 #pragma unroll
                     for (int kk = 0; kk < kD / 16; ++kk) {
-                        const uint32_t off = (kk / 4) * S::kPart + (kk % 4) * 32;
-                        tc_mma_ss(tmem + h * 128, desc_k(qa + off), desc_k(kb + off), kQk, kk > 0);
+                        const uint32_t off = ((kk / 4) * S::kPart + (kk % 4) * 32) / 16;
+                        tc_mma_ss(t_at + h * 128, q_lo + h * (S::kEntry / 16) + off, k_lo + entry * (S::kEntry / 16) + off, kQk, kk > 0);
                     }
                     tc_commit(&s_full[h]);
                 }
+                __syncwarp();
             };
-            for (unsigned turn = 0; ok && parts.get(turn, &p, &s_gave_up); ++turn) {
-                const int halves = p.n_new > (2 * p.tile + 1) * per ? 2 : 1;
+            for (unsigned turn = 0; ok && __all_sync(0xffffffffu, parts.get(turn, &p, &s_gave_up)); ++turn) {
+                const int b0 = uniform(p.b0), b1 = uniform(p.b1), len = uniform(p.len);
+                const int halves = uniform(p.n_new > (2 * p.tile + 1) * per ? 2 : 1);
                 for (int h = 0; ok && h < halves; ++h) {
-                    ok = bar_wait(&q_full[h], q_phase[h], &s_gave_up);
+                    ok = bar_wait_warp(&q_full[h], q_phase[h], &s_gave_up);
                     q_phase[h] ^= 1;
                 }
-                ok = ok && bar_wait(&full[e], phase, &s_gave_up);
+                ok = ok && bar_wait_warp(&full[e], phase, &s_gave_up);
                 if (!ok) break;
                 tc_fence_after();
-                for (int h = 0; h < halves; ++h) qk(h, e);
-                if (lane == 0) {
+                qk(0, e);
+                if (halves == 2) qk(1, e);
+                if (elect_one()) {
                     tc_commit(&empty[e]);
-                    if (p.b1 - p.b0 == 1) tc_commit(&q_empty);
+                    if (b1 - b0 == 1) tc_commit(&q_empty);
                 }
                 if (++e == kTileEntries) e = 0, phase ^= 1;
-                for (int b = p.b0; ok && b < p.b1; ++b) {
+                for (int b = b0; ok && b < b1; ++b) {
                     const int ve = e;
-                    ok = bar_wait(&full[ve], phase, &s_gave_up);
+                    ok = bar_wait_warp(&full[ve], phase, &s_gave_up);
                     if (!ok) break;
                     if (++e == kTileEntries) e = 0, phase ^= 1;
-                    if ((b + 1) * kTileBlock > p.len) {
+                    if ((b + 1) * kTileBlock > len) {
                         // V at or behind the sequence's end may hold anything: 0 there, since 0 * NaN is NaN.
-                        const int from = max(0, p.len - b * kTileBlock);
+                        const int from = max(0, len - b * kTileBlock);
                         uint8_t* v = smem_raw + (ring - smem_u32(smem_raw)) + ve * S::kEntry;
                         for (int i = lane; i < kParts * (kTileBlock - from) * 8; i += 32) {
                             const int h = i / ((kTileBlock - from) * 8), j = i % ((kTileBlock - from) * 8);
@@ -679,29 +683,31 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                     }
-                    const bool more = b + 1 < p.b1;
-                    if (more) ok = bar_wait(&full[e], phase, &s_gave_up);
-                    for (int h = 0; ok && h < halves; ++h) {
-                        ok = bar_wait(&p_full[h], p_phase[h], &s_gave_up);
+                    const bool more = b + 1 < b1;
+                    if (more) ok = bar_wait_warp(&full[e], phase, &s_gave_up);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (!ok || h >= halves) break;
+                        ok = bar_wait_warp(&p_full[h], p_phase[h], &s_gave_up);
                         if (!ok) break;
                         p_phase[h] ^= 1;
                         tc_fence_after();
-                        if (lane == 0) {
-                            const uint32_t vb = ring + ve * S::kEntry;
+                        if (elect_one()) {
 #pragma unroll
                             for (int kk = 0; kk < kTileBlock / 16; ++kk)
-                                tc_mma_ts(tmem + 256 + h * 128, tmem + h * 128 + kk * 8, desc_mn(vb + kk * 2048, S::kPart), kPv,
-                                          b > p.b0 || kk > 0);
+                                tc_mma_ts(t_at + 256 + h * 128, t_at + h * 128 + kk * 8, v_lo + ve * (S::kEntry / 16) + kk * (2048 / 16), kPv,
+                                          b > b0 || kk > 0);
                             if (!more) tc_commit(&o_full[h]);
                         }
+                        __syncwarp();
                         if (more) qk(h, e);
                     }
                     if (!ok) break;
-                    if (lane == 0) tc_commit(&empty[ve]);
+                    if (elect_one()) tc_commit(&empty[ve]);
                     if (more) {
-                        if (lane == 0) {
+                        if (elect_one()) {
                             tc_commit(&empty[e]);
-                            if (b + 2 == p.b1) tc_commit(&q_empty);
+                            if (b + 2 == b1) tc_commit(&q_empty);
                         }
                         if (++e == kTileEntries) e = 0, phase ^= 1;
                     }
@@ -709,7 +715,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
             // Nothing that was issued is left running.
             volatile int none = 0;
-            if (lane == 0) tc_commit(&drained);
+            if (elect_one()) tc_commit(&drained);
             __syncwarp();
             bar_wait(&drained, 0, &none);
         }
@@ -1222,39 +1228,43 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
         } else if (warp == 8) {
             constexpr uint32_t kInstr = tc_instr(kBf16, kWTileRows, false);
+            const uint32_t t_at = uniform(tmem), k_lo = uniform(desc_lo_k(k_at)), q_lo = uniform(desc_lo_k(q_at));
             int e = 0, kt = 0, buf = 0;
             unsigned phase = 0, s_phase = 1;  // the first wait for an empty S passes
             bool ok = true;
-            for (unsigned turn = 0; ok && parts.get(turn, &p, &s_gave_up); ++turn) {
-                const int kb = kt & 1;
-                if (!bar_wait(&k_full[kb], (kt >> 1) & 1, &s_gave_up)) break;
-                for (int b = 0; ok && b < p.n; ++b) {
-                    ok = bar_wait(&q_full[e], phase, &s_gave_up);
-                    for (int h = 0; ok && h < 2; ++h) {
-                        ok = bar_wait(&s_empty[h][buf], s_phase, &s_gave_up);
+            for (unsigned turn = 0; ok && __all_sync(0xffffffffu, parts.get(turn, &p, &s_gave_up)); ++turn) {
+                const int kb = kt & 1, n = uniform(p.n);
+                if (!bar_wait_warp(&k_full[kb], (kt >> 1) & 1, &s_gave_up)) break;
+                for (int b = 0; ok && b < n; ++b) {
+                    ok = bar_wait_warp(&q_full[e], phase, &s_gave_up);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (!ok) break;
+                        ok = bar_wait_warp(&s_empty[h][buf], s_phase, &s_gave_up);
                         if (!ok) break;
                         tc_fence_after();
-                        if (lane == 0) {
-                            const uint32_t ka = k_at + (2 * kb + h) * S::kEntry, qb = q_at + e * S::kEntry;
+                        if (elect_one()) {
 #pragma unroll
                             for (int kk = 0; kk < kD / 16; ++kk) {
-                                const uint32_t off = (kk / 4) * S::kPart + (kk % 4) * 32;
-                                tc_mma_ss(tmem + (h * 2 + buf) * 128, desc_k(ka + off), desc_k(qb + off), kInstr, kk > 0);
+                                const uint32_t off = ((kk / 4) * S::kPart + (kk % 4) * 32) / 16;
+                                tc_mma_ss(t_at + (h * 2 + buf) * 128, k_lo + (2 * kb + h) * (S::kEntry / 16) + off,
+                                          q_lo + e * (S::kEntry / 16) + off, kInstr, kk > 0);
                             }
                             tc_commit(&s_full[h][buf]);
                         }
+                        __syncwarp();
                     }
                     if (!ok) break;
-                    if (lane == 0) tc_commit(&q_empty[e]);
+                    if (elect_one()) tc_commit(&q_empty[e]);
                     if (++e == kWEntries) e = 0, phase ^= 1;
                     buf ^= 1;
                     if (buf == 0) s_phase ^= 1;
                 }
-                if (ok && lane == 0) tc_commit(&k_empty[kb]);
+                if (ok && elect_one()) tc_commit(&k_empty[kb]);
                 ++kt;
             }
             volatile int none = 0;
-            if (lane == 0) tc_commit(&drained);
+            if (elect_one()) tc_commit(&drained);
             __syncwarp();
             bar_wait(&drained, 0, &none);
         }

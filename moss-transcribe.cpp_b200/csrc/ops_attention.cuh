@@ -123,29 +123,44 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&x)[kN]) 
                  : "memory");
 }
 
-// Operand tiles of [dims / 64][rows][64 dims], 128-byte swizzle, 1024-byte aligned.
-// K-major (products over the dims): 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc_k(uint32_t at) {
-    return (uint64_t)((at >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// Descriptors of operand tiles of [dims / 64][rows][64 dims], 128-byte swizzle,
+// 1024-byte aligned: the low word is the tile's (an offset adds its bytes / 16), the
+// high word the layout's.  K-major (products over the dims): 8-row groups 1024 bytes
+// apart.  MN-major (over the rows): also 64-dim parts `part` bytes apart.
+__device__ __forceinline__ uint32_t desc_lo_k(uint32_t at) { return (at >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_lo_mn(uint32_t at, uint32_t part) { return (at >> 4) | ((part >> 4) << 16); }
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+
+// A value that all lanes have, as one the compiler knows to be uniform: the
+// tensor cores' operands are uniform registers, and anything else is moved there
+// for each product (measured: 90 clocks an issue instead of the product's 64).
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ bool bar_wait_warp(uint64_t* b, unsigned parity, volatile int* gave_up) {
+    return __all_sync(0xffffffffu, bar_wait(b, parity, gave_up));
 }
-// MN-major (products over the rows): 64-dim parts `part` bytes apart, 8-row groups 1024.
-__device__ __forceinline__ uint64_t desc_mn(uint32_t at, uint32_t part) {
-    return (uint64_t)((at >> 4) & 0x3FFF) | ((uint64_t)(part >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+__device__ __forceinline__ bool elect_one() {
+    uint32_t is;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(is));
+    return is;
 }
+
 // f32 sums of 16-bit products, 128 rows x n columns.
 constexpr uint32_t kNegateA = 1u << 13;
 __device__ __forceinline__ constexpr uint32_t tc_instr(bool bf16, int n, bool b_mn) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(128 >> 4) << 24);
 }
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-                 ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add)
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t instr, bool add) {
+    asm volatile("{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n"
+                 ::"r"(d), "r"(a), "r"(b), "r"(instr), "r"((uint32_t)add), "r"(kDescHi)
                  : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t instr, bool add) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-                 ::"r"(d), "r"(a), "l"(b), "r"(instr), "r"((uint32_t)add)
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t instr, bool add) {
+    asm volatile("{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n mov.b64 db, {%2, %5};\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n"
+                 ::"r"(d), "r"(a), "r"(b), "r"(instr), "r"((uint32_t)add), "r"(kDescHi)
                  : "memory");
 }
 
