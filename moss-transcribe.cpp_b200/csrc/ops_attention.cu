@@ -16,8 +16,9 @@ namespace {
 
 using namespace ops;
 
-constexpr int kRowsMinUnits = 2;  // pages of a CTA's interval at least
-constexpr int kTilesMinUnits = 1; // blocks of 128 slots
+// Units that stand for a tile's own cost, and those of a CTA's interval at least.
+constexpr int kRowsExtra = 2, kRowsMinUnits = 2;    // of 64 slots
+constexpr int kTilesExtra = 1, kTilesMinUnits = 2;  // of 128 slots
 constexpr int kMaxSms = 160;      // CTAs whose parts fit the workspace
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -26,6 +27,37 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// 2^x on the FMA units, for x in [-125, 127]: x = n + r, r in [-1/2, 1/2], a
+// degree-5 polynomial for 2^r (least relative error, 2.1e-7 as evaluated), n added
+// to the exponent.  Below -125: 2^-125, or 0.
+template <bool kZero>
+__device__ __forceinline__ float2 exp2_poly(float2 x0) {
+    float2 x = x0;
+    const float2 shift = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
+    x.x = fmaxf(x.x, -125.f);
+    x.y = fmaxf(x.y, -125.f);
+    const float2 t = __fadd2_rn(x, shift);  // the nearest integer, in the low bits
+    const float2 n = __fadd2_rn(t, back);
+    const float2 r = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+    float2 p = __ffma2_rn(make_float2(0.0013276471f, 0.0013276471f), r, make_float2(0.009675541f, 0.009675541f));
+    p = __ffma2_rn(p, r, make_float2(0.05550713f, 0.05550713f));
+    p = __ffma2_rn(p, r, make_float2(0.2402212f, 0.2402212f));
+    p = __ffma2_rn(p, r, make_float2(0.69314694f, 0.69314694f));
+    p = __ffma2_rn(p, r, make_float2(1.0000001f, 1.0000001f));
+    p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23));
+    p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23));
+    if (kZero) {
+        p.x = x0.x >= -125.f ? p.x : max_nan(x0.x, 0.f);  // a NaN stays one
+        p.y = x0.y >= -125.f ? p.y : max_nan(x0.y, 0.f);
+    }
+    return p;
+}
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -64,28 +96,28 @@ bool encode_cache(CUtensorMap* map, const PagedView& c, void* base) {
     return encode(map, c.type, 4, base, dims, strides, box);
 }
 
-// q: (dim, head, token) in boxes of 64 dims x one KV head's group x as many whole tokens as 128 rows hold.
-bool encode_q(CUtensorMap* map, const AttnArgs& a) {
+// q: (dim, head, token) in boxes of 64 dims x one KV head's group x as many whole tokens as the rows hold.
+bool encode_q(CUtensorMap* map, const AttnArgs& a, int rows) {
     const int G = a.n_heads / a.c.n_kv;
     const cuuint64_t dims[3] = {(cuuint64_t)a.c.head_dim, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_tokens};
     const cuuint64_t strides[2] = {(cuuint64_t)a.c.head_dim * 2, (cuuint64_t)a.q_stride * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(128 / G)};
+    const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(rows / G)};
     return encode(map, a.c.type, 3, const_cast<char*>(a.q), dims, strides, box);
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------
 //
-// A step or a verify pass: a tile of 16, 32 or 64 rows, so each K and V byte
+// A step or a verify pass: a tile of 16 or 32 rows, so each K and V byte
 // serves few products and the cache's bytes bound the kernel.  One CTA per SM
 // walks its interval of 64-slot pages; a producer warp brings a page's K and V
 // (TMA boxes of 64 slots x 64 dims, 128-byte swizzle: the ldmatrix reads below
 // are free of bank conflicts) into a ring of as many pages as shared memory
-// holds, across tile borders.  Each of four warps takes 16 of a page's 64
+// holds, and the next tile's q, across tile borders.  Each of four warps takes 16 of a page's 64
 // slots, with a maximum, sum and f32 result of its own (m16n8k16, scores stay in
 // registers as the second product's operand), so that no page costs a barrier among them;
-// they are joined when the tile's part ends.  Up to 32 rows two such sets of
+// they are joined when the tile's part ends.  16 rows: two such sets of
 // four warps take the pages in turn (a page is a chain of dependent steps, two
-// chains fill each other's gaps); 64 rows are two sets of 32 on the same page.
+// chains fill each other's gaps).
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -108,51 +140,56 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&d)[4], const uint32
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// MW: 16-row tiles of a warp; WM: sets of four warps by rows; WP: by pages.
-template <int kD, int MW, int WM, int WP>
+// MW: 16-row tiles of a warp; WP: sets of four warps, by pages.
+template <int kD, int MW, int WP>
 struct RowsShape {
-    static constexpr int kRows = 16 * MW * WM;
-    static constexpr int kWarps = 4 * WM * WP;                 // consumers
+    static constexpr int kRows = 16 * MW;
+    static constexpr int kWarps = 4 * WP;                      // consumers; they share all rows
     static constexpr int kThreads = (kWarps + 1) * 32;
     static constexpr int kHalf = kPage * 128;                  // bytes of 64 slots x 64 dims
     static constexpr int kStage = 2 * (kD / 64) * kHalf;       // a page's K, then its V
-    static constexpr int kQ = kRows * kD * 2;
-    static constexpr int kPad = kD + 8;                        // floats of a joined row: no two rows on the same banks
-    static constexpr int kBufs = 2 * WP;                       // half of the warps that share a row
-    static constexpr int kJoin = kBufs * kRows * kPad * 4;
-    static constexpr int kRoom = 227 * 1024 - 1024 - 6144;     // alignment, static
-    static constexpr int kFit = (kRoom - kQ - kJoin) / kStage;
+    static constexpr int kQ = kRows * kD * 2;                  // one of two
+    static constexpr int kPad = kD + 8;                        // floats of a warp's result row: no two rows on the same banks
+    static constexpr int kJoin = kWarps * kRows * kPad * 4;
+    static constexpr int kRoom = 227 * 1024 - 1024 - 4096;     // alignment, static
+    static constexpr int kFit = (kRoom - 2 * kQ - kJoin) / kStage;
     // A stage always falls to the same set of warps: each waits for every fill
     // of its stages, or a barrier's parity would say nothing.
     static constexpr int kStages = (kFit > 12 ? 12 : kFit) / WP * WP;
-    static constexpr int kSmem = 1024 + kStages * kStage + kQ + kJoin;
+    static constexpr int kSmem = 1024 + kStages * kStage + 2 * kQ + kJoin;
 };
 constexpr int kPartRing = 8;
 
-template <class T, int kD, int MW, int WM, int WP>
-__global__ void __launch_bounds__(RowsShape<kD, MW, WM, WP>::kThreads, 1)
-    k_attention_rows(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
-    using S = RowsShape<kD, MW, WM, WP>;
+template <class T, int kD, int MW, int WP>
+__global__ void __launch_bounds__(RowsShape<kD, MW, WP>::kThreads, 1)
+    k_attention_rows(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                     const __grid_constant__ CUtensorMap q_map) {
+    using S = RowsShape<kD, MW, WP>;
     constexpr int kParts = kD / 64;  // 64-dim parts of a row
-    constexpr int kSplit = 4 * WP;   // warps that share a row
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full[S::kStages], empty[S::kStages], all_bar;
+    __shared__ uint64_t full[S::kStages], empty[S::kStages], q_full[2], q_empty[2], all_bar, read_bar;
     __shared__ PartRing<kPartRing> parts;
     __shared__ int s_page[S::kStages];  // the stage's page, negative: masked
     __shared__ long long s_scan[16];
-    __shared__ float s_m[WM][kSplit][16 * MW], s_l[WM][kSplit][16 * MW];
+    __shared__ float s_m[S::kWarps][S::kRows], s_l[S::kWarps][S::kRows];
     __shared__ int s_gave_up, s_last;
     const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;
-    uint8_t* q_at = smem_raw + (ring - smem_u32(smem_raw)) + S::kStages * S::kStage;
-    float* join = reinterpret_cast<float*>(q_at + S::kQ);
+    const uint32_t q_at = ring + S::kStages * S::kStage;
+    float* join = reinterpret_cast<float*>(smem_raw + (q_at - smem_u32(smem_raw)) + 2 * S::kQ);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Geometry ge{a.n_heads / a.c.n_kv, S::kRows, kPage};
+    const int G = a.n_heads / a.c.n_kv, per = S::kRows / G, live = per * G;  // whole tokens and rows of a tile
+    const Geometry ge{G, live, kPage, kRowsExtra};
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kStages; ++i) {
             bar_init(&full[i], 1);
-            bar_init(&empty[i], 4 * WM);
+            bar_init(&empty[i], 4);
+        }
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&q_full[i], 1);
+            bar_init(&q_empty[i], S::kWarps);
         }
         bar_init(&all_bar, S::kWarps);
+        bar_init(&read_bar, S::kWarps);
         parts.init(S::kWarps);
         s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -160,6 +197,7 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM, WP>::kThreads, 1)
     if (threadIdx.x == S::kWarps * 32) {
         tma_prefetch(&k_map);
         tma_prefetch(&v_map);
+        tma_prefetch(&q_map);
     }
     __syncthreads();
     const Line line = find_line<S::kThreads, CutRows>(a, ge, kRowsMinUnits, s_scan, warp == S::kWarps);
@@ -173,6 +211,14 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM, WP>::kThreads, 1)
         bool ok = true;
         while (ok && walk.next(&p)) {
             if (!parts.put(turn, p, &s_gave_up)) break;
+            const int qb = turn & 1;
+            if (turn >= 2 && !bar_wait(&q_empty[qb], ((turn >> 1) - 1) & 1, &s_gave_up)) break;
+            if (lane == 0) {
+                bar_expect(&q_full[qb], live * kD * 2);
+#pragma unroll
+                for (int h = 0; h < kParts; ++h)
+                    tma_load_3d(q_at + qb * S::kQ + h * (S::kRows * 128), &q_map, h * 64, p.head * G, p.tok0 + p.tile * per, &q_full[qb]);
+            }
             ++turn;
             for (int b0 = p.b0; ok && b0 < p.b1; b0 += 32) {
                 int mine = -1;
@@ -206,55 +252,42 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM, WP>::kThreads, 1)
         p.n = 0;
         parts.put(turn, p, &s_gave_up);
         // No copy is left in flight when the CTA ends: each stage's last fill has landed.
+        volatile int none = 0;
         for (int i = 0; i < S::kStages; ++i) {
             const int fills = round + (i < st ? 1 : 0);
-            volatile int none = 0;
             if (fills > 0) bar_wait(&full[i], (fills - 1) & 1, &none);
+        }
+        for (int i = 0; i < 2; ++i) {
+            const int fills = (turn + 1 - i) / 2;
+            if (fills > 0) bar_wait(&q_full[i], (fills - 1) & 1, &none);
         }
         if (lane == 0 && s_gave_up) flag(a.c, BAD_WAIT);
         return;
     }
 
-    const int wp = warp / (4 * WM), group = (warp / 4) % WM, sw = warp & 3;
-    const int share = wp * 4 + sw;                 // of the warps that share its rows
-    const int tid = threadIdx.x;                   // of the consumers
+    const int wp = warp >> 2, sw = warp & 3;
     const float to_log2 = a.scale * kLog2e;
     SyncPoint all{&all_bar, 0, &s_gave_up};
-    int st = 0, mine = 0;                          // mine: whose turn the stage is
+    int st = 0, mine = 0;  // mine: whose turn the stage is
     unsigned phase = 0;
     for (unsigned turn = 0; parts.get(turn, &p, &s_gave_up); ++turn) {
         const int base = p.len - p.n_new;  // the first new token's slot
-        const int rows = min(S::kRows, p.n_new * ge.G - p.tile * S::kRows);
-        bool ok = true;
-        // The tile's q rows, swizzled like K; rows that are none are 0.
-        for (int i = tid; i < S::kRows * (kD / 8); i += S::kWarps * 32) {
-            const int r = i / (kD / 8), ch = i % (kD / 8);
-            long long token;
-            int head;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (r < rows && row_place(ge, p, r, &token, &head))
-                x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + token * a.q_stride + (long long)head * kD + ch * 8);
-            *reinterpret_cast<uint4*>(q_at + (ch / 8) * (S::kRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) * 16)) = x;
-        }
-        // Slots that the thread's rows see: [0, base + token(r) + 1); least, most: of the warp's rows.
+        const int rows = min(live, p.n_new * G - p.tile * live);
+        const int first = p.tile * per;    // the tile's first token
+        // Slots that the thread's rows see: [0, base + token(r) + 1); least, most: of the tile's rows.
         int sees[MW][2];
 #pragma unroll
         for (int mt = 0; mt < MW; ++mt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = group * 16 * MW + mt * 16 + e * 8 + lane / 4;
-                sees[mt][e] = r < rows ? base + (p.tile * S::kRows + r) / ge.G + 1 : 0;
-            }
-        const int r0 = group * 16 * MW, r1 = min(r0 + 16 * MW, rows) - 1;
-        const int least = r1 == r0 + 16 * MW - 1 ? base + (p.tile * S::kRows + r0) / ge.G + 1 : 0;
-        const int most = r1 >= r0 ? base + (p.tile * S::kRows + r1) / ge.G + 1 : 0;
-        all.sync();
-        const uint32_t qa = smem_u32(q_at);
+            for (int e = 0; e < 2; ++e) sees[mt][e] = base + first + (mt * 16 + e * 8 + lane / 4) / G + 1;
+        const int least = base + first + 1, most = base + min(first + per, p.n_new);
+        bool ok = bar_wait(&q_full[turn & 1], (turn >> 1) & 1, &s_gave_up);
+        const uint32_t qa = q_at + (turn & 1) * S::kQ;
         uint32_t q[MW == 1 ? kD / 16 : 1][4];
         if constexpr (MW == 1) {
 #pragma unroll
             for (int kk = 0; kk < kD / 16; ++kk) {
-                const int r = group * 16 + (lane & 15), ch = kk * 2 + (lane >> 4);
+                const int r = lane & 15, ch = kk * 2 + (lane >> 4);
                 ldsm4(q[kk], qa + (ch / 8) * (S::kRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) * 16));
             }
         }
@@ -268,7 +301,7 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM, WP>::kThreads, 1)
             m[mt][0] = m[mt][1] = -INFINITY;
             l[mt][0] = l[mt][1] = 0.f;
         }
-        for (int b = p.b0; b < p.b1; ++b) {
+        for (int b = p.b0; ok && b < p.b1; ++b) {
             const bool here = mine == wp;
             const int at = st;
             const unsigned parity = phase;
@@ -301,7 +334,7 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM, WP>::kThreads, 1)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) qf[e] = q[kk][e];
                         } else {
-                            const int r = group * 16 * MW + mt * 16 + (lane & 15), qc = kk * 2 + (lane >> 4);
+                            const int r = mt * 16 + (lane & 15), qc = kk * 2 + (lane >> 4);
                             ldsm4(qf, qa + (qc / 8) * (S::kRows * 128) + r * 128 + (((qc & 7) ^ (r & 7)) * 16));
                         }
                         mma16<T>(s[mt][0], qf, kf[0], kf[1]);
@@ -328,11 +361,11 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM, WP>::kThreads, 1)
                         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
                     }
                     // The maximum follows only when it has grown by more than 8.
-                    const bool grown = top[0] > m[mt][0] + 8.f || top[1] > m[mt][1] + 8.f;
-                    if (__any_sync(0xffffffffu, grown)) {
+                    const bool grown[2] = {top[0] > m[mt][0] + 8.f, top[1] > m[mt][1] + 8.f};
+                    if (__any_sync(0xffffffffu, grown[0] || grown[1])) {
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const float to = fmaxf(m[mt][e], top[e]);
+                            const float to = grown[e] ? top[e] : m[mt][e];  // a row goes by its own scores alone
                             const float f = to == -INFINITY ? 1.f : exp2_fast(m[mt][e] - to);
                             m[mt][e] = to;
                             l[mt][e] *= f;
@@ -359,9 +392,9 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM, WP>::kThreads, 1)
                 const bool tail = s0 + 16 > p.len;
                 uint32_t lo_on = 0xffffffffu, hi_on = 0xffffffffu;
                 if (tail) {
-                    const int first = s0 + (lane & 3) * 2;
-                    lo_on = (first < p.len ? 0xffffu : 0u) | (first + 1 < p.len ? 0xffff0000u : 0u);
-                    hi_on = (first + 8 < p.len ? 0xffffu : 0u) | (first + 9 < p.len ? 0xffff0000u : 0u);
+                    const int first_slot = s0 + (lane & 3) * 2;
+                    lo_on = (first_slot < p.len ? 0xffffu : 0u) | (first_slot + 1 < p.len ? 0xffff0000u : 0u);
+                    hi_on = (first_slot + 8 < p.len ? 0xffffu : 0u) | (first_slot + 9 < p.len ? 0xffff0000u : 0u);
                 }
 #pragma unroll
                 for (int nd = 0; nd < kD / 16; ++nd) {
@@ -384,73 +417,51 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM, WP>::kThreads, 1)
             __syncwarp();
             if (lane == 0) bar_arrive(&empty[at]);
         }
-        // The warps that share a row joined: maxima, then the scaled results, half of them stored, half added.
+        __syncwarp();
+        if (lane == 0) bar_arrive(&q_empty[turn & 1]);
+        // Every warp leaves its results in shared memory, once all are through with the last tile's.
+        if (turn > 0) bar_wait(&read_bar, (turn - 1) & 1, &s_gave_up);
 #pragma unroll
         for (int mt = 0; mt < MW; ++mt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+                const int r = mt * 16 + e * 8 + lane / 4;
                 l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 1);
                 l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 2);
+                if (r >= rows) continue;
                 if ((lane & 3) == 0) {
-                    s_m[group][share][mt * 16 + e * 8 + lane / 4] = m[mt][e];
-                    s_l[group][share][mt * 16 + e * 8 + lane / 4] = l[mt][e];
+                    s_m[warp][r] = m[mt][e];
+                    s_l[warp][r] = l[mt][e];
                 }
+#pragma unroll
+                for (int n = 0; n < kD / 8; ++n)
+                    *reinterpret_cast<float2*>(join + (warp * S::kRows + r) * S::kPad + n * 8 + (lane & 3) * 2) =
+                        make_float2(o[mt][n][2 * e], o[mt][n][2 * e + 1]);
             }
         all.sync();
-        float* buf = join + ((share % S::kBufs) * S::kRows + group * 16 * MW) * S::kPad;
-#pragma unroll
-        for (int add = 0; add < 2; ++add) {
-            if ((share < S::kBufs) == (add == 1)) {
-#pragma unroll
-                for (int mt = 0; mt < MW; ++mt)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int r = mt * 16 + e * 8 + lane / 4;
-                        if (group * 16 * MW + r >= rows) continue;
-                        float top = -INFINITY;
-#pragma unroll
-                        for (int x = 0; x < kSplit; ++x) top = fmaxf(top, s_m[group][x][r]);
-                        const float f = m[mt][e] == -INFINITY ? 0.f : exp2f(m[mt][e] - top);
-#pragma unroll
-                        for (int n = 0; n < kD / 8; ++n) {
-                            float2* to = reinterpret_cast<float2*>(buf + r * S::kPad + n * 8 + (lane & 3) * 2);
-                            float2 x = make_float2(o[mt][n][2 * e] * f, o[mt][n][2 * e + 1] * f);
-                            if (add == 1) {
-                                const float2 y = *to;
-                                x.x += y.x;
-                                x.y += y.y;
-                            }
-                            *to = x;
-                        }
-                    }
-            }
-            all.sync();
-        }
         const bool whole = p.b1 - p.b0 == p.n;
         float* part = whole ? nullptr : part_at<S::kRows, kD>(a, blockIdx.x, p.b0 == 0);
-        for (int i = tid; ok && i < rows * (kD / 4); i += S::kWarps * 32) {
-            const int r = i / (kD / 4), col = i % (kD / 4) * 4, g = r / (16 * MW), gr = r % (16 * MW);
+        for (int i = threadIdx.x; ok && i < rows * (kD / 4); i += S::kWarps * 32) {
+            const int r = i / (kD / 4), col = i % (kD / 4) * 4;
             float top = -INFINITY, sum = 0.f;
-#pragma unroll
-            for (int x = 0; x < kSplit; ++x) top = fmaxf(top, s_m[g][x][gr]);
-#pragma unroll
-            for (int x = 0; x < kSplit; ++x) {
-                const float mx = s_m[g][x][gr];
-                sum += s_l[g][x][gr] * (mx == -INFINITY ? 0.f : exp2f(mx - top));
-            }
             float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int x = 0; x < S::kBufs; ++x) {
+            for (int x = 0; x < S::kWarps; ++x) top = fmaxf(top, s_m[x][r]);
+            const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int x = 0; x < S::kWarps; ++x) {
+                const float f = exp2_fast(s_m[x][r] - from);
                 const float4 y = *reinterpret_cast<const float4*>(join + (x * S::kRows + r) * S::kPad + col);
-                z.x += y.x;
-                z.y += y.y;
-                z.z += y.z;
-                z.w += y.w;
+                sum = __fmaf_rn(s_l[x][r], f, sum);
+                z.x = __fmaf_rn(y.x, f, z.x);
+                z.y = __fmaf_rn(y.y, f, z.y);
+                z.z = __fmaf_rn(y.z, f, z.z);
+                z.w = __fmaf_rn(y.w, f, z.w);
             }
-            long long token;
-            int head;
-            row_place(ge, p, r, &token, &head);
             if (whole) {
+                long long token;
+                int head;
+                row_place(ge, p, r, &token, &head);
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
                 store4<T>(reinterpret_cast<T*>(a.out) + token * a.out_stride + (long long)head * kD + col,
                           make_float4(z.x * inv, z.y * inv, z.z * inv, z.w * inv));
@@ -463,22 +474,26 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WM, WP>::kThreads, 1)
                 }
             }
         }
+        __syncwarp();
+        if (lane == 0) bar_arrive(&read_bar);
         if (!whole) {
             all.sync();
-            if (tid == 0) s_last = part_is_last(a, p);
+            if (threadIdx.x == 0) s_last = part_is_last(a, p);
             all.sync();
             if (s_last) join_parts<T, S::kRows, kD, S::kWarps>(a, ge, p, warp);
         }
     }
 }
 
-template <class T, int kD, int MW, int WM, int WP>
+template <class T, int kD, int MW, int WP>
 cudaError_t launch_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int sms, cudaStream_t s) {
-    using S = RowsShape<kD, MW, WM, WP>;
-    auto* kernel = k_attention_rows<T, kD, MW, WM, WP>;
+    using S = RowsShape<kD, MW, WP>;
+    CUtensorMap qm;
+    if (!encode_q(&qm, a, S::kRows)) return cudaErrorInvalidValue;
+    auto* kernel = k_attention_rows<T, kD, MW, WP>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     if (e != cudaSuccess) return e;
-    kernel<<<sms, S::kThreads, S::kSmem, s>>>(a, km, vm);
+    kernel<<<sms, S::kThreads, S::kSmem, s>>>(a, km, vm, qm);
     return cudaGetLastError();
 }
 
@@ -501,6 +516,9 @@ constexpr int kTileThreads = 384;  // warps 0-3 and 4-7: the halves; 8: products
 constexpr int kHalfRegs = 224, kOtherRegs = 56;
 constexpr int kTileEntries = 4;    // ring of K and V blocks, in turn
 constexpr int kBadRing = 16;       // blocks whose bad-page bits are kept
+// Of eight pairs of exponentials, those that go to the FMA units (the polynomial
+// above) and not to the special function units, which would bound the kernel alone.
+constexpr int kPolyOf8 = 3;
 
 template <int kD>
 struct TileShape {
@@ -517,7 +535,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     constexpr int kParts = kD / 64;
     constexpr bool kBf16 = !std::is_same<T, __half>::value;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full[kTileEntries], empty[kTileEntries], q_full[2], q_empty, s_full[2], p_full[2], o_full[2], all_bar, drained;
+    __shared__ uint64_t full[kTileEntries], empty[kTileEntries], q_full[2], q_empty, s_full[2], p_full[2][2], o_full[2], all_bar, drained;
     __shared__ PartRing<kPartRing> parts;
     __shared__ long long s_scan[16];
     __shared__ int s_bad[kBadRing];  // bit 0, 1: the block's pages that are masked
@@ -528,7 +546,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // A half has as many whole tokens as 128 rows hold.
     const int G = a.n_heads / a.c.n_kv, per = 128 / G, live = per * G;
-    const Geometry ge{G, 2 * live, kTileBlock};
+    const Geometry ge{G, 2 * live, kTileBlock, kTilesExtra};
     if (threadIdx.x == 0) {
         for (int i = 0; i < kTileEntries; ++i) {
             bar_init(&full[i], 1);
@@ -537,7 +555,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int h = 0; h < 2; ++h) {
             bar_init(&q_full[h], 1);
             bar_init(&s_full[h], 1);
-            bar_init(&p_full[h], 4);
+            bar_init(&p_full[h][0], 4);
+            bar_init(&p_full[h][1], 4);
             bar_init(&o_full[h], 1);
         }
         bar_init(&q_empty, 1);
@@ -688,18 +707,23 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         if (!ok || h >= halves) break;
-                        ok = bar_wait_warp(&p_full[h], p_phase[h], &s_gave_up);
+                        // P comes in two halves of the block's slots; the first one's products hide the second one's making.
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            ok = ok && bar_wait_warp(&p_full[h][g], p_phase[h], &s_gave_up);
+                            if (!ok) break;
+                            tc_fence_after();
+                            if (elect_one()) {
+#pragma unroll
+                                for (int kk = g * (kTileBlock / 32); kk < (g + 1) * (kTileBlock / 32); ++kk)
+                                    tc_mma_ts(t_at + 256 + h * 128, t_at + h * 128 + kk * 8, v_lo + ve * (S::kEntry / 16) + kk * (2048 / 16),
+                                              kPv, b > b0 || kk > 0);
+                                if (g == 1 && !more) tc_commit(&o_full[h]);
+                            }
+                            __syncwarp();
+                        }
                         if (!ok) break;
                         p_phase[h] ^= 1;
-                        tc_fence_after();
-                        if (elect_one()) {
-#pragma unroll
-                            for (int kk = 0; kk < kTileBlock / 16; ++kk)
-                                tc_mma_ts(t_at + 256 + h * 128, t_at + h * 128 + kk * 8, v_lo + ve * (S::kEntry / 16) + kk * (2048 / 16), kPv,
-                                          b > b0 || kk > 0);
-                            if (!more) tc_commit(&o_full[h]);
-                        }
-                        __syncwarp();
                         if (more) qk(h, e);
                     }
                     if (!ok) break;
@@ -756,31 +780,32 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     const int bad = s_bad[slot];
                     slot = (slot + 1) % kBadRing;
                     const int s0 = b * kTileBlock;
-                    if (s0 + kTileBlock > least) {
+                    if (s0 + kTileBlock > least || bad) {
 #pragma unroll
-                        for (int i = 0; i < 128; ++i)
-                            if (s0 + i >= sees) s[i] = -INFINITY;
-                    }
-                    if (bad) {
+                        for (int c = 0; c < 4; ++c) {
+                            const int n = sees - s0 - c * 32;  // slots of these 32 that the row sees
+                            unsigned on = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
+                            if ((bad >> (c / 2)) & 1) on = 0u;
 #pragma unroll
-                        for (int i = 0; i < 128; ++i)
-                            if ((bad >> (i / kPage)) & 1) s[i] = -INFINITY;
+                            for (int i = 0; i < 32; ++i)
+                                if (!((on >> i) & 1)) s[c * 32 + i] = -INFINITY;
+                        }
                     }
+                    // A NaN among the scores makes the maximum NaN, and with it the row.
                     float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int i = 4; i < 128; i += 8)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            top[j] = i + 4 + j < 128 ? fmaxf(fmaxf(top[j], s[i + j]), s[i + 4 + j]) : fmaxf(top[j], s[i + j]);
-                    top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    for (int i = 4; i < 128; ++i) top[i & 3] = max_nan(top[i & 3], s[i]);
+                    top[0] = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
                     const float reach = top[0] * to_log2;
-                    if (__any_sync(0xffffffffu, reach > m + 8.f)) {
-                        const float to = fmaxf(m, reach);
+                    const bool grown = !(reach <= m + 8.f);
+                    if (__any_sync(0xffffffffu, grown)) {
+                        float to = grown ? max_nan(m, reach) : m;  // a row goes by its own scores alone
+                        if (to == INFINITY) to = NAN;
                         const float f = to == -INFINITY ? 1.f : exp2_fast(m - to);
                         m = to;
                         l *= f;
                         if (b > p.b0) {
-#pragma unroll
+#pragma unroll 1
                             for (int c = 0; c < kD / 32; ++c) {
                                 float o[32];
                                 tmem_ld32<0>(o, t_o + c * 32);
@@ -801,53 +826,60 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             float2 x = __ffma2_rn(make_float2(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), by, from);
-                            x.x = exp2_fast(x.x);
-                            x.y = exp2_fast(x.y);
+                            if (i % 8 < kPolyOf8) {
+                                x = exp2_poly<false>(x);
+                            } else {
+                                x.x = exp2_fast(x.x);
+                                x.y = exp2_fast(x.y);
+                            }
                             sum[i & 1] = __fadd2_rn(sum[i & 1], x);
                             pk[i] = pack2<T>(x.x, x.y);
                         }
                         tmem_st16<0>(t_s + c * 16, pk);
+                        if (c & 1) {
+                            tmem_wait_st();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) bar_arrive(&p_full[half][c >> 1]);
+                        }
                     }
-                    tmem_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(&p_full[half]);
                     l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                }
+                if (m == -INFINITY && l == l) l = 0.f;  // nothing seen: the polynomial leaves 2^-125 for 2^-inf
+                long long token = 0;
+                int head = 0;
+                const bool row = row_place(ge, p, r, &token, &head);
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                T* out = reinterpret_cast<T*>(a.out) + token * a.out_stride + (long long)head * kD;
+                float* part = whole ? nullptr : part_at<kTileRows2, kD>(a, blockIdx.x, p.b0 == 0);
+                if (ok && row && whole && a.lse) a.lse[token * a.n_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+                if (ok && row && !whole) {
+                    part[r] = m;
+                    part[kTileRows2 + r] = l;
+                    part += 2 * kTileRows2 + r * kD;
                 }
                 if (ok && bar_wait(&o_full[half], o_phase, &s_gave_up)) {
                     o_phase ^= 1;
                     tc_fence_after();
-                    long long token = 0;
-                    int head = 0;
-                    const bool row = row_place(ge, p, r, &token, &head);
-                    float* part = whole ? nullptr : part_at<kTileRows2, kD>(a, blockIdx.x, p.b0 == 0);
-                    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < kD / 32; ++c) {
                         float o[32];
                         tmem_ld32<0>(o, t_o + c * 32);
                         tmem_wait_ld();
                         if (!row) continue;
                         if (whole) {
-                            T* out = reinterpret_cast<T*>(a.out) + token * a.out_stride + (long long)head * kD + c * 32;
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 float x[8];
 #pragma unroll
                                 for (int k = 0; k < 8; ++k) x[k] = o[i * 8 + k] * inv;
-                                store_vec<T, 8>(out + i * 8, x);
+                                store_vec<T, 8>(out + c * 32 + i * 8, x);
                             }
                         } else {
 #pragma unroll
                             for (int i = 0; i < 8; ++i)
-                                *reinterpret_cast<float4*>(part + 2 * kTileRows2 + r * kD + c * 32 + i * 4) =
-                                    make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                                *reinterpret_cast<float4*>(part + c * 32 + i * 4) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                         }
-                    }
-                    if (row && whole && a.lse) a.lse[token * a.n_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-                    if (row && !whole) {
-                        part[r] = m;
-                        part[kTileRows2 + r] = l;
                     }
                 }
             } else {
@@ -870,7 +902,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 template <class T, int kD>
 cudaError_t launch_tiles(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int sms, cudaStream_t s) {
     CUtensorMap qm;
-    if (!encode_q(&qm, a)) return cudaErrorInvalidValue;
+    if (!encode_q(&qm, a, 128)) return cudaErrorInvalidValue;
     auto* kernel = k_attention_tiles<T, kD>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<kD>::kSmem);
     if (e != cudaSuccess) return e;
@@ -881,59 +913,91 @@ cudaError_t launch_tiles(const AttnArgs& a, const CUtensorMap& km, const CUtenso
 // ---- weights, few rows ---------------------------------------------------------------------------------------------
 //
 // weight[slot] += sum over rows exp2(s - lse log2 e), s formed again: K is read
-// a second time (from L2 as far as it still lies there), V is not.  As above, each of
-// four warps takes 16 slots of a page; a thread adds its rows' probabilities of
+// a second time (from L2 as far as it still lies there), V is not.  As above, a
+// set of four warps takes a page, 16 slots a warp, two sets in turn; a thread adds its rows' probabilities of
 // its columns, and eight lanes' sums make a slot's.  All rows of a (sequence, KV head)
 // pass over the part's pages 64 at a time, so nothing is joined between CTAs.
 constexpr int kWRows = 64;
-constexpr int kWThreads = 160;
+constexpr int kWWarps = 8, kWThreads = (kWWarps + 1) * 32;
 
 template <int kD>
 struct WRowsShape {
     static constexpr int kStage = (kD / 64) * kPage * 128;
     static constexpr int kQ = kWRows * kD * 2;
-    static constexpr int kStages = 8;
-    static constexpr int kSmem = 1024 + kStages * kStage + kQ;
+    static constexpr int kStages = 10;  // even: a stage falls to one set of warps
+    static constexpr int kSmem = 1024 + kStages * kStage + 2 * kQ;
 };
 
 template <class T, int kD>
-__global__ void __launch_bounds__(kWThreads, 1) k_weights_rows(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map) {
+__global__ void __launch_bounds__(kWThreads, 1)
+    k_weights_rows(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap q_map) {
     using S = WRowsShape<kD>;
     constexpr int kParts = kD / 64, kHalf = kPage * 128;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full[S::kStages], empty[S::kStages], all_bar;
+    __shared__ uint64_t full[S::kStages], empty[S::kStages], q_full[2], q_empty[2], all_bar;
     __shared__ PartRing<kPartRing> parts;
     __shared__ int s_page[S::kStages];
     __shared__ long long s_scan[16];
-    __shared__ float s_lse[kWRows];
+    __shared__ float s_lse[2][kWRows];
     __shared__ int s_gave_up;
     const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;
-    uint8_t* q_at = smem_raw + (ring - smem_u32(smem_raw)) + S::kStages * S::kStage;
+    const uint32_t q_at = ring + S::kStages * S::kStage;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Geometry ge{a.n_heads / a.c.n_kv, kWRows, kPage};
+    const int G = a.n_heads / a.c.n_kv, per = kWRows / G, live = per * G;  // tokens and rows that pass at once
+    const Geometry ge{G, live, kPage, 1};
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kStages; ++i) {
             bar_init(&full[i], 1);
             bar_init(&empty[i], 4);
         }
-        bar_init(&all_bar, 4);
-        parts.init(4);
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&q_full[i], 1);
+            bar_init(&q_empty[i], kWWarps);
+        }
+        bar_init(&all_bar, kWWarps);
+        parts.init(kWWarps);
         s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (threadIdx.x == 128) tma_prefetch(&k_map);
+    if (threadIdx.x == kWWarps * 32) {
+        tma_prefetch(&k_map);
+        tma_prefetch(&q_map);
+    }
     __syncthreads();
-    const Line line = find_line<kWThreads, CutPages>(a, ge, kRowsMinUnits, s_scan, warp == 4);
+    const Line line = find_line<kWThreads, CutPages>(a, ge, kRowsMinUnits, s_scan, warp == kWWarps);
     Part p;
-    if (warp == 4) {
+    if (warp == kWWarps) {
         Walk<CutPages> walk(a, ge, line);
         int st = 0, round = 0;
-        unsigned turn = 0;
+        unsigned turn = 0, pass = 0;
         bool ok = true;
         while (ok && walk.next(&p)) {
             if (!parts.put(turn, p, &s_gave_up)) break;
             ++turn;
-            for (int r0 = 0; ok && r0 < p.n_new * ge.G; r0 += kWRows)
+            for (int t0 = 0; ok && t0 < p.n_new; t0 += per) {
+                const int qb = pass & 1;
+                if (pass >= 2 && !bar_wait(&q_empty[qb], ((pass >> 1) - 1) & 1, &s_gave_up)) {
+                    ok = false;
+                    break;
+                }
+#pragma unroll
+                for (int i = 0; i < kWRows / 32; ++i) {
+                    const int r = i * 32 + lane, tok = t0 + r / G;
+                    float x = INFINITY;  // exp2(s - inf) = 0: no row, or one that sees nothing
+                    if (r < live && tok < p.n_new) {
+                        x = a.lse[(long long)(p.tok0 + tok) * a.n_heads + p.head * G + r % G] * kLog2e;
+                        if (x == -INFINITY) x = INFINITY;
+                    }
+                    s_lse[qb][r] = x;
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    bar_expect(&q_full[qb], live * kD * 2);
+#pragma unroll
+                    for (int h = 0; h < kParts; ++h)
+                        tma_load_3d(q_at + qb * S::kQ + h * (kWRows * 128), &q_map, h * 64, p.head * G, p.tok0 + t0, &q_full[qb]);
+                }
+                ++pass;
                 for (int b0 = p.b0; ok && b0 < p.b1; b0 += 32) {
                     const int mine = b0 + lane < p.b1 ? page_of(a.c, p.seq, b0 + lane) : -1;
                     for (int b = b0; b < min(p.b1, b0 + 32); ++b) {
@@ -957,61 +1021,54 @@ __global__ void __launch_bounds__(kWThreads, 1) k_weights_rows(const __grid_cons
                         if (++st == S::kStages) st = 0, ++round;
                     }
                 }
+            }
         }
         p.n = 0;
         parts.put(turn, p, &s_gave_up);
+        volatile int none = 0;
         for (int i = 0; i < S::kStages; ++i) {
             const int fills = round + (i < st ? 1 : 0);
-            volatile int none = 0;
             if (fills > 0) bar_wait(&full[i], (fills - 1) & 1, &none);
+        }
+        for (int i = 0; i < 2; ++i) {
+            const int fills = (pass + 1 - i) / 2;
+            if (fills > 0) bar_wait(&q_full[i], (fills - 1) & 1, &none);
         }
         if (lane == 0 && s_gave_up) flag(a.c, BAD_WAIT);
         return;
     }
+    const int wp = warp >> 2, sw = warp & 3;
     const float to_log2 = a.scale * kLog2e;
-    int st = 0;
-    unsigned phase = 0;
     SyncPoint all{&all_bar, 0, &s_gave_up};
-    for (unsigned turn = 0; parts.get(turn, &p, &s_gave_up); ++turn) {
-        const int base = p.len - p.n_new, rows = p.n_new * ge.G;
-        bool ok = true;
-        for (int r0 = 0; r0 < rows; r0 += kWRows) {
-            p.tile = r0 / kWRows;  // row_place() below goes by it
-            all.sync();            // all are through with the last rows
-            for (int i = threadIdx.x; i < kWRows * (kD / 8); i += 128) {
-                const int r = i / (kD / 8), ch = i % (kD / 8);
-                long long token;
-                int head;
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (row_place(ge, p, r, &token, &head))
-                    x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + token * a.q_stride + (long long)head * kD + ch * 8);
-                *reinterpret_cast<uint4*>(q_at + (ch / 8) * (kWRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) * 16)) = x;
-            }
-            if (threadIdx.x < kWRows) {
-                long long token;
-                int head;
-                float x = INFINITY;  // exp2(s - inf) = 0: no row, or one that sees nothing
-                if (row_place(ge, p, threadIdx.x, &token, &head)) {
-                    x = a.lse[token * a.n_heads + head] * kLog2e;
-                    if (x == -INFINITY) x = INFINITY;
-                }
-                s_lse[threadIdx.x] = x;
-            }
-            all.sync();
-            const uint32_t qa = smem_u32(q_at);
-            const int tiles = (min(rows - r0, kWRows) + 15) / 16;
-            for (int b = p.b0; b < p.b1 && ok; ++b) {
-                if (!bar_wait(&full[st], phase, &s_gave_up)) {
+    int st = 0, mine = 0;
+    unsigned phase = 0, pass = 0;
+    bool ok = true;
+    for (unsigned turn = 0; ok && parts.get(turn, &p, &s_gave_up); ++turn) {
+        const int base = p.len - p.n_new;
+        for (int t0 = 0; ok && t0 < p.n_new; t0 += per, ++pass) {
+            if (t0 > 0) all.sync();  // another set's warps may have left these slots' sums
+            const int qb = pass & 1;
+            const int rows = min(per, p.n_new - t0) * G, tiles = (rows + 15) / 16;
+            ok = bar_wait(&q_full[qb], (pass >> 1) & 1, &s_gave_up);
+            const uint32_t qa = q_at + qb * S::kQ;
+            for (int b = p.b0; ok && b < p.b1; ++b) {
+                const bool here = mine == wp;
+                const int at = st;
+                const unsigned parity = phase;
+                if (++st == S::kStages) st = 0, phase ^= 1;
+                mine ^= 1;
+                if (!here) continue;
+                if (!bar_wait(&full[at], parity, &s_gave_up)) {
                     ok = false;
                     break;
                 }
-                const int s0 = b * kPage + warp * 16, page = s_page[st];
+                const int s0 = b * kPage + sw * 16, page = s_page[at];
                 if (page >= 0 && s0 < p.len) {
-                    const uint32_t kb = ring + st * S::kStage;
+                    const uint32_t kb = ring + at * S::kStage;
                     uint32_t kf[kD / 16][4];
 #pragma unroll
                     for (int kk = 0; kk < kD / 16; ++kk) {
-                        const int slot = warp * 16 + ((lane >> 4) << 3) + (lane & 7), ch = kk * 2 + ((lane >> 3) & 1);
+                        const int slot = sw * 16 + ((lane >> 4) << 3) + (lane & 7), ch = kk * 2 + ((lane >> 3) & 1);
                         ldsm4(kf[kk], kb + (ch / 8) * kHalf + slot * 128 + (((ch & 7) ^ (slot & 7)) * 16));
                     }
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -1029,13 +1086,12 @@ __global__ void __launch_bounds__(kWThreads, 1) k_weights_rows(const __grid_cons
                             mma16<T>(s[0], qf, kf[kk][0], kf[kk][1]);
                             mma16<T>(s[1], qf, kf[kk][2], kf[kk][3]);
                         }
-                        const int top = r0 + mt * 16;  // the tile's first row
-                        const bool mask = s0 + 16 > base + top / ge.G + 1 || top + 16 > rows;
+                        const bool mask = s0 + 16 > base + t0 + mt * 16 / G + 1 || mt * 16 + 16 > rows;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int r = mt * 16 + (e >> 1) * 8 + lane / 4;
-                            const float less = s_lse[r];
-                            const int sees = !mask ? INT_MAX : r0 + r < rows ? base + (r0 + r) / ge.G + 1 : 0;
+                            const float less = s_lse[qb][r];
+                            const int sees = !mask ? INT_MAX : r < rows ? base + t0 + r / G + 1 : 0;
 #pragma unroll
                             for (int n = 0; n < 2; ++n) {
                                 const float x = exp2_fast(__fmaf_rn(s[n][e], to_log2, -less));
@@ -1050,19 +1106,20 @@ __global__ void __launch_bounds__(kWThreads, 1) k_weights_rows(const __grid_cons
                         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 16);
                     }
                     if (lane < 4) {
-                        float* at = a.c.weight + ((long long)page * a.c.n_kv + p.head) * kPage + warp * 16;
-                        const float decay = r0 == 0 ? a.decay : 1.f;  // later rows add to what the first ones left
+                        float* to = a.c.weight + ((long long)page * a.c.n_kv + p.head) * kPage + sw * 16;
+                        const float decay = t0 == 0 ? a.decay : 1.f;  // later rows add to what the first ones left
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int off = (i >> 1) * 8 + lane * 2 + (i & 1);
-                            if (s0 + off < p.len) at[off] = decay == 0.f ? sum[i] : __fmaf_rn(decay, at[off], sum[i]);
+                            if (s0 + off < p.len) to[off] = decay == 0.f ? sum[i] : __fmaf_rn(decay, to[off], sum[i]);
                         }
                     }
                 }
                 __syncwarp();
-                if (lane == 0) bar_arrive(&empty[st]);
-                if (++st == S::kStages) st = 0, phase ^= 1;
+                if (lane == 0) bar_arrive(&empty[at]);
             }
+            __syncwarp();
+            if (lane == 0) bar_arrive(&q_empty[qb]);
         }
     }
 }
@@ -1104,7 +1161,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t q_at = k_at + 4 * S::kEntry;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.n_heads / a.c.n_kv, per = kWTileRows / G, live = per * G;  // tokens and rows of a row tile
-    const Geometry ge{G, kWTileRows, kWTileSlots};
+    const Geometry ge{G, kWTileRows, kWTileSlots, 0};
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             bar_init(&k_full[i], 1);
@@ -1218,6 +1275,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         if (r < live && tok < p.n_new) {
                             less = -a.lse[(long long)(p.tok0 + tok) * a.n_heads + p.head * G + r % G] * kLog2e;
                             sees = base + tok + 1;
+                            if (sees <= 0) less = 0.f;  // sees nothing: all masked, and -inf + inf would be NaN
                         }
                         s_less[e][r] = less;
                         s_sees[e][r] = sees;
@@ -1227,7 +1285,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 }
             }
         } else if (warp == 8) {
-            constexpr uint32_t kInstr = tc_instr(kBf16, kWTileRows, false);
+            const uint32_t kInstr = tc_instr(kBf16, kWTileRows, false) | (a.scale < 0.f ? kNegateA : 0u);
             const uint32_t t_at = uniform(tmem), k_lo = uniform(desc_lo_k(k_at)), q_lo = uniform(desc_lo_k(q_at));
             int e = 0, kt = 0, buf = 0;
             unsigned phase = 0, s_phase = 1;  // the first wait for an empty S passes
@@ -1272,7 +1330,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kHalfRegs));
         const int half = warp >> 2;
         const uint32_t t_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 256;
-        const float to_log2 = a.scale * kLog2e;
+        const float to_log2 = fmaxf(fabsf(a.scale), 1e-37f) * kLog2e;  // above 0: a masked -inf stays -inf
         const float2 by = make_float2(to_log2, to_log2);
         int e = 0, buf = 0;
         unsigned phase = 0, s_phase = 0;
@@ -1288,31 +1346,36 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 const int t0 = (q0 + b) * per;
                 // Some row is none, or does not see all of the half's slots.
                 const bool mask = live < kWTileRows || t0 + per > p.n_new || h0 + 128 > p.len - p.n_new + t0 + 1;
+                float s[128];
+                tmem_ld32<0>(s, t_s + buf * 128);
+                tmem_ld32<32>(s, t_s + buf * 128 + 32);
+                tmem_ld32<64>(s, t_s + buf * 128 + 64);
+                tmem_ld32<96>(s, t_s + buf * 128 + 96);
+                tmem_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&s_empty[half][buf]);
+                if (mask) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float s[32];
-                    tmem_ld32<0>(s, t_s + buf * 128 + c * 32);
-                    tmem_wait_ld();
-                    if (c == 3) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) bar_arrive(&s_empty[half][buf]);
+                    for (int i = 0; i < 32; ++i) {
+                        const int4 sees = *reinterpret_cast<const int4*>(&s_sees[e][i * 4]);
+                        if (slot >= sees.x) s[4 * i] = -INFINITY;
+                        if (slot >= sees.y) s[4 * i + 1] = -INFINITY;
+                        if (slot >= sees.z) s[4 * i + 2] = -INFINITY;
+                        if (slot >= sees.w) s[4 * i + 3] = -INFINITY;
                     }
+                }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float4 less = *reinterpret_cast<const float4*>(&s_less[e][c * 32 + i * 4]);
-                        float2 x = __ffma2_rn(make_float2(s[4 * i], s[4 * i + 1]), by, make_float2(less.x, less.y));
-                        float2 y = __ffma2_rn(make_float2(s[4 * i + 2], s[4 * i + 3]), by, make_float2(less.z, less.w));
-                        if (mask) {
-                            const int4 sees = *reinterpret_cast<const int4*>(&s_sees[e][c * 32 + i * 4]);
-                            x.x = slot < sees.x ? x.x : -INFINITY;
-                            x.y = slot < sees.y ? x.y : -INFINITY;
-                            y.x = slot < sees.z ? y.x : -INFINITY;
-                            y.y = slot < sees.w ? y.y : -INFINITY;
-                        }
-                        sum[0] = __fadd2_rn(sum[0], make_float2(exp2_fast(x.x), exp2_fast(x.y)));
-                        sum[1] = __fadd2_rn(sum[1], make_float2(exp2_fast(y.x), exp2_fast(y.y)));
-                    }
+                for (int i = 0; i < 32; ++i) {
+                    const float4 less = *reinterpret_cast<const float4*>(&s_less[e][i * 4]);
+                    float2 x = __ffma2_rn(make_float2(s[4 * i], s[4 * i + 1]), by, make_float2(less.x, less.y));
+                    float2 y = __ffma2_rn(make_float2(s[4 * i + 2], s[4 * i + 3]), by, make_float2(less.z, less.w));
+                    if (2 * i % 8 < kPolyOf8) x = exp2_poly<true>(x);
+                    else x.x = exp2_fast(x.x), x.y = exp2_fast(x.y);
+                    if ((2 * i + 1) % 8 < kPolyOf8) y = exp2_poly<true>(y);
+                    else y.x = exp2_fast(y.x), y.y = exp2_fast(y.y);
+                    sum[0] = __fadd2_rn(sum[0], x);
+                    sum[1] = __fadd2_rn(sum[1], y);
                 }
                 __syncwarp();
                 if (lane == 0) bar_arrive(&l_empty[e]);
@@ -1337,13 +1400,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 }
 
 template <class T, int kD>
-cudaError_t launch_weights(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& qm, int sms, cudaStream_t s) {
+cudaError_t launch_weights(const AttnArgs& a, const CUtensorMap& km, int sms, cudaStream_t s) {
     const long long rows = (long long)a.max_tokens * (a.n_heads / a.c.n_kv);
+    CUtensorMap qm;
+    if (!encode_q(&qm, a, rows <= kWRows ? kWRows : kWTileRows)) return cudaErrorInvalidValue;
     cudaError_t e;
     if (rows <= kWRows) {
         auto* kernel = k_weights_rows<T, kD>;
         if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WRowsShape<kD>::kSmem)) != cudaSuccess) return e;
-        kernel<<<sms, kWThreads, WRowsShape<kD>::kSmem, s>>>(a, km);
+        kernel<<<sms, kWThreads, WRowsShape<kD>::kSmem, s>>>(a, km, qm);
     } else {
         auto* kernel = k_weights_tiles<T, kD>;
         if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WTileShape<kD>::kSmem)) != cudaSuccess) return e;
@@ -1355,9 +1420,8 @@ cudaError_t launch_weights(const AttnArgs& a, const CUtensorMap& km, const CUten
 template <class T, int kD>
 cudaError_t launch_by_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int sms, cudaStream_t s) {
     const long long rows = (long long)a.max_tokens * (a.n_heads / a.c.n_kv);
-    if (rows <= 16) return launch_rows<T, kD, 1, 1, 2>(a, km, vm, sms, s);
-    if (rows <= 32) return launch_rows<T, kD, 2, 1, 2>(a, km, vm, sms, s);
-    if (rows <= 64) return launch_rows<T, kD, 2, 2, 1>(a, km, vm, sms, s);
+    if (rows <= 16) return launch_rows<T, kD, 1, 2>(a, km, vm, sms, s);
+    if (rows <= 32) return launch_rows<T, kD, 2, 1>(a, km, vm, sms, s);
     return launch_tiles<T, kD>(a, km, vm, sms, s);
 }
 
@@ -1385,10 +1449,10 @@ cudaError_t launch_paged_attention(const AttnArgs& a, cudaStream_t s) {
 }
 
 cudaError_t launch_attention_weights(const AttnArgs& a, cudaStream_t s) {
-    CUtensorMap km, qm;
+    CUtensorMap km;
     const int sms = sm_count();
-    if (sms == 0 || !encode_cache(&km, a.c, a.c.k) || !encode_q(&qm, a)) return cudaErrorInvalidValue;
-    return by_type(a.c, [&](auto t, auto d) { return launch_weights<decltype(t), decltype(d)::value>(a, km, qm, sms, s); });
+    if (sms == 0 || !encode_cache(&km, a.c, a.c.k)) return cudaErrorInvalidValue;
+    return by_type(a.c, [&](auto t, auto d) { return launch_weights<decltype(t), decltype(d)::value>(a, km, sms, s); });
 }
 
 }  // namespace mtb

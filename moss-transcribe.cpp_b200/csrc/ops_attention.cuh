@@ -4,7 +4,7 @@
 // Rows: the new tokens of a sequence times the query heads of one KV head,
 // row r = (token r / G, head r % G); a tile is some consecutive rows.  Units: a
 // tile's visible cache in blocks of slots (at least one).  All units of
-// all (sequence, KV head, tile) stand in one line, and CTA c of g takes the
+// all (sequence, KV head, tile) stand in one line, each tile behind some units for its own cost, and CTA c of g takes the
 // c-th of g equal intervals of it, whatever the lengths are.  A tile that lies in
 // one interval is finished there.  One that spans several leaves its parts (f32
 // sums, row maxima and row sums) in the workspace, and whichever CTA comes last
@@ -172,6 +172,7 @@ struct SeqWork {
 
 struct Geometry {
     int G, rows, block;  // query heads per KV head, rows per tile, slots per block
+    int extra;           // units that stand for a tile's own cost (its q, its end) before those of its blocks
 };
 
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int s) {
@@ -217,13 +218,13 @@ __device__ __forceinline__ long long head_units(const SeqWork& w, const Geometry
     const int tiles = Cut::tiles(w, ge);
     long long u = 0;
     if (tiles <= 4)
-        for (int t = 0; t < tiles; ++t) u += Cut::units(w, ge, t);
+        for (int t = 0; t < tiles; ++t) u += Cut::units(w, ge, t) + ge.extra;
     for (unsigned many = __ballot_sync(0xffffffffu, tiles > 4); many; many &= many - 1) {
         const int from = __ffs(many) - 1;
         const SeqWork x{__shfl_sync(0xffffffffu, w.len, from), 0, __shfl_sync(0xffffffffu, w.n_new, from)};
         const int n = __shfl_sync(0xffffffffu, tiles, from);
         long long sum = 0;
-        for (int t = lane; t < n; t += 32) sum += Cut::units(x, ge, t);
+        for (int t = lane; t < n; t += 32) sum += Cut::units(x, ge, t) + ge.extra;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == from) u = sum;
@@ -383,7 +384,7 @@ struct Walk {
         long long off = l.off - head * l.per;
         const int lane = threadIdx.x & 31;
         for (;; tile += 32) {  // 32 tiles at a time
-            long long x = tile + lane < tiles ? Cut::units(w, ge, tile + lane) : 0;
+            long long x = tile + lane < tiles ? Cut::units(w, ge, tile + lane) + ge.extra : 0;
             const long long v = x;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -400,7 +401,7 @@ struct Walk {
             off -= __shfl_sync(0xffffffffu, x, 31);
         }
         if (kWhole && block > 0) {
-            at += Cut::units(w, ge, tile) - block;
+            at += Cut::units(w, ge, tile) + ge.extra - block;
             step();
         }
     }
@@ -417,16 +418,19 @@ struct Walk {
         }
     }
     __device__ bool next(Part* p) {
-        if (at >= line.hi) return false;
-        const int n = Cut::units(w, ge, tile);
-        const int take = kWhole ? n : (int)min((long long)(n - block), line.hi - at);
-        const long long u0 = at - block;
-        const bool cut = !kWhole && take < n;
-        *p = Part{seq, head, tile, block, block + take, n, w.len, w.tok0, w.n_new, cut ? cta_of(line, u0) : 0, cut ? cta_of(line, u0 + n - 1) : 0};
-        at += take;
-        block += take;
-        if (block == n) step();
-        return true;
+        while (at < line.hi) {
+            const int n = Cut::units(w, ge, tile), all = n + ge.extra;
+            const int take = kWhole ? all : (int)min((long long)(all - block), line.hi - at);
+            const long long u0 = at - block;
+            const int b0 = max(0, block - ge.extra), b1 = block + take - ge.extra;
+            const bool cut = b0 > 0 || b1 < n;
+            *p = Part{seq, head, tile, b0, b1, n, w.len, w.tok0, w.n_new, cut ? cta_of(line, u0 + ge.extra) : 0, cut ? cta_of(line, u0 + all - 1) : 0};
+            at += take;
+            block += take;
+            if (block == all) step();
+            if (b1 > 0) return true;  // else the interval ended before the tile's first block
+        }
+        return false;
     }
 };
 
