@@ -40,6 +40,22 @@ struct RopeArgs {
     char* out;
 };
 
+// n / d for n < 2^31, without a division on the device: the high word of
+// n * m, m = ceil(2^(32 + s) / d), shifted by s (d <= 2^(s + 1)).
+struct FastDiv {
+    uint32_t m;
+    int s;
+    static FastDiv of(int d) {
+        FastDiv f{0, 0};
+        while ((2ll << f.s) < d) ++f.s;
+        f.m = d == 1 ? 0 : uint32_t(((1ull << (32 + f.s)) + d - 1) / d);
+        return f;
+    }
+#ifdef __CUDACC__
+    __device__ __forceinline__ int operator()(int n) const { return m ? int(__umulhi(uint32_t(n), m) >> s) : n; }
+#endif
+};
+
 struct AttnArgs {
     PagedView c;
     const int* cu;
@@ -53,6 +69,8 @@ struct AttnArgs {
     float* lse;        // written by the attention, read by the weights
     float decay;       // weights only
     char* workspace;
+    int G, per;         // query heads per KV head, new tokens per tile
+    FastDiv by_G, by_per;
 };
 
 struct EvictArgs {

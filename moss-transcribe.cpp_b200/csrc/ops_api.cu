@@ -115,6 +115,8 @@ int attention_args(const char* what, const mtb_paged_cache* cache, const int32_t
     a->q_stride = q_stride;
     a->n_heads = n_heads;
     a->scale = scale;
+    a->G = n_heads / cache->n_kv_heads;
+    a->by_G = FastDiv::of(a->G);
     return 0;
 }
 

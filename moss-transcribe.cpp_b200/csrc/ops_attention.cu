@@ -17,15 +17,10 @@ namespace {
 using namespace ops;
 
 // Units that stand for a tile's own cost, and those of a CTA's interval at least.
-constexpr int kRowsExtra = 2, kRowsMinUnits = 2;    // of 64 slots
-constexpr int kTilesExtra = 1, kTilesMinUnits = 2;  // of 128 slots
+constexpr int kRowsExtra = 2, kRowsMinUnits = 16;    // of 64 slots
+constexpr int kTilesExtra = 1, kTilesMinUnits = 4;  // of 128 slots
 constexpr int kMaxSms = 160;      // CTAs whose parts fit the workspace
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 __device__ __forceinline__ float max_nan(float a, float b) {
     float y;
@@ -98,7 +93,7 @@ bool encode_cache(CUtensorMap* map, const PagedView& c, void* base) {
 
 // q: (dim, head, token) in boxes of 64 dims x one KV head's group x as many whole tokens as the rows hold.
 bool encode_q(CUtensorMap* map, const AttnArgs& a, int rows) {
-    const int G = a.n_heads / a.c.n_kv;
+    const int G = a.G;
     const cuuint64_t dims[3] = {(cuuint64_t)a.c.head_dim, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_tokens};
     const cuuint64_t strides[2] = {(cuuint64_t)a.c.head_dim * 2, (cuuint64_t)a.q_stride * 2};
     const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(rows / G)};
@@ -177,8 +172,8 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WP>::kThreads, 1)
     const uint32_t q_at = ring + S::kStages * S::kStage;
     float* join = reinterpret_cast<float*>(smem_raw + (q_at - smem_u32(smem_raw)) + 2 * S::kQ);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int G = a.n_heads / a.c.n_kv, per = S::kRows / G, live = per * G;  // whole tokens and rows of a tile
-    const Geometry ge{G, live, kPage, kRowsExtra};
+    const int G = a.G, per = a.per, live = per * G;  // whole tokens and rows of a tile
+    const Geometry ge = geometry(a, kPage, kRowsExtra);
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kStages; ++i) {
             bar_init(&full[i], 1);
@@ -253,10 +248,12 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WP>::kThreads, 1)
         parts.put(turn, p, &s_gave_up);
         // No copy is left in flight when the CTA ends: each stage's last fill has landed.
         volatile int none = 0;
+        #pragma unroll 1
         for (int i = 0; i < S::kStages; ++i) {
             const int fills = round + (i < st ? 1 : 0);
             if (fills > 0) bar_wait(&full[i], (fills - 1) & 1, &none);
         }
+        #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
             const int fills = (turn + 1 - i) / 2;
             if (fills > 0) bar_wait(&q_full[i], (fills - 1) & 1, &none);
@@ -279,7 +276,7 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WP>::kThreads, 1)
 #pragma unroll
         for (int mt = 0; mt < MW; ++mt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) sees[mt][e] = base + first + (mt * 16 + e * 8 + lane / 4) / G + 1;
+            for (int e = 0; e < 2; ++e) sees[mt][e] = base + first + ge.by_G(mt * 16 + e * 8 + lane / 4) + 1;
         const int least = base + first + 1, most = base + min(first + per, p.n_new);
         bool ok = bar_wait(&q_full[turn & 1], (turn >> 1) & 1, &s_gave_up);
         const uint32_t qa = q_at + (turn & 1) * S::kQ;
@@ -441,6 +438,7 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WP>::kThreads, 1)
         all.sync();
         const bool whole = p.b1 - p.b0 == p.n;
         float* part = whole ? nullptr : part_at<S::kRows, kD>(a, blockIdx.x, p.b0 == 0);
+#pragma unroll 1
         for (int i = threadIdx.x; ok && i < rows * (kD / 4); i += S::kWarps * 32) {
             const int r = i / (kD / 4), col = i % (kD / 4) * 4;
             float top = -INFINITY, sum = 0.f;
@@ -478,11 +476,19 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WP>::kThreads, 1)
         if (lane == 0) bar_arrive(&read_bar);
         if (!whole) {
             all.sync();
-            if (threadIdx.x == 0) s_last = part_is_last(a, p);
+            if (threadIdx.x == 0) s_last = parts_if_last(a, p);
             all.sync();
-            if (s_last) join_parts<T, S::kRows, kD, S::kWarps>(a, ge, p, warp);
+            if (s_last) join_parts<T, S::kRows, kD, S::kWarps>(a, ge, p, s_last, all);
         }
     }
+}
+
+// The arguments with a tile of `rows` rows at most.
+AttnArgs with_tile(const AttnArgs& a, int rows) {
+    AttnArgs b = a;
+    b.per = rows / a.G;
+    b.by_per = FastDiv::of(b.per);
+    return b;
 }
 
 template <class T, int kD, int MW, int WP>
@@ -493,7 +499,7 @@ cudaError_t launch_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensor
     auto* kernel = k_attention_rows<T, kD, MW, WP>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     if (e != cudaSuccess) return e;
-    kernel<<<sms, S::kThreads, S::kSmem, s>>>(a, km, vm, qm);
+    kernel<<<sms, S::kThreads, S::kSmem, s>>>(with_tile(a, S::kRows), km, vm, qm);
     return cudaGetLastError();
 }
 
@@ -545,8 +551,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t q_at = ring + kTileEntries * S::kEntry;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // A half has as many whole tokens as 128 rows hold.
-    const int G = a.n_heads / a.c.n_kv, per = 128 / G, live = per * G;
-    const Geometry ge{G, 2 * live, kTileBlock, kTilesExtra};
+    const int G = a.G, per = a.per / 2, live = per * G;
+    const Geometry ge = geometry(a, kTileBlock, kTilesExtra);
     if (threadIdx.x == 0) {
         for (int i = 0; i < kTileEntries; ++i) {
             bar_init(&full[i], 1);
@@ -626,6 +632,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
             p.n = 0;
             parts.put(turn, p, &s_gave_up);
+            #pragma unroll 1
             for (int i = 0; i < kTileEntries; ++i) {  // every copy has landed before the CTA ends
                 const int fills = round + (i < e ? 1 : 0);
                 volatile int none = 0;
@@ -762,7 +769,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 bool ok = true;
                 float m = -INFINITY, l = 0.f;
                 const int first = (2 * p.tile + half) * per;  // the half's first token
-                const int sees = min(first + in_half / G, p.n_new - 1) + base + 1;
+                const int sees = min(first + ge.by_G(in_half), p.n_new - 1) + base + 1;
                 const int least = first + base + 1;           // slots that every row of the half sees
                 for (int b = p.b0; b < p.b1; ++b) {
                     if (!bar_wait(&s_full[half], s_phase, &s_gave_up)) {
@@ -887,9 +894,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
             if (!whole) {
                 all.sync();
-                if (threadIdx.x == 0) s_last = part_is_last(a, p);
+                if (threadIdx.x == 0) s_last = parts_if_last(a, p);
                 all.sync();
-                if (s_last) join_parts<T, kTileRows2, kD, 8>(a, ge, p, warp);
+                if (s_last) join_parts<T, kTileRows2, kD, 8>(a, ge, p, s_last, all);
             }
         }
     }
@@ -899,6 +906,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
+// A tile is two halves of whole tokens.
+AttnArgs two_halves(const AttnArgs& a) {
+    AttnArgs b = a;
+    b.per = 2 * (128 / a.G);
+    b.by_per = FastDiv::of(b.per);
+    return b;
+}
+
 template <class T, int kD>
 cudaError_t launch_tiles(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int sms, cudaStream_t s) {
     CUtensorMap qm;
@@ -906,7 +921,7 @@ cudaError_t launch_tiles(const AttnArgs& a, const CUtensorMap& km, const CUtenso
     auto* kernel = k_attention_tiles<T, kD>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<kD>::kSmem);
     if (e != cudaSuccess) return e;
-    kernel<<<sms, kTileThreads, TileShape<kD>::kSmem, s>>>(a, km, vm, qm);
+    kernel<<<sms, kTileThreads, TileShape<kD>::kSmem, s>>>(two_halves(a), km, vm, qm);
     return cudaGetLastError();
 }
 
@@ -943,8 +958,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
     const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;
     const uint32_t q_at = ring + S::kStages * S::kStage;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int G = a.n_heads / a.c.n_kv, per = kWRows / G, live = per * G;  // tokens and rows that pass at once
-    const Geometry ge{G, live, kPage, 1};
+    const int G = a.G, per = a.per, live = per * G;  // tokens and rows that pass at once
+    const Geometry ge = geometry(a, kPage, 1);
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kStages; ++i) {
             bar_init(&full[i], 1);
@@ -982,10 +997,10 @@ __global__ void __launch_bounds__(kWThreads, 1)
                 }
 #pragma unroll
                 for (int i = 0; i < kWRows / 32; ++i) {
-                    const int r = i * 32 + lane, tok = t0 + r / G;
+                    const int r = i * 32 + lane, tok = t0 + ge.by_G(r);
                     float x = INFINITY;  // exp2(s - inf) = 0: no row, or one that sees nothing
                     if (r < live && tok < p.n_new) {
-                        x = a.lse[(long long)(p.tok0 + tok) * a.n_heads + p.head * G + r % G] * kLog2e;
+                        x = a.lse[(long long)(p.tok0 + tok) * a.n_heads + p.head * G + r - ge.by_G(r) * G] * kLog2e;
                         if (x == -INFINITY) x = INFINITY;
                     }
                     s_lse[qb][r] = x;
@@ -1026,10 +1041,12 @@ __global__ void __launch_bounds__(kWThreads, 1)
         p.n = 0;
         parts.put(turn, p, &s_gave_up);
         volatile int none = 0;
+        #pragma unroll 1
         for (int i = 0; i < S::kStages; ++i) {
             const int fills = round + (i < st ? 1 : 0);
             if (fills > 0) bar_wait(&full[i], (fills - 1) & 1, &none);
         }
+        #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
             const int fills = (pass + 1 - i) / 2;
             if (fills > 0) bar_wait(&q_full[i], (fills - 1) & 1, &none);
@@ -1072,6 +1089,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
                         ldsm4(kf[kk], kb + (ch / 8) * kHalf + slot * 128 + (((ch & 7) ^ (slot & 7)) * 16));
                     }
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
                     for (int mt = 0; mt < tiles; ++mt) {
                         float s[2][4];
 #pragma unroll
@@ -1086,12 +1104,12 @@ __global__ void __launch_bounds__(kWThreads, 1)
                             mma16<T>(s[0], qf, kf[kk][0], kf[kk][1]);
                             mma16<T>(s[1], qf, kf[kk][2], kf[kk][3]);
                         }
-                        const bool mask = s0 + 16 > base + t0 + mt * 16 / G + 1 || mt * 16 + 16 > rows;
+                        const bool mask = s0 + 16 > base + t0 + ge.by_G(mt * 16) + 1 || mt * 16 + 16 > rows;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int r = mt * 16 + (e >> 1) * 8 + lane / 4;
                             const float less = s_lse[qb][r];
-                            const int sees = !mask ? INT_MAX : r < rows ? base + t0 + r / G + 1 : 0;
+                            const int sees = !mask ? INT_MAX : r < rows ? base + t0 + ge.by_G(r) + 1 : 0;
 #pragma unroll
                             for (int n = 0; n < 2; ++n) {
                                 const float x = exp2_fast(__fmaf_rn(s[n][e], to_log2, -less));
@@ -1160,8 +1178,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t k_at = (smem_u32(smem_raw) + 1023) & ~1023u;
     const uint32_t q_at = k_at + 4 * S::kEntry;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int G = a.n_heads / a.c.n_kv, per = kWTileRows / G, live = per * G;  // tokens and rows of a row tile
-    const Geometry ge{G, kWTileRows, kWTileSlots, 0};
+    const int G = a.G, per = a.per, live = per * G;  // tokens and rows of a row tile
+    const Geometry ge = geometry(a, kWTileSlots, 0);
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             bar_init(&k_full[i], 1);
@@ -1248,10 +1266,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             p.n = 0;
             parts.put(turn, p, &s_gave_up);
             volatile int none = 0;
+            #pragma unroll 1
             for (int i = 0; i < kWEntries; ++i) {
                 const int fills = round + (i < e ? 1 : 0);
                 if (fills > 0) bar_wait(&q_full[i], (fills - 1) & 1, &none);
             }
+            #pragma unroll 1
             for (int i = 0; i < 2; ++i) {
                 const int fills = (kt + 1 - i) / 2;
                 if (fills > 0) bar_wait(&k_full[i], (fills - 1) & 1, &none);
@@ -1269,11 +1289,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     }
 #pragma unroll
                     for (int i = 0; i < kWTileRows / 32; ++i) {
-                        const int r = i * 32 + lane, tok = (q0 + b) * per + r / G;
+                        const int r = i * 32 + lane, tok = (q0 + b) * per + ge.by_G(r);
                         float less = 0.f;
                         int sees = 0;
                         if (r < live && tok < p.n_new) {
-                            less = -a.lse[(long long)(p.tok0 + tok) * a.n_heads + p.head * G + r % G] * kLog2e;
+                            less = -a.lse[(long long)(p.tok0 + tok) * a.n_heads + p.head * G + r - ge.by_G(r) * G] * kLog2e;
                             sees = base + tok + 1;
                             if (sees <= 0) less = 0.f;  // sees nothing: all masked, and -inf + inf would be NaN
                         }
@@ -1401,25 +1421,25 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
 template <class T, int kD>
 cudaError_t launch_weights(const AttnArgs& a, const CUtensorMap& km, int sms, cudaStream_t s) {
-    const long long rows = (long long)a.max_tokens * (a.n_heads / a.c.n_kv);
+    const long long rows = (long long)a.max_tokens * a.G;
     CUtensorMap qm;
     if (!encode_q(&qm, a, rows <= kWRows ? kWRows : kWTileRows)) return cudaErrorInvalidValue;
     cudaError_t e;
     if (rows <= kWRows) {
         auto* kernel = k_weights_rows<T, kD>;
         if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WRowsShape<kD>::kSmem)) != cudaSuccess) return e;
-        kernel<<<sms, kWThreads, WRowsShape<kD>::kSmem, s>>>(a, km, qm);
+        kernel<<<sms, kWThreads, WRowsShape<kD>::kSmem, s>>>(with_tile(a, kWRows), km, qm);
     } else {
         auto* kernel = k_weights_tiles<T, kD>;
         if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WTileShape<kD>::kSmem)) != cudaSuccess) return e;
-        kernel<<<sms, kTileThreads, WTileShape<kD>::kSmem, s>>>(a, km, qm);
+        kernel<<<sms, kTileThreads, WTileShape<kD>::kSmem, s>>>(with_tile(a, kWTileRows), km, qm);
     }
     return cudaGetLastError();
 }
 
 template <class T, int kD>
 cudaError_t launch_by_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int sms, cudaStream_t s) {
-    const long long rows = (long long)a.max_tokens * (a.n_heads / a.c.n_kv);
+    const long long rows = (long long)a.max_tokens * a.G;
     if (rows <= 16) return launch_rows<T, kD, 1, 2>(a, km, vm, sms, s);
     if (rows <= 32) return launch_rows<T, kD, 2, 1>(a, km, vm, sms, s);
     return launch_tiles<T, kD>(a, km, vm, sms, s);

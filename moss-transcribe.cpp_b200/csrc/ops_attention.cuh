@@ -34,29 +34,23 @@ __device__ __forceinline__ void bar_arrive(uint64_t* b) {
 __device__ __forceinline__ void bar_expect(uint64_t* b, unsigned bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ unsigned long long now_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-constexpr unsigned long long kWaitNs = 4000000000ull;
+constexpr int kWaitTries = 1 << 22;  // at least some 50 ms; a wait here is for copies, products or warps of the same CTA
 
 // Waits for a phase; false once the wait ran out or another wait of this CTA
 // did (`gave_up`, shared memory), so that every role leaves its loop.
 __device__ __forceinline__ bool bar_wait(uint64_t* b, unsigned parity, volatile int* gave_up) {
     const uint32_t at = smem_u32(b);
-    unsigned long long t0 = 0;
-    for (unsigned it = 0;; ++it) {
+    int left = kWaitTries;
+#pragma unroll 1
+    for (;;) {
         uint32_t ok;
         asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
                      : "=r"(ok)
                      : "r"(at), "r"(parity)
                      : "memory");
         if (ok) return true;
-        if (it < 64) continue;  // the time is looked at once it has become long
-        if (it == 64) t0 = now_ns();
         if (*gave_up) return false;
-        if (now_ns() - t0 > kWaitNs) {
+        if (--left == 0) {
             *gave_up = 1;
             return false;
         }
@@ -77,6 +71,11 @@ struct SyncPoint {
     }
 };
 
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
@@ -166,14 +165,23 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, ui
 
 // ---- the line of units ---------------------------------------------------------------------------------------------
 
+constexpr int kMaxCtas = 1024;  // counters that fit the workspace
+
 struct SeqWork {
     int len, tok0, n_new;
 };
 
+// Tiles hold whole tokens, so that a tile's q is one box: `per` tokens, `rows` =
+// per G rows.
 struct Geometry {
-    int G, rows, block;  // query heads per KV head, rows per tile, slots per block
-    int extra;           // units that stand for a tile's own cost (its q, its end) before those of its blocks
+    int G, per, rows;
+    FastDiv by_G, by_per;
+    int block;  // slots per block
+    int extra;  // units that stand for a tile's own cost (its q, its end) before those of its blocks
 };
+__device__ __forceinline__ Geometry geometry(const AttnArgs& a, int block, int extra) {
+    return Geometry{a.G, a.per, a.per * a.G, a.by_G, a.by_per, block, extra};
+}
 
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int s) {
     const int b = a.cu[s], e = a.cu[s + 1], n = a.c.kv_len[s];  // together: none waits for another
@@ -188,26 +196,25 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int s) {
 
 // How a sequence's work under one KV head is cut: tiles, and units of a tile.
 struct CutRows {  // the attention: tiles of rows, in blocks of the slots that they see, at least one
-    static __device__ __forceinline__ int tiles(const SeqWork& w, const Geometry& ge) { return (w.n_new * ge.G + ge.rows - 1) / ge.rows; }
+    static __device__ __forceinline__ int tiles(const SeqWork& w, const Geometry& ge) { return ge.by_per(w.n_new + ge.per - 1); }
     static __device__ __forceinline__ int units(const SeqWork& w, const Geometry& ge, int tile) {
-        const int last = min(w.n_new - 1, ((tile + 1) * ge.rows - 1) / ge.G);
-        return max(1, (w.len - w.n_new + last + ge.block) / ge.block);
+        const int end = min(w.n_new, (tile + 1) * ge.per);
+        return max(1, (w.len - w.n_new + end + ge.block - 1) / ge.block);
     }
 };
 struct CutPages {  // the weights of few rows: one tile, in blocks of slots
     static __device__ __forceinline__ int tiles(const SeqWork& w, const Geometry&) { return w.n_new > 0 && w.len > 0; }
     static __device__ __forceinline__ int units(const SeqWork& w, const Geometry& ge, int) { return (w.len + ge.block - 1) / ge.block; }
 };
-struct CutSlots {  // the weights of many: tiles of slots, in tiles of the new tokens (rows / G each) that see some of them
+struct CutSlots {  // the weights of many: tiles of slots, in tiles of the new tokens that see some of them
     static __device__ __forceinline__ int tiles(const SeqWork& w, const Geometry& ge) {
         return w.n_new > 0 ? (w.len + ge.block - 1) / ge.block : 0;
     }
     static __device__ __forceinline__ int first(const SeqWork& w, const Geometry& ge, int tile) {
-        return max(0, tile * ge.block - (w.len - w.n_new)) / (ge.rows / ge.G);
+        return ge.by_per(max(0, tile * ge.block - (w.len - w.n_new)));
     }
     static __device__ __forceinline__ int units(const SeqWork& w, const Geometry& ge, int tile) {
-        const int per = ge.rows / ge.G;
-        return (w.n_new + per - 1) / per - first(w, ge, tile);
+        return ge.by_per(w.n_new + ge.per - 1) - first(w, ge, tile);
     }
 };
 // Units of a sequence under one KV head, one sequence a lane: few tiles by
@@ -218,12 +225,15 @@ __device__ __forceinline__ long long head_units(const SeqWork& w, const Geometry
     const int tiles = Cut::tiles(w, ge);
     long long u = 0;
     if (tiles <= 4)
+#pragma unroll 1
         for (int t = 0; t < tiles; ++t) u += Cut::units(w, ge, t) + ge.extra;
+#pragma unroll 1
     for (unsigned many = __ballot_sync(0xffffffffu, tiles > 4); many; many &= many - 1) {
         const int from = __ffs(many) - 1;
         const SeqWork x{__shfl_sync(0xffffffffu, w.len, from), 0, __shfl_sync(0xffffffffu, w.n_new, from)};
         const int n = __shfl_sync(0xffffffffu, tiles, from);
         long long sum = 0;
+#pragma unroll 1
         for (int t = lane; t < n; t += 32) sum += Cut::units(x, ge, t) + ge.extra;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -232,31 +242,41 @@ __device__ __forceinline__ long long head_units(const SeqWork& w, const Geometry
     return u;
 }
 
-// x * y / z of values that are mostly small: 32-bit division where it does.
-__device__ __forceinline__ long long mul_div(long long x, int y, long long z) {
-    if (x < (1 << 20) && y <= 1024 && z < (1ll << 31)) return (long long)((unsigned)x * (unsigned)y / (unsigned)z);
-    return x * y / z;
+// x / z for a quotient below 2^20: values mostly fit 32 bits, and where they do
+// not, bit by bit (a call of the 64-bit division would cost the kernels registers).
+__device__ __forceinline__ int div_small(long long x, long long z) {
+    if (x < (1ll << 32) && z < (1ll << 32)) return (int)((unsigned)x / (unsigned)z);
+    int q = 0;
+#pragma unroll 1
+    for (int bit = 1 << 19; bit; bit >>= 1)
+        if ((q | bit) * z <= x) q |= bit;
+    return q;
 }
-__device__ __forceinline__ long long div_small(long long x, long long z) {
-    return x < (1ll << 31) && z < (1ll << 31) ? (long long)((unsigned)x / (unsigned)z) : x / z;
+// total * b / parts, both below 2^11.
+__device__ __forceinline__ long long share_of(long long total, int b, int parts) {
+    const unsigned hi = (unsigned)(total >> 20), d = (unsigned)parts;
+    const unsigned q1 = hi / d, low = ((hi - q1 * d) << 20) | (unsigned)(total & 0xfffff), q0 = low / d;
+    return (((long long)q1 << 20) + q0) * b + (low - q0 * d) * (unsigned)b / d;
 }
 
 // The CTA's interval of the line, and where it begins.
 struct Line {
-    long long total, lo, hi;
+    long long total, tiles, lo, hi;
     int ctas;       // CTAs that have an interval
     int seq;        // sequence of unit lo
     long long off;  // of lo in that sequence's units
     long long per;  // that sequence's units under one KV head
 };
 
+// As many CTAs as there are, but fewer where their intervals would be shorter
+// than min_units, unless there is a tile for each.
 __device__ __forceinline__ void cut_line(Line* l, int min_units) {
-    const long long fit = max(1ll, div_small(l->total, min_units));
+    const long long fit = max(max(1ll, l->tiles), l->total / min_units);
     l->ctas = l->total ? (int)min((long long)gridDim.x, fit) : 0;
     l->lo = l->hi = 0;
     if ((int)blockIdx.x < l->ctas) {
-        l->lo = mul_div(l->total, blockIdx.x, l->ctas);
-        l->hi = mul_div(l->total, blockIdx.x + 1, l->ctas);
+        l->lo = share_of(l->total, blockIdx.x, l->ctas);
+        l->hi = share_of(l->total, blockIdx.x + 1, l->ctas);
     }
 }
 
@@ -278,6 +298,10 @@ __device__ Line find_line_warp(const AttnArgs& a, const Geometry& ge, int min_un
     }
     Line l{};
     l.total = __shfl_sync(0xffffffffu, x, 31);
+    int tiles = min(Cut::tiles(w, ge) * a.c.n_kv, kMaxCtas);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    l.tiles = tiles;
     cut_line(&l, min_units);
     const unsigned at = __ballot_sync(0xffffffffu, v > 0 && x - v <= l.lo && l.lo < x);
     l.seq = max(0, __ffs(at) - 1);
@@ -288,7 +312,7 @@ __device__ Line find_line_warp(const AttnArgs& a, const Geometry& ge, int min_un
 
 // Any number: all threads of the CTA; s_scan: one long long a warp + 3.
 template <int kThreads, class Cut>
-__device__ Line find_line_cta(const AttnArgs& a, const Geometry& ge, int min_units, long long* s_scan) {
+__device__ __noinline__ Line find_line_cta(const AttnArgs& a, const Geometry ge, int min_units, long long* s_scan) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     constexpr int kWarps = kThreads / 32;
     auto units_of = [&](int s, bool report) {
@@ -309,7 +333,9 @@ __device__ Line find_line_cta(const AttnArgs& a, const Geometry& ge, int min_uni
     if (lane == 0) s_scan[warp] = sum;
     __syncthreads();
     Line l{};
+#pragma unroll 1
     for (int w = 0; w < kWarps; ++w) l.total += s_scan[w];
+    l.tiles = kMaxCtas;  // more sequences than 32: hardly fewer tiles than CTAs
     cut_line(&l, min_units);
     long long base = 0;
     for (int s0 = 0; s0 < a.c.n_seq; s0 += kThreads) {
@@ -324,6 +350,7 @@ __device__ Line find_line_cta(const AttnArgs& a, const Geometry& ge, int min_uni
         if (lane == 31) s_scan[warp] = x;
         __syncthreads();
         long long before = base;
+#pragma unroll 1
         for (int w = 0; w < kWarps; ++w) {
             if (w < warp) before += s_scan[w];
             base += s_scan[w];
@@ -332,7 +359,7 @@ __device__ Line find_line_cta(const AttnArgs& a, const Geometry& ge, int min_uni
         if (v > 0 && first <= l.lo && l.lo < first + v) {
             s_scan[kWarps] = s0 + threadIdx.x;
             s_scan[kWarps + 1] = l.lo - first;
-            s_scan[kWarps + 2] = div_small(v, a.c.n_kv);
+            s_scan[kWarps + 2] = v / a.c.n_kv;
         }
     }
     __syncthreads();
@@ -352,17 +379,17 @@ __device__ __forceinline__ Line find_line(const AttnArgs& a, const Geometry& ge,
 }
 
 // The CTA whose interval holds unit u.
-__device__ __forceinline__ int cta_of(const Line& l, long long u) {
-    if (u < (1 << 20) && l.ctas <= 1024) return (int)(((unsigned)(u + 1) * (unsigned)l.ctas - 1) / (unsigned)l.total);
-    return (int)(((u + 1) * l.ctas - 1) / l.total);
-}
+__device__ __forceinline__ int cta_of(long long total, int ctas, long long u) { return div_small((u + 1) * ctas - 1, total); }
 
 // A CTA's part of one tile: blocks [b0, b1) of its n, with what the roles need
 // of its sequence.  n == 0: there are no more parts.
 struct Part {
     int seq, head, tile, b0, b1, n;
     int len, tok0, n_new;
-    int c0, c1;  // the CTAs that have parts of the tile
+    int ctas;  // of the line
+    long long u0, total;  // the tile's first block in the line of `total` units
+    __device__ int first_cta() const { return cta_of(total, ctas, u0); }
+    __device__ int last_cta() const { return cta_of(total, ctas, u0 + n - 1); }
 };
 
 // Walks the CTA's interval, one warp.  Whole: a tile goes undivided to the
@@ -380,7 +407,7 @@ struct Walk {
         if (l.lo >= l.hi) return;
         w = seq_work(a, seq);
         tiles = Cut::tiles(w, ge);
-        head = a.c.n_kv == 1 ? 0 : (int)div_small(l.off, l.per);
+        head = a.c.n_kv == 1 ? 0 : div_small(l.off, l.per);
         long long off = l.off - head * l.per;
         const int lane = threadIdx.x & 31;
         for (;; tile += 32) {  // 32 tiles at a time
@@ -423,8 +450,7 @@ struct Walk {
             const int take = kWhole ? all : (int)min((long long)(all - block), line.hi - at);
             const long long u0 = at - block;
             const int b0 = max(0, block - ge.extra), b1 = block + take - ge.extra;
-            const bool cut = b0 > 0 || b1 < n;
-            *p = Part{seq, head, tile, b0, b1, n, w.len, w.tok0, w.n_new, cut ? cta_of(line, u0 + ge.extra) : 0, cut ? cta_of(line, u0 + all - 1) : 0};
+            *p = Part{seq, head, tile, b0, b1, n, w.len, w.tok0, w.n_new, line.ctas, u0 + ge.extra, line.total};
             at += take;
             block += take;
             if (block == all) step();
@@ -472,7 +498,6 @@ struct PartRing {
 // CTA: of the tile that reached into its interval, and of the one that begins
 // there.  A part: row maxima (log2), row sums, f32 sums of p v.
 constexpr size_t kPartsAt = 8192;
-constexpr int kMaxCtas = 1024;  // counters that fit
 
 template <int kRows, int kD>
 __device__ __forceinline__ float* part_at(const AttnArgs& a, int cta, bool begins) {
@@ -483,11 +508,6 @@ __device__ __forceinline__ float* part_at(const AttnArgs& a, int cta, bool begin
 __device__ __forceinline__ float ld_cg(const float* p) {
     float x;
     asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(x) : "l"(p));
-    return x;
-}
-__device__ __forceinline__ float2 ld_cg2(const float* p) {
-    float2 x;
-    asm volatile("ld.global.cg.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "l"(p));
     return x;
 }
 __device__ __forceinline__ float4 ld_cg4(const float* p) {
@@ -509,102 +529,86 @@ __device__ __forceinline__ void store4(T* p, float4 x) {
 
 // Where row r of a part's tile goes; false: not a row of the sequence.
 __device__ __forceinline__ bool row_place(const Geometry& ge, const Part& p, int r, long long* token, int* head) {
-    const int row = p.tile * ge.rows + r;
-    if (r >= ge.rows || row >= p.n_new * ge.G) return false;
-    *token = p.tok0 + row / ge.G;
-    *head = p.head * ge.G + row % ge.G;
+    const int t = ge.by_G(r), tok = p.tile * ge.per + t;
+    if (t >= ge.per || tok >= p.n_new) return false;
+    *token = p.tok0 + tok;
+    *head = p.head * ge.G + r - t * ge.G;
     return true;
 }
 
-// Counts a part of a split tile as written; true for whom it was the last.
-// By one thread, between two barriers of the CTA: its release covers what the
-// others wrote before the first, its acquire what they read behind the second.
-__device__ __forceinline__ bool part_is_last(const AttnArgs& a, const Part& p) {
-    int* count = reinterpret_cast<int*>(a.workspace) + p.c0;
+// Counts a part of a split tile as written; the number of its parts for whom it was
+// the last, else 0.  By one thread, between two barriers of the CTA: its release
+// covers what the others wrote before the first, its acquire what they read behind the second.
+__device__ __forceinline__ int parts_if_last(const AttnArgs& a, const Part& p) {
+    const int c0 = p.first_cta(), parts = p.last_cta() - c0 + 1;
+    int* count = reinterpret_cast<int*>(a.workspace) + c0;
     int before;
     asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
-    const bool last = before == p.c1 - p.c0;
-    if (last) *count = 0;
-    return last;
+    if (before != parts - 1) return 0;
+    *count = 0;
+    return parts;
 }
 
-// Joins a split tile's parts, by kWarps warps: a warp a row, a lane a part's
-// maximum and sum and some columns; the columns' loads wait for nothing.
+// Joins a split tile's parts, by kWarps warps numbered from 0.  First each row's
+// factors, which take the maxima's place: few rows a warp each, a lane a part; many
+// rows a thread each.  Then the sums: four columns a thread, whose loads wait for nothing.
 template <class T, int kRows, int kD, int kWarps>
-__device__ __forceinline__ void join_parts(const AttnArgs& a, const Geometry& ge, const Part& p, int warp) {
-    constexpr int kCols = kD / 32, kBatch = 8;
-    const int rows = min(ge.rows, p.n_new * ge.G - p.tile * ge.rows);
-    const int lane = threadIdx.x & 31;
-    const int parts = p.c1 - p.c0 + 1;
-    int c_first = p.c0;
-    asm volatile("" : "+r"(c_first));  // addresses are formed here, not kept through the loops above
-    auto at = [&](int i) { return part_at<kRows, kD>(a, c_first + i, i == 0); };
+__device__ __forceinline__ void join_parts(const AttnArgs& a, const Geometry& ge, const Part& p, int parts, SyncPoint& all) {
+    const int rows = min(ge.rows, (p.n_new - p.tile * ge.per) * ge.G);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr size_t kStep = 2 * (size_t)kRows * (kD + 2);  // from a part to the next; the first is the one that begins the tile
+    float* first = part_at<kRows, kD>(a, p.first_cta(), true);
+    float* others = first - kStep / 2;  // part i > 0 at others + i kStep
+    const bool few = rows <= 32;
 #pragma unroll 1
-    for (int r = warp; r < rows; r += kWarps) {
-        float x[kBatch][kCols];
-        auto load = [&](int c0) {
-            const float* from = part_at<kRows, kD>(a, c_first + c0, false) + 2 * kRows + r * kD + lane * kCols;
+    for (int r = few ? warp : threadIdx.x; r < rows; r += few ? kWarps : kWarps * 32) {
+        const int c0 = few ? lane : 0, step = few ? 32 : 1;
+        float m = -INFINITY, sum = 0.f;
+#pragma unroll 2
+        for (int c = c0; c < parts; c += step) m = fmaxf(m, ld_cg((c ? others + c * kStep : first) + r));
+        if (few)
 #pragma unroll
-            for (int c = 0; c < kBatch; ++c)
-                if (c0 + c < parts) {
-                    const float* q = from + c * (2 * kRows * (kD + 2)) + (c == 0 && c0 == 0 ? kRows * (kD + 2) : 0);
-                    if constexpr (kCols == 4) {
-                        const float4 y = ld_cg4(q);
-                        x[c][0] = y.x, x[c][1] = y.y, x[c][2] = y.z, x[c][3] = y.w;
-                    } else {
-                        const float2 y = ld_cg2(q);
-                        x[c][0] = y.x, x[c][1] = y.y;
-                    }
-                }
-        };
-        load(0);
-        float mi = -INFINITY, li = 0.f;
-        if (lane < parts) {
-            mi = ld_cg(at(lane) + r);
-            li = ld_cg(at(lane) + kRows + r);
-        }
-        float m = mi;
-        for (int i = 32 + lane; i < parts; i += 32) m = fmaxf(m, ld_cg(at(i) + r));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         const float base = m == -INFINITY ? 0.f : m;
-        float o[kCols], sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < kCols; ++k) o[k] = 0.f;
-#pragma unroll 1
-        for (int c0 = 0; c0 < parts; c0 += 32) {
-            if (c0 > 0 && c0 + lane < parts) {
-                mi = ld_cg(at(c0 + lane) + r);
-                li = ld_cg(at(c0 + lane) + kRows + r);
-            }
-            const float f = c0 + lane < parts ? exp2f(mi - base) : 0.f;
-            sum += c0 + lane < parts ? f * li : 0.f;
-#pragma unroll 1
-            for (int h = 0; h < 32 && c0 + h < parts; h += kBatch) {
-                if (c0 + h > 0) load(c0 + h);
-#pragma unroll
-                for (int c = 0; c < kBatch; ++c) {
-                    const float fc = __shfl_sync(0xffffffffu, f, h + c);
-                    if (c0 + h + c < parts)
-#pragma unroll
-                        for (int k = 0; k < kCols; ++k) o[k] = __fmaf_rn(fc, x[c][k], o[k]);
-                }
-            }
+#pragma unroll 2
+        for (int c = c0; c < parts; c += step) {
+            const float* q = (c ? others + c * kStep : first) + r;
+            sum = __fmaf_rn(exp2_fast(ld_cg(q) - base), ld_cg(q + kRows), sum);
         }
+        if (few)
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll 2
+        for (int c = c0; c < parts; c += step) {
+            float* q = (c ? others + c * kStep : first) + r;
+            __stcg(q, exp2_fast(ld_cg(q) - base) * inv);
+        }
         long long token;
         int head;
-        row_place(ge, p, r, &token, &head);
-        T* out = reinterpret_cast<T*>(a.out) + token * a.out_stride + (long long)head * kD + lane * kCols;
-        if constexpr (kCols == 4) {
-            store4<T>(out, make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv));
-        } else {
-            out[0] = from_f32<T>(o[0] * inv);
-            out[1] = from_f32<T>(o[1] * inv);
+        if (c0 == 0 && a.lse && row_place(ge, p, r, &token, &head))
+            a.lse[token * a.n_heads + head] = sum == 0.f ? -INFINITY : (m + __log2f(sum)) * kLn2;
+    }
+    all.sync();
+    constexpr int kCols = kD / 4;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < rows * kCols; i += kWarps * 32) {
+        const int r = i / kCols, col = i % kCols * 4;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int c = 0; c < parts; ++c) {
+            const float* q = c ? others + c * kStep : first;
+            const float f = ld_cg(q + r);
+            const float4 x = ld_cg4(q + 2 * kRows + r * kD + col);
+            o.x = __fmaf_rn(f, x.x, o.x);
+            o.y = __fmaf_rn(f, x.y, o.y);
+            o.z = __fmaf_rn(f, x.z, o.z);
+            o.w = __fmaf_rn(f, x.w, o.w);
         }
-        if (lane == 0 && a.lse) a.lse[token * a.n_heads + head] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+        long long token;
+        int head;
+        if (row_place(ge, p, r, &token, &head))
+            store4<T>(reinterpret_cast<T*>(a.out) + token * a.out_stride + (long long)head * kD + col, o);
     }
 }
 
