@@ -497,7 +497,8 @@ cudaError_t launch_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensor
     CUtensorMap qm;
     if (!encode_q(&qm, a, S::kRows)) return cudaErrorInvalidValue;
     auto* kernel = k_attention_rows<T, kD, MW, WP>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(kernel, S::kSmem, &done);
     if (e != cudaSuccess) return e;
     kernel<<<sms, S::kThreads, S::kSmem, s>>>(with_tile(a, S::kRows), km, vm, qm);
     return cudaGetLastError();
@@ -919,7 +920,8 @@ cudaError_t launch_tiles(const AttnArgs& a, const CUtensorMap& km, const CUtenso
     CUtensorMap qm;
     if (!encode_q(&qm, a, 128)) return cudaErrorInvalidValue;
     auto* kernel = k_attention_tiles<T, kD>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<kD>::kSmem);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(kernel, TileShape<kD>::kSmem, &done);
     if (e != cudaSuccess) return e;
     kernel<<<sms, kTileThreads, TileShape<kD>::kSmem, s>>>(two_halves(a), km, vm, qm);
     return cudaGetLastError();
@@ -1427,11 +1429,13 @@ cudaError_t launch_weights(const AttnArgs& a, const CUtensorMap& km, int sms, cu
     cudaError_t e;
     if (rows <= kWRows) {
         auto* kernel = k_weights_rows<T, kD>;
-        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WRowsShape<kD>::kSmem)) != cudaSuccess) return e;
+        static std::atomic<uint64_t> done{0};
+        if ((e = allow_smem(kernel, WRowsShape<kD>::kSmem, &done)) != cudaSuccess) return e;
         kernel<<<sms, kWThreads, WRowsShape<kD>::kSmem, s>>>(with_tile(a, kWRows), km, qm);
     } else {
         auto* kernel = k_weights_tiles<T, kD>;
-        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WTileShape<kD>::kSmem)) != cudaSuccess) return e;
+        static std::atomic<uint64_t> done{0};
+        if ((e = allow_smem(kernel, WTileShape<kD>::kSmem, &done)) != cudaSuccess) return e;
         kernel<<<sms, kTileThreads, WTileShape<kD>::kSmem, s>>>(with_tile(a, kWTileRows), km, qm);
     }
     return cudaGetLastError();
@@ -1446,9 +1450,14 @@ cudaError_t launch_by_rows(const AttnArgs& a, const CUtensorMap& km, const CUten
 }
 
 int sm_count() {
+    static std::atomic<int> known[64];
     int device = 0, n = 0;
-    if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
-    return std::min(n, kMaxSms);
+    if (cudaGetDevice(&device) != cudaSuccess) return 0;
+    if (device < 64 && (n = known[device].load(std::memory_order_relaxed))) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
+    n = std::min(n, kMaxSms);
+    if (device < 64) known[device].store(n, std::memory_order_relaxed);
+    return n;
 }
 
 }  // namespace

@@ -3,12 +3,14 @@
 
 #include <algorithm>
 #include <climits>
+#include <cooperative_groups.h>
 #include <cstdint>
 
 namespace mtb {
 namespace {
 
 using namespace ops;
+namespace cg = cooperative_groups;
 
 // ---- mtb_rope_append ----------------------------------------------------------------------------------------------
 //
@@ -177,11 +179,14 @@ cudaError_t rope_typed(const RopeArgs& a, cudaStream_t s) {
 
 // ---- mtb_cache_evict ----------------------------------------------------------------------------------------------
 //
-// Two kernels.  k_evict_rank, one CTA per (sequence, KV head): each slot's rank
+// Two kernels.  The first, one cluster per (sequence, KV head): each slot's rank
 // as a 32-bit key (protected: all ones; else the weight's bits in ascending
 // order; NaN 0), the keep-th largest key by three passes of 11, 11 and 10 bits,
 // and lists of the gaps below `keep` and of the kept slots behind it.  Ties at
-// the threshold go to the lowest slots.  k_evict_move copies the listed rows:
+// the threshold go to the lowest slots.  k_evict_rank_regs holds eight slots a
+// thread in registers, in as many CTAs as that takes (four SMs for a half-hour
+// recording); k_evict_rank, one CTA, takes longer lists and books that are not 16-byte
+// aligned.  The second, k_evict_move, copies the listed rows:
 // sources lie at or behind `keep`, gaps below it, so no row is both and the
 // copies need no order.
 
@@ -339,11 +344,163 @@ __global__ void __launch_bounds__(kRankThreads) k_evict_rank(EvictArgs a) {
     if (threadIdx.x == 0) *head = EvictHead{min(moves, same), a.keep};
 }
 
+// Eight slots a thread.  What the cluster's CTAs tell one another (histograms,
+// counts) they read from one another's shared memory, behind cluster barriers.
+constexpr int kRankEach = 8;
+constexpr int kRankCopies = 4;  // of the histogram, by lane: neighbours' weights fall into the same few bins
+
+struct RankShared {
+    int hist[kRankCopies][kRankBins];
+    int warp[32];
+    int newest, bad, ties, gaps, come, pick, left;
+};
+
+__global__ void __launch_bounds__(kRankThreads) k_evict_rank_regs(EvictArgs a, int width) {
+    __shared__ __align__(16) RankShared sh;
+    cg::cluster_group cluster = cg::this_cluster();
+    const PagedView& c = a.c;
+    const int list = blockIdx.x / width, part = blockIdx.x % width, seq = list / c.n_kv, h = list % c.n_kv;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    char* ws = a.workspace + evict_workspace(1, 1, c.table_stride) * list;
+    EvictHead* head = reinterpret_cast<EvictHead*>(ws);
+    int* to = reinterpret_cast<int*>(ws + 256);
+    int* from = to + c.table_stride * (kPage / 2);
+    const int n = seq_len(c, seq);
+    if (n <= a.keep) {
+        if (part == 0 && threadIdx.x == 0) *head = EvictHead{0, n};
+        return;  // the whole cluster
+    }
+    const int i0 = (part * kRankThreads + threadIdx.x) * kRankEach;
+    const int mine = min(max(n - i0, 0), kRankEach);
+    int pos[kRankEach];
+    unsigned key[kRankEach];
+    int newest = INT_MIN;
+    if (threadIdx.x == 0) sh.bad = 0;
+    __syncthreads();
+    if (mine > 0) {
+        const int page = page_of(c, seq, i0 / kPage);
+        if (page < 0) {
+            sh.bad = 1;
+        } else {
+            const long long at = ((long long)page * c.n_kv + h) * kPage + i0 % kPage;
+            const int4 p0 = *reinterpret_cast<const int4*>(c.position + at), p1 = *reinterpret_cast<const int4*>(c.position + at + 4);
+            const float4 w0 = *reinterpret_cast<const float4*>(c.weight + at), w1 = *reinterpret_cast<const float4*>(c.weight + at + 4);
+            pos[0] = p0.x, pos[1] = p0.y, pos[2] = p0.z, pos[3] = p0.w, pos[4] = p1.x, pos[5] = p1.y, pos[6] = p1.z, pos[7] = p1.w;
+            const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+            for (int e = 0; e < kRankEach; ++e) {
+                key[e] = weight_key(w[e]);
+                if (e < mine) newest = max(newest, pos[e]);
+            }
+        }
+    }
+    newest = block_max(newest, sh.warp);
+    if (threadIdx.x == 0) sh.newest = newest;
+    cluster.sync();
+    int bad = 0;
+    for (int r = 0; r < width; ++r) {
+        const RankShared* o = cluster.map_shared_rank(&sh, r);
+        newest = max(newest, o->newest);
+        bad |= o->bad;
+    }
+    if (bad) {  // the same in all CTAs; a last barrier, for they read one another's
+        if (part == 0 && threadIdx.x == 0) *head = EvictHead{0, n};
+        cluster.sync();
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < kRankEach; ++e)
+        if (e < mine && (pos[e] < a.sinks || (long long)pos[e] > (long long)newest - a.recent)) key[e] = 0xffffffffu;
+    unsigned prefix = 0, known = 0;
+    int left = a.keep;
+    for (int pass = 0; pass < 3 && a.keep > 0; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+        for (int i = threadIdx.x; i < kRankCopies * kRankBins; i += kRankThreads) (&sh.hist[0][0])[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kRankEach; ++e)
+            if (e < mine && (key[e] & known) == prefix) atomicAdd(&sh.hist[threadIdx.x % kRankCopies][(key[e] >> shift) & (bins - 1)], 1);
+        cluster.sync();
+        // Bins from the top: thread t has bins 2047 - 2t and 2046 - 2t, of all CTAs.
+        const int b1 = kRankBins - 1 - 2 * threadIdx.x;
+        int c1 = 0, c0 = 0;
+        for (int r = 0; r < width; ++r) {
+            const RankShared* o = cluster.map_shared_rank(&sh, r);
+#pragma unroll
+            for (int k = 0; k < kRankCopies; ++k) {
+                const int2 x = *reinterpret_cast<const int2*>(&o->hist[k][b1 - 1]);
+                c0 += x.x;
+                c1 += x.y;
+            }
+        }
+        int total;
+        const int before = block_scan(c1 + c0, sh.warp, &total);
+        if (before < left && left <= before + c1) {
+            sh.pick = b1;
+            sh.left = left - before;
+        } else if (before + c1 < left && left <= before + c1 + c0) {
+            sh.pick = b1 - 1;
+            sh.left = left - before - c1;
+        }
+        cluster.sync();  // the histograms may be cleared, the pick be read
+        prefix |= (unsigned)sh.pick << shift;
+        known |= (unsigned)(bins - 1) << shift;
+        left = sh.left;
+    }
+    // Keys above prefix stay, and the first `left` of those equal to it.
+    int ties = 0, total;
+#pragma unroll
+    for (int e = 0; e < kRankEach; ++e) ties += e < mine && key[e] == prefix;
+    int tie = block_scan(ties, sh.warp, &total);
+    if (threadIdx.x == 0) sh.ties = total;
+    cluster.sync();
+    for (int r = 0; r < part; ++r) tie += cluster.map_shared_rank(&sh, r)->ties;
+    unsigned stays = 0;
+    int gaps = 0, come = 0;
+#pragma unroll
+    for (int e = 0; e < kRankEach; ++e) {
+        const bool st = e < mine && a.keep > 0 && (key[e] > prefix || (key[e] == prefix && tie++ < left));
+        stays |= (unsigned)st << e;
+        gaps += e < mine && !st && i0 + e < a.keep;
+        come += st && i0 + e >= a.keep;
+    }
+    int gap_total, come_total;
+    int g = block_scan(gaps, sh.warp, &gap_total);
+    int f = block_scan(come, sh.warp, &come_total);
+    if (threadIdx.x == 0) {
+        sh.gaps = gap_total;
+        sh.come = come_total;
+    }
+    cluster.sync();
+    int moves = 0;
+    for (int r = 0; r < width; ++r) {
+        const RankShared* o = cluster.map_shared_rank(&sh, r);
+        if (r < part) {
+            g += o->gaps;
+            f += o->come;
+        }
+        moves += o->gaps;
+    }
+#pragma unroll
+    for (int e = 0; e < kRankEach; ++e) {
+        const bool st = (stays >> e) & 1;
+        if (e < mine && !st && i0 + e < a.keep) to[g++] = i0 + e;
+        if (st && i0 + e >= a.keep) from[f++] = i0 + e;
+    }
+    if (part == 0 && threadIdx.x == 0) *head = EvictHead{moves, a.keep};
+    cluster.sync();  // nobody leaves while its counts are read
+}
+
 constexpr int kMoveThreads = 256;
+constexpr int kMoveBatch = 8;  // rows of a warp in flight
 
 __global__ void __launch_bounds__(kMoveThreads) k_evict_move(EvictArgs a, int lists) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the ranking still runs
     const PagedView& c = a.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per_row = c.head_dim / 8;  // 16-byte pieces of a K or V row
+    char* base = lane < per_row ? c.k : c.v;
+    const int piece = 16 * (lane % per_row);
     for (int l = blockIdx.y; l < lists; l += gridDim.y) {
         const int seq = l / c.n_kv, h = l % c.n_kv;
         const char* ws = a.workspace + evict_workspace(1, 1, c.table_stride) * l;
@@ -352,21 +509,30 @@ __global__ void __launch_bounds__(kMoveThreads) k_evict_move(EvictArgs a, int li
         const int* from = to + c.table_stride * (kPage / 2);
         const int* table = c.table + (long long)seq * c.table_stride;
         if (blockIdx.x == 0 && threadIdx.x == 0 && h == 0) a.new_len[seq] = head.new_len;
-        const int per_row = c.head_dim / 8;  // 16-byte pieces of a K or V row
-        for (int i = blockIdx.x * (kMoveThreads / 32) + warp; i < head.moves; i += gridDim.x * (kMoveThreads / 32)) {
-            const int d = to[i], f = from[i];
-            const long long pd = table[d / kPage], pf = table[f / kPage];
-            const long long od = pd * c.page_stride + h * c.head_stride + (long long)(d % kPage) * c.head_dim;
-            const long long of = pf * c.page_stride + h * c.head_stride + (long long)(f % kPage) * c.head_dim;
-            if (lane < 2 * per_row) {
-                char* base = lane < per_row ? c.k : c.v;
-                const int piece = lane % per_row;
-                const uint4 x = *reinterpret_cast<const uint4*>(base + 2 * of + 16 * piece);
-                *reinterpret_cast<uint4*>(base + 2 * od + 16 * piece) = x;
+        for (int i0 = (blockIdx.x * (kMoveThreads / 32) + warp) * kMoveBatch; i0 < head.moves; i0 += gridDim.x * (kMoveThreads / 32) * kMoveBatch) {
+            // A lane a row: its places, its weight and position.
+            long long od = 0, of = 0;
+            const int rows = min(kMoveBatch, head.moves - i0);
+            if (lane < rows) {
+                const int d = to[i0 + lane], f = from[i0 + lane];
+                const long long pd = table[d / kPage], pf = table[f / kPage];
+                const long long md = (pd * c.n_kv + h) * kPage + d % kPage, mf = (pf * c.n_kv + h) * kPage + f % kPage;
+                c.weight[md] = c.weight[mf];
+                c.position[md] = c.position[mf];
+                od = 2 * (pd * c.page_stride + h * c.head_stride + (long long)(d % kPage) * c.head_dim);
+                of = 2 * (pf * c.page_stride + h * c.head_stride + (long long)(f % kPage) * c.head_dim);
             }
-            const long long md = (pd * c.n_kv + h) * kPage + d % kPage, mf = (pf * c.n_kv + h) * kPage + f % kPage;
-            if (lane == 0) c.weight[md] = c.weight[mf];
-            if (lane == 1) c.position[md] = c.position[mf];
+            uint4 x[kMoveBatch];
+#pragma unroll
+            for (int r = 0; r < kMoveBatch; ++r) {
+                const long long o = __shfl_sync(0xffffffffu, of, r);
+                if (r < rows && lane < 2 * per_row) x[r] = *reinterpret_cast<const uint4*>(base + o + piece);
+            }
+#pragma unroll
+            for (int r = 0; r < kMoveBatch; ++r) {
+                const long long o = __shfl_sync(0xffffffffu, od, r);
+                if (r < rows && lane < 2 * per_row) *reinterpret_cast<uint4*>(base + o + piece) = x[r];
+            }
         }
     }
 }
@@ -382,16 +548,40 @@ cudaError_t launch_rope_append(const RopeArgs& a, cudaStream_t s) {
 
 cudaError_t launch_cache_evict(const EvictArgs& a, cudaStream_t s) {
     const int lists = a.c.n_seq * a.c.n_kv;
-    const long long slots = std::min<long long>((long long)a.c.table_stride * kPage, kRankKeys);
-    const int smem = int(slots) * 4;
-    cudaError_t e = cudaFuncSetAttribute(k_evict_rank, cudaFuncAttributeMaxDynamicSharedMemorySize, kRankKeys * 4);
+    const long long most_len = (long long)a.c.table_stride * kPage;
+    // As many CTAs a list as its longest needs with eight slots a thread.
+    int width = 1;
+    while (width < 8 && most_len > (long long)width * kRankThreads * kRankEach) width *= 2;
+    const bool regs = most_len <= (long long)width * kRankThreads * kRankEach && reinterpret_cast<uintptr_t>(a.c.position) % 16 == 0 &&
+                      reinterpret_cast<uintptr_t>(a.c.weight) % 16 == 0;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at[1];
+    cfg.stream = s;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaError_t e;
+    if (regs) {
+        cfg.gridDim = dim3(lists * width);
+        cfg.blockDim = dim3(kRankThreads);
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim = {(unsigned)width, 1, 1};
+        e = cudaLaunchKernelEx(&cfg, k_evict_rank_regs, a, width);
+    } else {
+        static std::atomic<uint64_t> done{0};
+        if ((e = allow_smem(k_evict_rank, kRankKeys * 4, &done)) != cudaSuccess) return e;
+        k_evict_rank<<<lists, kRankThreads, int(std::min<long long>(most_len, kRankKeys)) * 4, s>>>(a);
+        e = cudaGetLastError();
+    }
     if (e != cudaSuccess) return e;
-    k_evict_rank<<<lists, kRankThreads, smem, s>>>(a);
-    const long long most = std::min<long long>(a.keep, (long long)a.c.table_stride * kPage / 2);
-    const int rows = kMoveThreads / 32;
+    const long long most = std::min<long long>(a.keep, most_len / 2);
+    const int rows = kMoveThreads / 32 * kMoveBatch;
     const int wide = (int)std::max<long long>(1, std::min<long long>((most + rows - 1) / rows, 1 + 148 * 8 / lists));
-    k_evict_move<<<dim3(wide, std::min(lists, 65535)), kMoveThreads, 0, s>>>(a, lists);
-    return cudaGetLastError();
+    cfg.gridDim = dim3(wide, std::min(lists, 65535));
+    cfg.blockDim = dim3(kMoveThreads);
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    e = cudaLaunchKernelEx(&cfg, k_evict_move, a, lists);
+    return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 }  // namespace mtb

@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 namespace mtb {
 namespace ops {
 
@@ -99,6 +101,20 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
         for (int j = 0; j < per; ++j) t[j] = from_f32<T>(x[i * per + j]);
         *reinterpret_cast<uint4*>(p + i * per) = u;
     }
+}
+
+// Lets a kernel have that much dynamic shared memory, once on each device.
+template <class K>
+cudaError_t allow_smem(K* kernel, int bytes, std::atomic<uint64_t>* done, bool wide_clusters = false) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (device & 63);
+    if (done->load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && wide_clusters) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) done->fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 }  // namespace ops

@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import sys
 
 import numpy as np
@@ -562,20 +563,23 @@ def spec_run_group(decoders, max_steps: int = 0) -> int:
 
 
 # ---- operators on a caller's own device memory -----------------------------
+# A step's calls take a few microseconds on the device, so what is done here for each call is kept short.
 
-_TYPE_CODES = {}  # dtype object -> (name, element size), filled as dtypes are met
+
+class _Names(dict):
+    """dtype object -> its name, filled as dtypes are met."""
+
+    def __missing__(self, dtype):
+        name = self[dtype] = str(dtype).rsplit(".", 1)[-1]
+        return name
+
+
+_NAME = _Names()
 _CODES = {"float32": T_F32, "float16": T_F16, "bfloat16": T_BF16}
-
-
-def _dtype(t):
-    name = _TYPE_CODES.get(t.dtype)
-    if name is None:
-        name = _TYPE_CODES[t.dtype] = str(t.dtype).rsplit(".", 1)[-1]
-    return name
-
-
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
+_PACK_CACHE = struct.Struct("@PPiiiiqqPiiPPPP").pack  # mtb_paged_cache
+_PACK_LOGITS = struct.Struct("@PqPPPPPPPqPPPqiP").pack  # mtb_logits_params
+assert struct.calcsize("@PPiiiiqqPiiPPPP") == C.sizeof(PagedCacheView)
+assert struct.calcsize("@PqPPPPPPPqPPPqiP") == C.sizeof(LogitsParams)
 
 
 def _need(ok, what):
@@ -583,39 +587,44 @@ def _need(ok, what):
         raise MtbError(what)
 
 
-def _flat(t, name, dtype, n=None, device=None):
-    """The pointer of a tensor without gaps, 0 for None; n: the least number of its elements."""
+def _shape(t, name, dims):
+    shape = t.shape
+    if len(shape) != dims:
+        raise MtbError(f"{name} must have {dims} dimensions")
+    return shape
+
+
+def _flat(t, name, dtype, n, device):
+    """The pointer of a tensor without gaps on `device`, 0 for None; n: the least number of its elements."""
     if t is None:
         return 0
-    if _dtype(t) != dtype or not t.is_contiguous() or (n is not None and t.numel() < n) or (device is not None and t.device != device):
-        raise MtbError(f"{name} must be contiguous {dtype}" + (f" with at least {n} elements" if n is not None else "")
-                       + (f" on {device}" if device is not None else ""))
+    if _NAME[t.dtype] != dtype or not t.is_contiguous() or t.numel() < n or t.get_device() != device:
+        raise MtbError(f"{name} must be contiguous {dtype} with at least {n} elements on the others' device")
     return t.data_ptr()
 
 
-def _rows(t, name, heads, dim, device):
+def _rows(t, name, tokens, heads, dim, dtype, device):
     """(pointer, elements between tokens) of [tokens][heads][dim] whose tokens' rows have no gaps."""
-    sh, st = t.shape, t.stride()
-    if (len(sh) != 3 or (heads is not None and sh[1] != heads) or sh[2] != dim or st[2] != 1 or (sh[1] > 1 and st[1] != dim)
-            or t.device != device):
-        raise MtbError(f"{name} must be [tokens][{'heads' if heads is None else heads}][{dim}] on {device} with a token's rows "
-                       "contiguous")
-    return t.data_ptr(), (st[0] if sh[0] > 1 else max(st[0], sh[1] * dim))
+    if t.shape == (tokens, heads, dim) and _NAME[t.dtype] == dtype and t.get_device() == device:
+        s0, s1, s2 = t.stride()
+        if s2 == 1 and (s1 == dim or heads == 1):
+            return t.data_ptr(), (s0 if tokens > 1 else max(s0, heads * dim))
+    raise MtbError(f"{name} must be {dtype} [{tokens}][{heads}][{dim}] on the cache's device with a token's rows contiguous")
 
 
 def _space(t, device):
     """(pointer, bytes) of a workspace."""
-    if not t.is_contiguous() or t.device != device:
-        raise MtbError(f"workspace must be contiguous, on {device}")
+    if not t.is_contiguous() or t.get_device() != device:
+        raise MtbError("workspace must be contiguous, on the cache's device")
     return t.data_ptr(), t.numel() * t.element_size()
 
 
-def _stream(t, stream):
-    """A cudaStream_t: the one given, else torch's current stream of the tensor's device."""
+def _stream(device, stream):
+    """A cudaStream_t: the one given, else torch's current stream of the device."""
     if stream is not None:
         return stream if isinstance(stream, int) else stream.cuda_stream
     torch = sys.modules.get("torch")
-    return torch._C._cuda_getCurrentRawStream(t.device.index) if torch is not None and t.device.type == "cuda" else 0
+    return torch._C._cuda_getCurrentRawStream(device) if torch is not None and device >= 0 else 0
 
 
 def _ok(rc, what):
@@ -629,24 +638,26 @@ class PagedCache:
     [sequences] with the new tokens included; position (int32) and weight (f32) [pages][kv_heads][64] and status (int32,
     BAD_* bits) where wanted.  It keeps the tensors alive and may be used for any number of calls."""
 
+    __slots__ = ("kept", "heads", "dim", "type", "n_seq", "table_len", "device", "view")
+
     def __init__(self, k, v, page_table, kv_len, position=None, weight=None, status=None):
-        sh, st, name = k.shape, k.stride(), _dtype(k)
-        _need(len(sh) == 4 and sh[2] == PAGE and st[3] == 1 and st[2] == sh[3],
-              "k must be [pages][kv_heads][64][head_dim] with a page's rows contiguous")
-        _need(tuple(v.shape) == tuple(sh) and _dtype(v) == name and v.stride() == st, "v must have k's shape, strides and type")
-        _need(name in ("float16", "bfloat16"), "the cache's type is float16 or bfloat16")
-        _need(len(page_table.shape) == 2 and _dtype(page_table) == "int32" and page_table.is_contiguous() and page_table.device == k.device,
-              "page_table must be contiguous int32 [sequences][pages] on the cache's device")
-        n_seq, meta, dev = page_table.shape[0], sh[0] * sh[1] * PAGE, k.device
-        block = PAGE * sh[3]
+        shape, strides, name, device = k.shape, k.stride(), _NAME[k.dtype], k.get_device()
+        if len(shape) != 4 or shape[2] != PAGE or strides[3] != 1 or strides[2] != shape[3]:
+            raise MtbError("k must be [pages][kv_heads][64][head_dim] with a page's rows contiguous")
+        if v.shape != shape or v.stride() != strides or v.dtype != k.dtype or v.get_device() != device:
+            raise MtbError("v must have k's shape, strides, type and device")
+        if name != "float16" and name != "bfloat16":
+            raise MtbError("the cache's type is float16 or bfloat16")
+        pages, heads, _, dim = shape
+        n_seq, table_len = _shape(page_table, "page_table", 2)
+        meta, block = pages * heads * PAGE, PAGE * dim
         self.kept = (k, v, page_table, kv_len, position, weight, status)
-        self.heads, self.dim, self.type, self.n_seq, self.device = sh[1], sh[3], name, n_seq, dev
-        self.view = PagedCacheView(
-            k.data_ptr(), v.data_ptr(), _CODES[name], sh[3], sh[1], sh[0], st[0] if sh[0] > 1 else max(st[0], sh[1] * block),
-            st[1] if sh[1] > 1 else max(st[1], block), page_table.data_ptr(), page_table.shape[1], n_seq,
-            _flat(kv_len, "kv_len", "int32", n_seq, dev), _flat(position, "position", "int32", meta, dev),
-            _flat(weight, "weight", "float32", meta, dev), _flat(status, "status", "int32", 1, dev))
-        self.ref = C.byref(self.view)
+        self.heads, self.dim, self.type, self.n_seq, self.table_len, self.device = heads, dim, name, n_seq, table_len, device
+        self.view = _PACK_CACHE(
+            k.data_ptr(), v.data_ptr(), _CODES[name], dim, heads, pages, strides[0] if pages > 1 else max(strides[0], heads * block),
+            strides[1] if heads > 1 else max(strides[1], block), _flat(page_table, "page_table", "int32", 0, device), table_len, n_seq,
+            _flat(kv_len, "kv_len", "int32", n_seq, device), _flat(position, "position", "int32", meta, device),
+            _flat(weight, "weight", "float32", meta, device), _flat(status, "status", "int32", 1, device))
 
 
 def rope_frequencies(rotary_dim: int, base: float, kind: int = ROPE_PLAIN, factor: float = 1.0, original_len: float = 0.0,
@@ -664,18 +675,18 @@ def rope_append(cache: PagedCache, cu_tokens, positions, q, k, v, inv_freq, q_ou
     """Rotary positions of q and k and the append of k and v to the cache (mtb_rope_append).  q [tokens][heads][dim], k and v
     [tokens][kv_heads][dim] (views of a fused projection's rows will do), inv_freq float64 [rotary / 2], q_out of the
     cache's type.  Token i of a sequence's n goes to slot kv_len - n + i."""
-    n, heads = q.shape[0], q.shape[1]
-    qp, qs = _rows(q, "q", None, cache.dim, cache.device)
-    kp, ks = _rows(k, "k", cache.heads, cache.dim, cache.device)
-    vp, vs = _rows(v, "v", cache.heads, cache.dim, cache.device)
-    op, os_ = _rows(q_out, "q_out", heads, cache.dim, cache.device)
-    name = _dtype(q)
-    _need(k.shape[0] == n and v.shape[0] == n and q_out.shape[0] == n and _dtype(k) == name and _dtype(v) == name
-          and _dtype(q_out) == cache.type and name in _CODES, "q, k, v and q_out must agree in tokens and types")
-    _ok(lib().mtb_rope_append(cache.ref, _flat(cu_tokens, "cu_tokens", "int32", cache.n_seq + 1, cache.device), n,
-                              _flat(positions, "positions", "int32", n, cache.device), _CODES[name], qp, qs, heads, kp, ks, vp, vs,
-                              _flat(inv_freq, "inv_freq", "float64", None, cache.device), 2 * inv_freq.numel(), int(interleaved), factor, op, os_,
-                              _stream(q, stream)), "rope_append")
+    n, heads, _ = _shape(q, "q", 3)
+    name, dim, dev = _NAME[q.dtype], cache.dim, cache.device
+    qp, qs = _rows(q, "q", n, heads, dim, name, dev)
+    kp, ks = _rows(k, "k", n, cache.heads, dim, name, dev)
+    vp, vs = _rows(v, "v", n, cache.heads, dim, name, dev)
+    op, os_ = _rows(q_out, "q_out", n, heads, dim, cache.type, dev)
+    rc = lib().mtb_rope_append(cache.view, _flat(cu_tokens, "cu_tokens", "int32", cache.n_seq + 1, dev), n,
+                               _flat(positions, "positions", "int32", n, dev), _CODES.get(name, -1), qp, qs, heads, kp, ks, vp, vs,
+                               _flat(inv_freq, "inv_freq", "float64", 0, dev), 2 * inv_freq.numel(), interleaved, factor, op, os_,
+                               _stream(dev, stream))
+    if rc != 0:
+        _ok(rc, "rope_append")
 
 
 def paged_attention(cache: PagedCache, cu_tokens, q, out, workspace, lse=None, scale: float | None = None, max_tokens: int = 0,
@@ -683,24 +694,29 @@ def paged_attention(cache: PagedCache, cu_tokens, q, out, workspace, lse=None, s
     """Causal attention of the new tokens over the cache (mtb_paged_attention).  q and out [tokens][heads][dim] of the
     cache's type, lse f32 [tokens][heads]; workspace: ATTENTION_WORKSPACE bytes, zeroed once before its first use and not
     shared by calls that overlap."""
-    n, heads = q.shape[0], q.shape[1]
-    qp, qs = _rows(q, "q", None, cache.dim, cache.device)
-    op, os_ = _rows(out, "out", heads, cache.dim, cache.device)
-    _need(out.shape[0] == n and _dtype(q) == cache.type and _dtype(out) == cache.type, "q and out must agree, in the cache's type")
-    _ok(lib().mtb_paged_attention(cache.ref, _flat(cu_tokens, "cu_tokens", "int32", cache.n_seq + 1, cache.device), n, max_tokens, qp, qs, heads,
-                                  cache.dim ** -0.5 if scale is None else scale, op, os_, _flat(lse, "lse", "float32", n * heads, cache.device),
-                                  *_space(workspace, cache.device), _stream(q, stream)), "paged_attention")
+    n, heads, _ = _shape(q, "q", 3)
+    dim, dev = cache.dim, cache.device
+    qp, qs = _rows(q, "q", n, heads, dim, cache.type, dev)
+    op, os_ = _rows(out, "out", n, heads, dim, cache.type, dev)
+    wp, wn = _space(workspace, dev)
+    rc = lib().mtb_paged_attention(cache.view, _flat(cu_tokens, "cu_tokens", "int32", cache.n_seq + 1, dev), n, max_tokens, qp, qs, heads,
+                                   dim ** -0.5 if scale is None else scale, op, os_, _flat(lse, "lse", "float32", n * heads, dev), wp, wn,
+                                   _stream(dev, stream))
+    if rc != 0:
+        _ok(rc, "paged_attention")
 
 
 def attention_weights(cache: PagedCache, cu_tokens, q, lse, decay: float = 1.0, scale: float | None = None, max_tokens: int = 0,
                       stream=None):
     """cache weight = decay * weight + the softmax weight each position received in that attention (mtb_attention_weights)."""
-    n, heads = q.shape[0], q.shape[1]
-    qp, qs = _rows(q, "q", None, cache.dim, cache.device)
-    _need(_dtype(q) == cache.type, "q must have the cache's type")
-    _ok(lib().mtb_attention_weights(cache.ref, _flat(cu_tokens, "cu_tokens", "int32", cache.n_seq + 1, cache.device), n, max_tokens, qp, qs, heads,
-                                    cache.dim ** -0.5 if scale is None else scale, _flat(lse, "lse", "float32", n * heads, cache.device), decay,
-                                    _stream(q, stream)), "attention_weights")
+    n, heads, _ = _shape(q, "q", 3)
+    dim, dev = cache.dim, cache.device
+    qp, qs = _rows(q, "q", n, heads, dim, cache.type, dev)
+    rc = lib().mtb_attention_weights(cache.view, _flat(cu_tokens, "cu_tokens", "int32", cache.n_seq + 1, dev), n, max_tokens, qp, qs, heads,
+                                     dim ** -0.5 if scale is None else scale, _flat(lse, "lse", "float32", n * heads, dev), decay,
+                                     _stream(dev, stream))
+    if rc != 0:
+        _ok(rc, "attention_weights")
 
 
 def cache_evict_workspace(n_seq: int, n_kv_heads: int, table_stride: int) -> int:
@@ -711,8 +727,12 @@ def cache_evict_workspace(n_seq: int, n_kv_heads: int, table_stride: int) -> int
 def cache_evict(cache: PagedCache, keep: int, new_len, workspace, sinks: int = 0, recent: int = 0, stream=None):
     """Keep the `keep` slots of each longer sequence that rank highest, in place (mtb_cache_evict); new_len int32 [sequences]
     gets the lengths (it may be kv_len itself)."""
-    _ok(lib().mtb_cache_evict(cache.ref, keep, sinks, recent, _flat(new_len, "new_len", "int32", cache.n_seq, cache.device), *_space(workspace, cache.device),
-                              _stream(new_len, stream)), "cache_evict")
+    dev = cache.device
+    wp, wn = _space(workspace, dev)
+    rc = lib().mtb_cache_evict(cache.view, keep, sinks, recent, _flat(new_len, "new_len", "int32", cache.n_seq, dev), wp, wn,
+                               _stream(dev, stream))
+    if rc != 0:
+        _ok(rc, "cache_evict")
 
 
 def logits_process(logits, out=None, choice=None, history=None, hist_begin=None, hist_end=None, repetition=None, presence=None,
@@ -720,29 +740,33 @@ def logits_process(logits, out=None, choice=None, history=None, hist_begin=None,
                    stream=None):
     """Penalties, biases and masks on logits [rows][vocab], and the greedy choice (mtb_logits_process).  Row r's history is
     history[hist_begin[r]:hist_end[r]], its biases likewise; mask int32 or uint32 [mask rows][words], bit i % 32 of word i / 32."""
-    _need(len(logits.shape) == 2 and _dtype(logits) in _CODES, "logits must be [rows][vocab] of float32, float16 or bfloat16")
-    rows, vocab = logits.shape
-    st = logits.stride()
-    _need(st[1] == 1 or vocab == 1, "a logits row must be contiguous")
-    os_ = 0
+    rows, vocab = _shape(logits, "logits", 2)
+    name, dev, st = _NAME[logits.dtype], logits.get_device(), logits.stride()
+    _need(name in _CODES and (st[1] == 1 or vocab == 1), "logits must be [rows][vocab] of float32, float16 or bfloat16, rows contiguous")
+    op = os_ = 0
     if out is not None:
-        _need(tuple(out.shape) == (rows, vocab) and out.dtype == logits.dtype and out.device == logits.device and (out.stride()[1] == 1 or vocab == 1),
+        _need(out.shape == logits.shape and out.dtype == logits.dtype and out.get_device() == dev,
               "out must have the shape, type and device of logits")
-        os_ = out.stride()[0] if rows > 1 else max(out.stride()[0], vocab)
-    dev = logits.device
+        os_, s1 = out.stride()
+        _need(s1 == 1 or vocab == 1, "an out row must be contiguous")
+        op, os_ = out.data_ptr(), (os_ if rows > 1 else max(os_, vocab))
+    mp = ms = mn = 0
     if mask is not None:
-        _need(len(mask.shape) == 2 and _dtype(mask) in ("int32", "uint32") and mask.stride()[1] == 1 and mask.device == dev
-              and mask.shape[1] * 32 >= vocab and (mask_row is not None or mask.shape[0] >= rows),
+        mn, words = _shape(mask, "mask", 2)
+        ms, s1 = mask.stride()
+        _need(_NAME[mask.dtype] in ("int32", "uint32") and s1 == 1 and mask.get_device() == dev and words * 32 >= vocab
+              and (mask_row is not None or mn >= rows),
               "mask must be int32 [mask rows][vocab / 32 words], with a row for each logits row or mask_row given")
+        mp, ms = mask.data_ptr(), max(ms, words)
+    n_hist = 0 if history is None else history.numel()
     n_bias = 0 if bias_ids is None else bias_ids.numel()
-    p = LogitsParams(_flat(history, "history", "int32", None, dev), 0 if history is None else history.numel(),
-                     _flat(hist_begin, "hist_begin", "int32", rows, dev),
+    p = _PACK_LOGITS(_flat(history, "history", "int32", 0, dev), n_hist, _flat(hist_begin, "hist_begin", "int32", rows, dev),
                      _flat(hist_end, "hist_end", "int32", rows, dev), _flat(repetition, "repetition", "float32", rows, dev),
                      _flat(presence, "presence", "float32", rows, dev), _flat(frequency, "frequency", "float32", rows, dev),
-                     _flat(bias_ids, "bias_ids", "int32", None, dev), _flat(bias_values, "bias_values", "float32", n_bias, dev), n_bias,
-                     _flat(bias_begin, "bias_begin", "int32", rows, dev), _flat(bias_end, "bias_end", "int32", rows, dev), _ptr(mask),
-                     0 if mask is None else max(mask.stride()[0], mask.shape[1]), 0 if mask is None else mask.shape[0],
+                     _flat(bias_ids, "bias_ids", "int32", 0, dev), _flat(bias_values, "bias_values", "float32", n_bias, dev), n_bias,
+                     _flat(bias_begin, "bias_begin", "int32", rows, dev), _flat(bias_end, "bias_end", "int32", rows, dev), mp, ms, mn,
                      _flat(mask_row, "mask_row", "int32", rows, dev))
-    _ok(lib().mtb_logits_process(logits.data_ptr(), _CODES[_dtype(logits)], rows, vocab, st[0] if rows > 1 else max(st[0], vocab),
-                                 C.byref(p), _ptr(out), os_, _flat(choice, "choice", "int32", rows, dev), _stream(logits, stream)),
-        "logits_process")
+    rc = lib().mtb_logits_process(logits.data_ptr(), _CODES[name], rows, vocab, st[0] if rows > 1 else max(st[0], vocab), p, op, os_,
+                                  _flat(choice, "choice", "int32", rows, dev), _stream(dev, stream))
+    if rc != 0:
+        _ok(rc, "logits_process")
