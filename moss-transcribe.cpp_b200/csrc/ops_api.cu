@@ -261,6 +261,7 @@ int mtb_cache_evict(const mtb_paged_cache* cache, int keep, int sinks, int recen
         if (const int rc = view_of("cache_evict", cache, &a.c)) return rc;
         if (keep < 0 || sinks < 0 || recent < 0 || int64_t(sinks) + recent > keep)
             return fail(-2, w + ": sinks + recent must be in [0, keep]");
+        if (cache->n_pages > (1 << 25)) return fail(-2, w + ": n_pages must be at most 2^25 (rows of the pool are counted in int32)");
         if (cache->n_seq == 0) return 0;
         if (!cache->position || !cache->weight || !new_len || !workspace)
             return fail(-1, w + ": null pointer (the cache's position and weight are needed)");

@@ -182,7 +182,7 @@ cudaError_t rope_typed(const RopeArgs& a, cudaStream_t s) {
 // Two kernels.  The first, one cluster per (sequence, KV head): each slot's rank
 // as a 32-bit key (protected: all ones; else the weight's bits in ascending
 // order; NaN 0), the keep-th largest key by three passes of 11, 11 and 10 bits,
-// and lists of the gaps below `keep` and of the kept slots behind it.  Ties at
+// and lists of the gaps below `keep` and of the kept slots behind it, as rows of the pool.  Ties at
 // the threshold go to the lowest slots.  k_evict_rank_regs holds eight slots a
 // thread in registers, in as many CTAs as that takes (four SMs for a half-hour
 // recording); k_evict_rank, one CTA, takes longer lists and books that are not 16-byte
@@ -338,8 +338,9 @@ __global__ void __launch_bounds__(kRankThreads) k_evict_rank(EvictArgs a) {
     tie = tie0;
     for (int i = lo; i < hi; ++i) {
         const bool st = stays(i);
-        if (!st && i < a.keep) to[g++] = i;
-        if (st && i >= a.keep) from[f++] = i;
+        const int row = table[i / kPage] * kPage + i % kPage;
+        if (!st && i < a.keep) to[g++] = row;
+        if (st && i >= a.keep) from[f++] = row;
     }
     if (threadIdx.x == 0) *head = EvictHead{min(moves, same), a.keep};
 }
@@ -352,7 +353,8 @@ constexpr int kRankCopies = 4;  // of the histogram, by lane: neighbours' weight
 struct RankShared {
     int hist[kRankCopies][kRankBins];
     int warp[32];
-    int newest, bad, ties, gaps, come, pick, left;
+    int sums[kRankBins];
+    int newest, bad, ties, gaps, come, pick, left, count;
 };
 
 __global__ void __launch_bounds__(kRankThreads) k_evict_rank_regs(EvictArgs a, int width) {
@@ -374,11 +376,12 @@ __global__ void __launch_bounds__(kRankThreads) k_evict_rank_regs(EvictArgs a, i
     const int mine = min(max(n - i0, 0), kRankEach);
     int pos[kRankEach];
     unsigned key[kRankEach];
-    int newest = INT_MIN;
+    int newest = INT_MIN, row0 = 0;  // row0: the first slot's row of the pool
     if (threadIdx.x == 0) sh.bad = 0;
     __syncthreads();
     if (mine > 0) {
         const int page = page_of(c, seq, i0 / kPage);
+        row0 = page * kPage + i0 % kPage;
         if (page < 0) {
             sh.bad = 1;
         } else {
@@ -420,15 +423,23 @@ __global__ void __launch_bounds__(kRankThreads) k_evict_rank_regs(EvictArgs a, i
 #pragma unroll
         for (int e = 0; e < kRankEach; ++e)
             if (e < mine && (key[e] & known) == prefix) atomicAdd(&sh.hist[threadIdx.x % kRankCopies][(key[e] >> shift) & (bins - 1)], 1);
-        cluster.sync();
-        // Bins from the top: thread t has bins 2047 - 2t and 2046 - 2t, of all CTAs.
+        __syncthreads();
+        // Bins from the top: thread t has bins 2047 - 2t and 2046 - 2t; of its CTA, then of all.
         const int b1 = kRankBins - 1 - 2 * threadIdx.x;
         int c1 = 0, c0 = 0;
-        for (int r = 0; r < width; ++r) {
-            const RankShared* o = cluster.map_shared_rank(&sh, r);
 #pragma unroll
-            for (int k = 0; k < kRankCopies; ++k) {
-                const int2 x = *reinterpret_cast<const int2*>(&o->hist[k][b1 - 1]);
+        for (int k = 0; k < kRankCopies; ++k) {
+            const int2 x = *reinterpret_cast<const int2*>(&sh.hist[k][b1 - 1]);
+            c0 += x.x;
+            c1 += x.y;
+        }
+        if (width > 1) {
+            *reinterpret_cast<int2*>(&sh.sums[b1 - 1]) = make_int2(c0, c1);
+            cluster.sync();
+            c0 = c1 = 0;
+#pragma unroll 4
+            for (int r = 0; r < width; ++r) {
+                const int2 x = *reinterpret_cast<const int2*>(&cluster.map_shared_rank(&sh, r)->sums[b1 - 1]);
                 c0 += x.x;
                 c1 += x.y;
             }
@@ -438,19 +449,26 @@ __global__ void __launch_bounds__(kRankThreads) k_evict_rank_regs(EvictArgs a, i
         if (before < left && left <= before + c1) {
             sh.pick = b1;
             sh.left = left - before;
+            sh.count = c1;
         } else if (before + c1 < left && left <= before + c1 + c0) {
             sh.pick = b1 - 1;
             sh.left = left - before - c1;
+            sh.count = c0;
         }
-        cluster.sync();  // the histograms may be cleared, the pick be read
+        if (width > 1) cluster.sync();  // the sums may be written again, the pick be read
+        else __syncthreads();
         prefix |= (unsigned)sh.pick << shift;
         known |= (unsigned)(bins - 1) << shift;
         left = sh.left;
+        if (left == sh.count) break;  // all of the bin's keys stay: their other bits do not matter
     }
-    // Keys above prefix stay, and the first `left` of those equal to it.
+    // Keys above prefix stay, and the first `left` of those equal to it, as far as it is known.
     int ties = 0, total;
 #pragma unroll
-    for (int e = 0; e < kRankEach; ++e) ties += e < mine && key[e] == prefix;
+    for (int e = 0; e < kRankEach; ++e) {
+        key[e] &= known;
+        ties += e < mine && key[e] == prefix;
+    }
     int tie = block_scan(ties, sh.warp, &total);
     if (threadIdx.x == 0) sh.ties = total;
     cluster.sync();
@@ -484,8 +502,8 @@ __global__ void __launch_bounds__(kRankThreads) k_evict_rank_regs(EvictArgs a, i
 #pragma unroll
     for (int e = 0; e < kRankEach; ++e) {
         const bool st = (stays >> e) & 1;
-        if (e < mine && !st && i0 + e < a.keep) to[g++] = i0 + e;
-        if (st && i0 + e >= a.keep) from[f++] = i0 + e;
+        if (e < mine && !st && i0 + e < a.keep) to[g++] = row0 + e;
+        if (st && i0 + e >= a.keep) from[f++] = row0 + e;
     }
     if (part == 0 && threadIdx.x == 0) *head = EvictHead{moves, a.keep};
     cluster.sync();  // nobody leaves while its counts are read
@@ -507,27 +525,30 @@ __global__ void __launch_bounds__(kMoveThreads) k_evict_move(EvictArgs a, int li
         const EvictHead head = *reinterpret_cast<const EvictHead*>(ws);
         const int* to = reinterpret_cast<const int*>(ws + 256);
         const int* from = to + c.table_stride * (kPage / 2);
-        const int* table = c.table + (long long)seq * c.table_stride;
         if (blockIdx.x == 0 && threadIdx.x == 0 && h == 0) a.new_len[seq] = head.new_len;
-        for (int i0 = (blockIdx.x * (kMoveThreads / 32) + warp) * kMoveBatch; i0 < head.moves; i0 += gridDim.x * (kMoveThreads / 32) * kMoveBatch) {
-            // A lane a row: its places, its weight and position.
-            long long od = 0, of = 0;
+        const int step = gridDim.x * (kMoveThreads / 32) * kMoveBatch;
+        int i0 = (blockIdx.x * (kMoveThreads / 32) + warp) * kMoveBatch;
+        // A lane a row: its places, read one batch ahead.
+        int d = 0, f = 0;
+        if (lane < kMoveBatch && i0 + lane < head.moves) d = to[i0 + lane], f = from[i0 + lane];
+        for (; i0 < head.moves; i0 += step) {
             const int rows = min(kMoveBatch, head.moves - i0);
-            if (lane < rows) {
-                const int d = to[i0 + lane], f = from[i0 + lane];
-                const long long pd = table[d / kPage], pf = table[f / kPage];
-                const long long md = (pd * c.n_kv + h) * kPage + d % kPage, mf = (pf * c.n_kv + h) * kPage + f % kPage;
-                c.weight[md] = c.weight[mf];
-                c.position[md] = c.position[mf];
-                od = 2 * (pd * c.page_stride + h * c.head_stride + (long long)(d % kPage) * c.head_dim);
-                of = 2 * (pf * c.page_stride + h * c.head_stride + (long long)(f % kPage) * c.head_dim);
-            }
+            const long long od = 2 * ((long long)(d / kPage) * c.page_stride + h * c.head_stride + (long long)(d % kPage) * c.head_dim);
+            const long long of = 2 * ((long long)(f / kPage) * c.page_stride + h * c.head_stride + (long long)(f % kPage) * c.head_dim);
             uint4 x[kMoveBatch];
 #pragma unroll
             for (int r = 0; r < kMoveBatch; ++r) {
                 const long long o = __shfl_sync(0xffffffffu, of, r);
                 if (r < rows && lane < 2 * per_row) x[r] = *reinterpret_cast<const uint4*>(base + o + piece);
             }
+            if (lane < rows) {
+                const long long md = ((long long)(d / kPage) * c.n_kv + h) * kPage + d % kPage, mf = ((long long)(f / kPage) * c.n_kv + h) * kPage + f % kPage;
+                const float w = c.weight[mf];
+                const int p = c.position[mf];
+                c.weight[md] = w;
+                c.position[md] = p;
+            }
+            if (lane < kMoveBatch && i0 + step + lane < head.moves) d = to[i0 + step + lane], f = from[i0 + step + lane];
 #pragma unroll
             for (int r = 0; r < kMoveBatch; ++r) {
                 const long long o = __shfl_sync(0xffffffffu, od, r);

@@ -667,3 +667,28 @@ def test_a_bounded_cache_serves_a_run(dtype):
                     held = set(c["position"][page, h, place].tolist())
                     assert {0, 1, 2, 3} <= held and set(range(told[s] - 64, told[s])) <= held and len(held) == c["kv"][s]
     assert told[0] > budget and int(c["status"]) == 0
+
+
+def test_logits_longer_lists_than_16_bits():
+    """Histories and bias lists of more than 65535 entries: counts and the last entry are still exact."""
+    vocab, n = 40000, 70001
+    x = normal(2, vocab, seed=4)
+    g = torch.Generator().manual_seed(1)
+    hist = torch.randint(0, 30, (n,), generator=g).to(torch.int32)
+    hist[:1000] = torch.randint(0, vocab, (1000,), generator=g).to(torch.int32)
+    ids = torch.randint(0, vocab, (n,), generator=g).to(torch.int32)
+    val = torch.randn(n, generator=g)
+    lo, hi = torch.tensor([0, 69000], dtype=torch.int32, device=DEV), torch.tensor([n, n], dtype=torch.int32, device=DEV)
+    freq = torch.tensor([2.0 ** -10, 0.5], device=DEV)
+    out, choice = torch.empty_like(x), torch.empty(2, dtype=torch.int32, device=DEV)
+    capi.logits_process(x, out, choice, history=hist.to(DEV), hist_begin=lo, hist_end=hi, frequency=freq, bias_ids=ids.to(DEV),
+                        bias_values=val.to(DEV), bias_begin=lo, bias_end=hi)
+    for r in range(2):
+        a = int(lo[r])
+        count = torch.bincount(hist[a:].long(), minlength=vocab).to(DEV)
+        last = torch.full((vocab,), -1, dtype=torch.int64)
+        last.scatter_reduce_(0, ids[a:].long(), torch.arange(a, n), "amax")
+        bias = torch.where(last >= 0, val[last.clamp(min=0)], torch.zeros(())).to(DEV)
+        want = torch.where(count > 0, x[r] - freq[r] * count, x[r])  # f32 in the operator's order: equal to the bit
+        want = torch.where(last.to(DEV) >= 0, want + bias, want)
+        assert torch.equal(out[r], want) and int(choice[r]) == int(want.argmax())
