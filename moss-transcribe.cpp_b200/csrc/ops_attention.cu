@@ -19,7 +19,6 @@ using namespace ops;
 // Units that stand for a tile's own cost, and those of a CTA's interval at least.
 constexpr int kRowsExtra = 2, kRowsMinUnits = 16;    // of 64 slots
 constexpr int kTilesExtra = 1, kTilesMinUnits = 4;  // of 128 slots
-constexpr int kMaxSms = 160;      // CTAs whose parts fit the workspace
 
 
 __device__ __forceinline__ float max_nan(float a, float b) {

@@ -166,6 +166,7 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, ui
 // ---- the line of units ---------------------------------------------------------------------------------------------
 
 constexpr int kMaxCtas = 1024;  // counters that fit the workspace
+constexpr int kMaxSms = 160;    // CTAs whose parts fit it
 
 struct SeqWork {
     int len, tok0, n_new;
@@ -266,6 +267,7 @@ struct Line {
     int seq;        // sequence of unit lo
     long long off;  // of lo in that sequence's units
     long long per;  // that sequence's units under one KV head
+    SeqWork work;   // that sequence's
 };
 
 // As many CTAs as there are, but fewer where their intervals would be shorter
@@ -307,6 +309,7 @@ __device__ Line find_line_warp(const AttnArgs& a, const Geometry& ge, int min_un
     l.seq = max(0, __ffs(at) - 1);
     l.off = l.lo - __shfl_sync(0xffffffffu, x - v, l.seq);
     l.per = __shfl_sync(0xffffffffu, per, l.seq);
+    l.work = SeqWork{__shfl_sync(0xffffffffu, w.len, l.seq), __shfl_sync(0xffffffffu, w.tok0, l.seq), __shfl_sync(0xffffffffu, w.n_new, l.seq)};
     return l;
 }
 
@@ -366,6 +369,7 @@ __device__ __noinline__ Line find_line_cta(const AttnArgs& a, const Geometry ge,
     l.seq = (int)s_scan[kWarps];
     l.off = s_scan[kWarps + 1];
     l.per = s_scan[kWarps + 2];
+    if (l.lo < l.hi) l.work = seq_work(a, l.seq);
     return l;
 }
 
@@ -405,7 +409,7 @@ struct Walk {
 
     __device__ Walk(const AttnArgs& args, const Geometry& g, const Line& l) : a(args), ge(g), line(l), at(l.lo), seq(l.seq) {
         if (l.lo >= l.hi) return;
-        w = seq_work(a, seq);
+        w = l.work;
         tiles = Cut::tiles(w, ge);
         head = a.c.n_kv == 1 ? 0 : div_small(l.off, l.per);
         long long off = l.off - head * l.per;
@@ -551,64 +555,98 @@ __device__ __forceinline__ int parts_if_last(const AttnArgs& a, const Part& p) {
 
 // Joins a split tile's parts, by kWarps warps numbered from 0.  First each row's
 // factors, which take the maxima's place: few rows a warp each, a lane a part; many
-// rows a thread each.  Then the sums: four columns a thread, whose loads wait for nothing.
+// rows a thread each.  Then the sums: four columns a thread; the loads wait for
+// nothing, and go out for eight parts (few rows) or eight rows (many) at a time.
 template <class T, int kRows, int kD, int kWarps>
 __device__ __forceinline__ void join_parts(const AttnArgs& a, const Geometry& ge, const Part& p, int parts, SyncPoint& all) {
+    constexpr bool kFew = kRows <= 32;
+    constexpr int kThreads = kWarps * 32, kStep = 2 * kRows * (kD + 2);  // floats from a part to the next; the first is the one that begins the tile
+    constexpr int kEach = kFew ? (kMaxSms + 31) / 32 : 1;                 // parts of a lane
     const int rows = min(ge.rows, (p.n_new - p.tile * ge.per) * ge.G);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr size_t kStep = 2 * (size_t)kRows * (kD + 2);  // from a part to the next; the first is the one that begins the tile
-    float* first = part_at<kRows, kD>(a, p.first_cta(), true);
-    float* others = first - kStep / 2;  // part i > 0 at others + i kStep
-    const bool few = rows <= 32;
+    const int lane = threadIdx.x & 31;
+    float* others = part_at<kRows, kD>(a, p.first_cta(), false);  // part i > 0 at others + i kStep, part 0 half a step behind
+    auto at = [&](int c) { return others + (size_t)c * kStep + (c ? 0 : kStep / 2); };
 #pragma unroll 1
-    for (int r = few ? warp : threadIdx.x; r < rows; r += few ? kWarps : kWarps * 32) {
-        const int c0 = few ? lane : 0, step = few ? 32 : 1;
+    for (int r = kFew ? threadIdx.x >> 5 : threadIdx.x; r < rows; r += kFew ? kWarps : kThreads) {
         float m = -INFINITY, sum = 0.f;
-#pragma unroll 2
-        for (int c = c0; c < parts; c += step) m = fmaxf(m, ld_cg((c ? others + c * kStep : first) + r));
-        if (few)
+        if constexpr (kFew) {
+            float mi[kEach], li[kEach];
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                const int c = lane + 32 * k;
+                mi[k] = c < parts ? ld_cg(at(c) + r) : -INFINITY;
+                li[k] = c < parts ? ld_cg(at(c) + kRows + r) : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) m = fmaxf(m, mi[k]);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll 2
-        for (int c = c0; c < parts; c += step) {
-            const float* q = (c ? others + c * kStep : first) + r;
-            sum = __fmaf_rn(exp2_fast(ld_cg(q) - base), ld_cg(q + kRows), sum);
-        }
-        if (few)
+            const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                mi[k] = exp2_fast(mi[k] - base);
+                sum = __fmaf_rn(mi[k], li[k], sum);
+            }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll 2
-        for (int c = c0; c < parts; c += step) {
-            float* q = (c ? others + c * kStep : first) + r;
-            __stcg(q, exp2_fast(ld_cg(q) - base) * inv);
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+            for (int k = 0; k < kEach; ++k)
+                if (lane + 32 * k < parts) __stcg(at(lane + 32 * k) + r, mi[k] * inv);
+        } else {
+#pragma unroll 4
+            for (int c = 0; c < parts; ++c) m = fmaxf(m, ld_cg(at(c) + r));
+            const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+            for (int c = 0; c < parts; ++c) sum = __fmaf_rn(exp2_fast(ld_cg(at(c) + r) - base), ld_cg(at(c) + kRows + r), sum);
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll 4
+            for (int c = 0; c < parts; ++c) __stcg(at(c) + r, exp2_fast(ld_cg(at(c) + r) - base) * inv);
         }
         long long token;
         int head;
-        if (c0 == 0 && a.lse && row_place(ge, p, r, &token, &head))
+        if ((!kFew || lane == 0) && a.lse && row_place(ge, p, r, &token, &head))
             a.lse[token * a.n_heads + head] = sum == 0.f ? -INFINITY : (m + __log2f(sum)) * kLn2;
     }
     all.sync();
-    constexpr int kCols = kD / 4;
-#pragma unroll 2
-    for (int i = threadIdx.x; i < rows * kCols; i += kWarps * 32) {
-        const int r = i / kCols, col = i % kCols * 4;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int c = 0; c < parts; ++c) {
-            const float* q = c ? others + c * kStep : first;
-            const float f = ld_cg(q + r);
-            const float4 x = ld_cg4(q + 2 * kRows + r * kD + col);
-            o.x = __fmaf_rn(f, x.x, o.x);
-            o.y = __fmaf_rn(f, x.y, o.y);
-            o.z = __fmaf_rn(f, x.z, o.z);
-            o.w = __fmaf_rn(f, x.w, o.w);
+    constexpr int kCols = kD / 4, kItems = kFew ? 1 : 8, kParts = kFew ? 8 : 1;
+    const int items = rows * kCols;
+#pragma unroll 1
+    for (int i0 = threadIdx.x; i0 < items; i0 += kItems * kThreads) {
+        float4 o[kItems];
+#pragma unroll
+        for (int u = 0; u < kItems; ++u) o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int c0 = 0; c0 < parts; c0 += kParts) {
+            float f[kItems * kParts];
+            float4 x[kItems * kParts];
+#pragma unroll
+            for (int u = 0; u < kItems * kParts; ++u) {
+                const int i = i0 + (kFew ? 0 : u * kThreads), c = c0 + (kFew ? u : 0), r = i / kCols;
+                f[u] = 0.f;
+                x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < items && c < parts) {
+                    f[u] = ld_cg(at(c) + r);
+                    x[u] = ld_cg4(at(c) + 2 * kRows + r * kD + i % kCols * 4);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kItems * kParts; ++u) {
+                float4& y = o[kFew ? 0 : u];
+                y.x = __fmaf_rn(f[u], x[u].x, y.x);
+                y.y = __fmaf_rn(f[u], x[u].y, y.y);
+                y.z = __fmaf_rn(f[u], x[u].z, y.z);
+                y.w = __fmaf_rn(f[u], x[u].w, y.w);
+            }
         }
-        long long token;
-        int head;
-        if (row_place(ge, p, r, &token, &head))
-            store4<T>(reinterpret_cast<T*>(a.out) + token * a.out_stride + (long long)head * kD + col, o);
+#pragma unroll
+        for (int u = 0; u < kItems; ++u) {
+            const int i = i0 + u * kThreads;
+            long long token;
+            int head;
+            if (i < items && row_place(ge, p, i / kCols, &token, &head))
+                store4<T>(reinterpret_cast<T*>(a.out) + token * a.out_stride + (long long)head * kD + i % kCols * 4, o[u]);
+        }
     }
 }
 
