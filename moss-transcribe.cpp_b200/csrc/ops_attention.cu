@@ -29,8 +29,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // 2^x on the FMA units, for x in [-125, 127]: x = n + r, r in [-1/2, 1/2], a
 // degree-5 polynomial for 2^r (least relative error, 2.1e-7 as evaluated), n added
-// to the exponent.  Below -125: 2^-125, or 0.
-template <bool kZero>
+// to the exponent.  Below -125: 0.
 __device__ __forceinline__ float2 exp2_poly(float2 x0) {
     float2 x = x0;
     const float2 shift = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
@@ -46,10 +45,8 @@ __device__ __forceinline__ float2 exp2_poly(float2 x0) {
     p = __ffma2_rn(p, r, make_float2(1.0000001f, 1.0000001f));
     p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23));
     p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23));
-    if (kZero) {
-        p.x = x0.x >= -125.f ? p.x : max_nan(x0.x, 0.f);  // a NaN stays one
-        p.y = x0.y >= -125.f ? p.y : max_nan(x0.y, 0.f);
-    }
+    p.x = x0.x >= -125.f ? p.x : max_nan(x0.x, 0.f);  // a NaN stays one
+    p.y = x0.y >= -125.f ? p.y : max_nan(x0.y, 0.f);
     return p;
 }
 template <class T>
@@ -522,9 +519,6 @@ constexpr int kTileThreads = 384;  // warps 0-3 and 4-7: the halves; 8: products
 constexpr int kHalfRegs = 224, kOtherRegs = 56;
 constexpr int kTileEntries = 4;    // ring of K and V blocks, in turn
 constexpr int kBadRing = 16;       // blocks whose bad-page bits are kept
-// Of eight pairs of exponentials, those that go to the FMA units (the polynomial
-// above) and not to the special function units, which would bound the kernel alone.
-constexpr int kPolyOf8 = 3;
 
 template <int kD>
 struct TileShape {
@@ -798,16 +792,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                 if (!((on >> i) & 1)) s[c * 32 + i] = -INFINITY;
                         }
                     }
-                    // A NaN among the scores makes the maximum NaN, and with it the row.
+                    // A NaN is no maximum, but its exponential makes the row's sum NaN.
                     float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int i = 4; i < 128; ++i) top[i & 3] = max_nan(top[i & 3], s[i]);
-                    top[0] = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
+                    for (int i = 4; i < 124; i += 8)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) top[j] = fmaxf(fmaxf(top[j], s[i + j]), s[i + 4 + j]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], s[124 + j]);
+                    top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                     const float reach = top[0] * to_log2;
-                    const bool grown = !(reach <= m + 8.f);
+                    const bool grown = reach > m + 8.f;
                     if (__any_sync(0xffffffffu, grown)) {
-                        float to = grown ? max_nan(m, reach) : m;  // a row goes by its own scores alone
-                        if (to == INFINITY) to = NAN;
+                        const float to = grown ? reach : m;  // a row goes by its own scores alone
                         const float f = to == -INFINITY ? 1.f : exp2_fast(m - to);
                         m = to;
                         l *= f;
@@ -833,12 +830,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             float2 x = __ffma2_rn(make_float2(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), by, from);
-                            if (i % 8 < kPolyOf8) {
-                                x = exp2_poly<false>(x);
-                            } else {
-                                x.x = exp2_fast(x.x);
-                                x.y = exp2_fast(x.y);
-                            }
+                            x.x = exp2_fast(x.x);
+                            x.y = exp2_fast(x.y);
                             sum[i & 1] = __fadd2_rn(sum[i & 1], x);
                             pk[i] = pack2<T>(x.x, x.y);
                         }
@@ -852,7 +845,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                     l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 }
-                if (m == -INFINITY && l == l) l = 0.f;  // nothing seen: the polynomial leaves 2^-125 for 2^-inf
                 long long token = 0;
                 int head = 0;
                 const bool row = row_place(ge, p, r, &token, &head);
@@ -1152,6 +1144,10 @@ __global__ void __launch_bounds__(kWThreads, 1)
 // ahead.  The exponentials bound it: one for each product of 128 dims.
 constexpr int kWTileSlots = 256, kWTileRows = 128;
 constexpr int kWEntries = 2;  // ring of row tiles
+// Of eight pairs of exponentials, those that go to the FMA units (the polynomial
+// above) and not to the special function units: the long chunk takes 274 us with none,
+// 256 with 1, 255 with 2, 269 with 3, 322 with 4.  (The attention is fastest with none, 340 us; 344, 356, 366, 376.)
+constexpr int kPolyOf8 = 2;
 constexpr int kWLse = 4;      // ring of their log-sums
 
 template <int kD>
@@ -1391,9 +1387,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     const float4 less = *reinterpret_cast<const float4*>(&s_less[e][i * 4]);
                     float2 x = __ffma2_rn(make_float2(s[4 * i], s[4 * i + 1]), by, make_float2(less.x, less.y));
                     float2 y = __ffma2_rn(make_float2(s[4 * i + 2], s[4 * i + 3]), by, make_float2(less.z, less.w));
-                    if (2 * i % 8 < kPolyOf8) x = exp2_poly<true>(x);
+                    if (2 * i % 8 < kPolyOf8) x = exp2_poly(x);
                     else x.x = exp2_fast(x.x), x.y = exp2_fast(x.y);
-                    if ((2 * i + 1) % 8 < kPolyOf8) y = exp2_poly<true>(y);
+                    if ((2 * i + 1) % 8 < kPolyOf8) y = exp2_poly(y);
                     else y.x = exp2_fast(y.x), y.y = exp2_fast(y.y);
                     sum[0] = __fadd2_rn(sum[0], x);
                     sum[1] = __fadd2_rn(sum[1], y);
