@@ -692,3 +692,95 @@ def test_logits_longer_lists_than_16_bits():
         want = torch.where(count > 0, x[r] - freq[r] * count, x[r])  # f32 in the operator's order: equal to the bit
         want = torch.where(last.to(DEV) >= 0, want + bias, want)
         assert torch.equal(out[r], want) and int(choice[r]) == int(want.argmax())
+
+
+# ---- captured together, and over the whole range --------------------------------------------------------------------
+
+
+def test_a_captured_step_replays_on_what_the_host_changes():
+    """Append, attention, weights, eviction and choice in one graph: replays follow lengths, pages, tokens and books."""
+    Hk, G, D, V, dtype = 2, 2, 128, 3000, torch.bfloat16
+    c = ref.make_cache([640, 640], Hk, D, dtype, DEV)
+    c["kv"] = [500, 301]
+    c["kv_len"].copy_(torch.tensor(c["kv"], dtype=torch.int32))
+    fill_books(c)
+    new, n = [2, 1], 3
+    cu = ref.cu_of(new, DEV)
+    rows, pos = normal(n, Hk * G + 2 * Hk, D, dtype=dtype), torch.tensor([1200, 1201, 900], dtype=torch.int32, device=DEV)
+    inv = torch.from_numpy(capi.rope_frequencies(D, 1e6)[0]).to(DEV)
+    q, lse, ws = torch.zeros(n, Hk * G, D, dtype=dtype, device=DEV), torch.zeros(n, Hk * G, device=DEV), space()
+    out, x = torch.zeros_like(q), normal(2, V)
+    ews = torch.zeros(capi.cache_evict_workspace(2, Hk, c["table"].shape[1]), dtype=torch.uint8, device=DEV)
+    y, choice, new_len = torch.zeros_like(x), torch.zeros(2, dtype=torch.int32, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV)
+    hist, lo, hi = torch.tensor([5, 6, 7], dtype=torch.int32, device=DEV), torch.tensor([0, 1], dtype=torch.int32, device=DEV), torch.tensor([3, 3], dtype=torch.int32, device=DEV)
+    rep = torch.tensor([1.5, 1.2], device=DEV)
+    cache = view(c, position=c["position"], weight=c["weight"])
+
+    def step():
+        capi.rope_append(cache, cu, pos, rows[:, :Hk * G], rows[:, Hk * G:Hk * G + Hk], rows[:, Hk * G + Hk:], inv, q)
+        capi.paged_attention(cache, cu, q, out, ws, lse=lse, max_tokens=2)
+        capi.attention_weights(cache, cu, q, lse, decay=0.5, max_tokens=2)
+        capi.cache_evict(cache, 300, new_len, ews, sinks=4, recent=50)
+        capi.logits_process(x, y, choice, history=hist, hist_begin=lo, hist_end=hi, repetition=rep)
+
+    state = [c[k].clone() for k in ("pool", "position", "weight")]
+
+    def reset():
+        for k, v in zip(("pool", "position", "weight"), state):
+            c[k].copy_(v)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for lengths in ([500, 301], [640, 299]):
+        c["kv_len"].copy_(torch.tensor(lengths, dtype=torch.int32))
+        x.copy_(normal(2, V, seed=lengths[0]))
+        reset()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (c["pool"], c["position"], c["weight"], out, lse, new_len, y, choice)]
+        reset()
+        step()
+        torch.cuda.synchronize()
+        for a, b in zip(got, (c["pool"], c["position"], c["weight"], out, lse, new_len, y, choice)):
+            assert torch.equal(a, b)
+        assert new_len.tolist() == [min(t, 300) for t in lengths]
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_attention_over_the_range(seed):
+    import random
+    r = random.Random(seed)
+    Hk, D, G = r.choice([1, 2, 3, 5, 8]), r.choice([64, 128]), r.choice([1, 2, 3, 4, 5, 6, 8, 12])
+    n_seq = r.choice([1, 2, 3, 7, 40])
+    new = [r.choice([0, 1, 1, 2, r.randrange(1, 40), r.randrange(1, 600 // (1 + n_seq // 8))]) for _ in range(n_seq)]
+    if not sum(new):
+        new[0] = 1
+    kv = [max(0, n + r.choice([0, 0, r.randrange(0, 300), r.randrange(0, 5000)])) for n in new]
+    c = ref.make_cache(kv, Hk, D, r.choice([torch.float16, torch.bfloat16]), DEV, seed=seed, apart=r.random() < 0.3)
+    run_attention(c, new, Hk * G, seed=seed, decay=r.choice([0.0, 0.7, 1.0]), pad=r.choice([0, 3]), strided=r.random() < 0.3,
+                  max_tokens=r.choice([0, max(new), 1]))
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_evict_over_the_range(seed):
+    import random
+    r = random.Random(100 + seed)
+    kv = [r.randrange(0, r.choice([70, 700, 9000])) for _ in range(r.choice([1, 3, 6]))]
+    keep = r.randrange(0, max(kv) + 2)
+    sinks = r.randrange(0, min(8, keep) + 1)
+    c = fill_books(ref.make_cache(kv, r.choice([1, 2, 5]), r.choice([64, 128]), r.choice([torch.float16, torch.bfloat16]), DEV, seed=seed), seed, r.random() < 0.4)
+    run_evict(c, keep, sinks, r.randrange(0, keep - sinks + 1), alias=r.random() < 0.5)
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_logits_over_the_range(seed):
+    import random
+    r = random.Random(200 + seed)
+    vocab = r.choice([r.randrange(1, 100), r.randrange(100, 5000), r.randrange(5000, 200000)])
+    rows = max(1, min(300, 400000 // vocab))
+    run_logits(r.randrange(1, rows + 1), vocab, r.choice([torch.float32, torch.float16, torch.bfloat16]), hist=r.choice([0, 30, 7000]),
+               biases=r.choice([0, 1, 400]), masked=r.choice([None, 0.5, 1.0]), seed=seed, lead=r.choice([0, 0, 1]), gap=r.choice([0, 3]),
+               in_place=r.random() < 0.3)
