@@ -316,9 +316,12 @@ int mtb_audio_debug_chunk(mtb_audio* a, const float* samples, int n_samples, flo
  * the device.  `stream` is a cudaStream_t (NULL: the default stream); a call
  * is asynchronous on it, may be captured into a graph, runs on the device that
  * owns the memory and leaves the caller's current device as it found it.
- * 0 on success; -1 for a CUDA error or a null or non-device pointer, -2 for
- * an argument outside its limits, with mtb_global_error() set and nothing
- * launched.  Sizes that live on the device (lengths, page-table entries) are
+ * 0 on success; -1 for a CUDA error, a null pointer, or the cache's k (or the
+ * logits) not in device memory, -2 for an argument outside its limits, with
+ * mtb_global_error() set and nothing launched.  Pointers are aligned to their
+ * elements, and further where it says so; the others are taken as memory of the
+ * same device.  Calls may run at once on any streams as long as no memory that
+ * one writes is used by another.  Sizes that live on the device (lengths, page-table entries) are
  * checked by the kernels: a violated check sets its bit in *status (never
  * cleared by the library) and the access is skipped, never made. */
 enum { MTB_T_F32 = 0, MTB_T_F16 = 1, MTB_T_BF16 = 2 };
@@ -407,13 +410,16 @@ int mtb_paged_attention(const mtb_paged_cache* cache, const int32_t* cu_tokens, 
 /* The softmax weight each cached position received in that attention:
  * cache->weight[slot] = decay * cache->weight[slot] + sum of exp(score - lse) over the
  * new tokens that see the slot and the query heads of its KV head (decay 0
- * ignores the old value).  Slots at or behind kv_len are left as they are;
+ * ignores the old value).  A page whose weights are written belongs to one
+ * sequence.  Slots at or behind kv_len are left as they are;
  * sequences without new tokens too.  Arguments as above. */
 int mtb_attention_weights(const mtb_paged_cache* cache, const int32_t* cu_tokens, int n_tokens, int max_tokens,
                           const void* q, int64_t q_stride, int n_heads, float scale, const float* lse, float decay,
                           void* stream);
 
-/* Device bytes of mtb_cache_evict's workspace (needs no GPU). */
+/* Device bytes of mtb_cache_evict's workspace (needs no GPU); -2 for sizes that
+ * a cache cannot have (n_seq and n_kv_heads at most 65535, their product and table_stride
+ * at most 2^24).  Needs no zeroing; calls that share one must not overlap. */
 int64_t mtb_cache_evict_workspace(int n_seq, int n_kv_heads, int table_stride);
 /* Eviction by accumulated weight, in place, each KV head on its own: of a
  * sequence with kv_len > keep the `keep` slots stay that rank highest, others go.
@@ -424,7 +430,7 @@ int64_t mtb_cache_evict_workspace(int n_seq, int n_kv_heads, int table_stride);
  * is then slots [0, keep) in no particular order of positions: attention of later
  * tokens does not depend on it, since rotary positions are in K.
  * new_len[s] = min(kv_len, keep); it may be kv_len itself.  Needs position
- * and weight, sinks + recent <= keep, pages that no other sequence shares. */
+ * and weight, sinks + recent <= keep, n_pages <= 2^25, and each page in the table once. */
 int mtb_cache_evict(const mtb_paged_cache* cache, int keep, int sinks, int recent, int32_t* new_len, void* workspace,
                     size_t workspace_bytes, void* stream);
 
@@ -451,7 +457,8 @@ typedef struct mtb_logits_params {
  * then + the bias of the id's last entry; then -inf where the mask forbids it.
  * Evaluated in f32 in this order, each step rounded; out is rounded once more.
  * choice: the lowest id of the largest f32 value; NaN never wins; -1 when no
- * value is above -inf.  Ids outside [0, vocab) in history or biases are skipped. */
+ * value is above -inf.  Ids outside [0, vocab) in history or biases are skipped.
+ * vocab, history_len and bias_len are at most 2^30, rows at most 2^26. */
 int mtb_logits_process(const void* logits, int type, int rows, int vocab, int64_t stride,
                        const mtb_logits_params* params, void* out, int64_t out_stride, int32_t* choice, void* stream);
 

@@ -36,6 +36,8 @@ int guarded(F&& f) {
 }
 
 bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+template <class... P>
+bool words(const P*... p) { return (aligned(p, 4) && ...); }
 
 // Makes the device that owns `p` current; the caller's comes back at the end.
 struct OnDevice {
@@ -78,6 +80,7 @@ int view_of(const char* what, const mtb_paged_cache* c, PagedView* out) {
     if (c->n_seq > 65535) return fail(-2, w + ": n_seq must be at most 65535");
     if (int64_t(c->n_seq) * c->n_kv_heads > (1 << 24)) return fail(-2, w + ": n_seq * n_kv_heads must be at most 2^24");
     if (!aligned(c->k, 16) || !aligned(c->v, 16)) return fail(-2, w + ": k and v must be 16-byte aligned");
+    if (!words(c->page_table, c->kv_len, c->position, c->weight, c->status)) return fail(-2, w + ": a pointer is not aligned to its elements");
     const int64_t block = int64_t(kPage) * c->head_dim;
     if (c->head_stride % 8 || c->page_stride % 8 || c->head_stride < block || c->page_stride < block)
         return fail(-2, w + ": the cache's strides must be multiples of 8 elements that hold a page's rows");
@@ -107,6 +110,7 @@ int attention_args(const char* what, const mtb_paged_cache* cache, const int32_t
     if (!cu || !q) return fail(-1, w + ": null pointer");
     if (!aligned(q, 16) || q_stride % 8 || q_stride < int64_t(n_heads) * cache->head_dim || q_stride >= (1ll << 38))
         return fail(-2, w + ": q must be 16-byte aligned, its stride a multiple of 8 elements that holds a token's rows");
+    if (!words(cu)) return fail(-2, w + ": a pointer is not aligned to its elements");
     if (!std::isfinite(scale)) return fail(-2, w + ": scale must be finite");
     a->cu = cu;
     a->n_tokens = n_tokens;
@@ -180,7 +184,8 @@ int mtb_rope_append(const mtb_paged_cache* cache, const int32_t* cu_tokens, int 
         if (n_tokens == 0 || cache->n_seq == 0) return 0;
         if (!cu_tokens || !positions || !q || !k || !v || !q_out || (rotary_dim && !inv_freq)) return fail(-1, w + ": null pointer");
         const size_t in_size = in_type == MTB_T_F32 ? 4 : 2;
-        if (!aligned(q, in_size) || !aligned(k, in_size) || !aligned(v, in_size) || !aligned(q_out, 2) || !aligned(inv_freq, 8))
+        if (!aligned(q, in_size) || !aligned(k, in_size) || !aligned(v, in_size) || !aligned(q_out, 2) || !aligned(inv_freq, 8) ||
+            !words(cu_tokens, positions))
             return fail(-2, w + ": a pointer is not aligned to its elements");
         if (q == q_out && (in_type != cache->type || q_stride != q_out_stride))
             return fail(-2, w + ": q_out may be q only in the same type, with the same stride");
@@ -218,6 +223,7 @@ int mtb_paged_attention(const mtb_paged_cache* cache, const int32_t* cu_tokens, 
         if (!out || !workspace) return fail(-1, w + ": null pointer");
         if (!aligned(out, 16) || out_stride % 8 || out_stride < int64_t(n_heads) * cache->head_dim)
             return fail(-2, w + ": out must be 16-byte aligned, its stride a multiple of 8 elements that holds a token's rows");
+        if (!words(lse)) return fail(-2, w + ": a pointer is not aligned to its elements");
         if (workspace_bytes < size_t(kAttnWorkspace) || !aligned(workspace, 256))
             return fail(-2, w + ": the workspace must have MTB_ATTENTION_WORKSPACE bytes, 256-byte aligned");
         a.out = static_cast<char*>(out);
@@ -239,6 +245,7 @@ int mtb_attention_weights(const mtb_paged_cache* cache, const int32_t* cu_tokens
         if (const int rc = attention_args("attention_weights", cache, cu_tokens, n_tokens, max_tokens, q, q_stride, n_heads, scale, &a)) return rc;
         if (n_tokens == 0 || cache->n_seq == 0) return 0;
         if (!lse || !cache->weight) return fail(-1, w + ": null pointer (lse and the cache's weight are needed)");
+        if (!words(lse)) return fail(-2, w + ": a pointer is not aligned to its elements");
         if (!std::isfinite(decay)) return fail(-2, w + ": decay must be finite");
         a.lse = const_cast<float*>(lse);
         a.decay = decay;
@@ -249,7 +256,9 @@ int mtb_attention_weights(const mtb_paged_cache* cache, const int32_t* cu_tokens
 }
 
 int64_t mtb_cache_evict_workspace(int n_seq, int n_kv_heads, int table_stride) {
-    if (n_seq < 0 || n_kv_heads < 1 || table_stride < 1) return -2;
+    if (n_seq < 0 || n_seq > 65535 || n_kv_heads < 1 || n_kv_heads > 65535 || int64_t(n_seq) * n_kv_heads > (1 << 24) || table_stride < 1 ||
+        table_stride > (1 << 24))
+        return -2;
     return evict_workspace(n_seq, n_kv_heads, table_stride);
 }
 
@@ -265,6 +274,7 @@ int mtb_cache_evict(const mtb_paged_cache* cache, int keep, int sinks, int recen
         if (cache->n_seq == 0) return 0;
         if (!cache->position || !cache->weight || !new_len || !workspace)
             return fail(-1, w + ": null pointer (the cache's position and weight are needed)");
+        if (!words(new_len)) return fail(-2, w + ": a pointer is not aligned to its elements");
         if (int64_t(workspace_bytes) < evict_workspace(cache->n_seq, cache->n_kv_heads, cache->table_stride) || !aligned(workspace, 16))
             return fail(-2, w + ": the workspace must have mtb_cache_evict_workspace bytes, 16-byte aligned");
         a.keep = keep;
@@ -283,7 +293,8 @@ int mtb_logits_process(const void* logits, int type, int rows, int vocab, int64_
     return guarded([&]() -> int {
         const std::string w("logits_process");
         if (type != MTB_T_F32 && type != MTB_T_F16 && type != MTB_T_BF16) return fail(-2, w + ": unknown type");
-        if (rows < 0 || vocab < 1) return fail(-2, w + ": rows must not be negative, vocab must be positive");
+        // Ids and places in the lists are counted in int32, with steps beyond the end.
+        if (rows < 0 || vocab < 1 || vocab > (1 << 30)) return fail(-2, w + ": rows must not be negative, vocab in [1, 2^30]");
         if (stride < vocab || (out && out_stride < vocab)) return fail(-2, w + ": a stride is shorter than a row");
         if (!out && !choice) return fail(-1, w + ": out and choice are both null");
         const mtb_logits_params none{};
@@ -294,11 +305,15 @@ int mtb_logits_process(const void* logits, int type, int rows, int vocab, int64_
             return fail(-1, w + ": biases need ids, values and bounds");
         if (p.mask && p.mask_stride < (vocab + 31) / 32) return fail(-2, w + ": mask_stride is shorter than a mask row");
         if (p.history_len < 0 || p.bias_len < 0 || p.mask_rows < 0) return fail(-2, w + ": a length must not be negative");
+        if (p.history_len > (1 << 30) || p.bias_len > (1 << 30)) return fail(-2, w + ": a list has at most 2^30 entries");
         if (rows > (1 << 26)) return fail(-2, w + ": rows must be at most 2^26");
         if (rows == 0) return 0;
         if (!logits) return fail(-1, w + ": null pointer");
         const size_t size = type == MTB_T_F32 ? 4 : 2;
-        if (!aligned(logits, size) || (out && !aligned(out, size))) return fail(-2, w + ": a pointer is not aligned to its elements");
+        if (!aligned(logits, size) || (out && !aligned(out, size)) ||
+            !words(choice, p.history, p.history_begin, p.history_end, p.repetition, p.presence, p.frequency, p.bias_ids, p.bias_values, p.bias_begin,
+                   p.bias_end, p.mask, p.mask_row))
+            return fail(-2, w + ": a pointer is not aligned to its elements");
         if (out == logits && stride != out_stride) return fail(-2, w + ": in place, both strides are the same");
         LogitsArgs a{};
         a.x = static_cast<const char*>(logits);
@@ -316,8 +331,8 @@ int mtb_logits_process(const void* logits, int type, int rows, int vocab, int64_
             a.pres = p.presence;
             a.freq = p.frequency;
         }
-        a.hist_len = int(std::min<int64_t>(p.history_len, INT32_MAX));
-        a.bias_len = int(std::min<int64_t>(p.bias_len, INT32_MAX));
+        a.hist_len = int(p.history_len);
+        a.bias_len = int(p.bias_len);
         a.mask_rows = p.mask_rows;
         a.bias_ids = p.bias_ids;
         a.bias_val = p.bias_values;

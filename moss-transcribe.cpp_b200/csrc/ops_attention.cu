@@ -480,6 +480,7 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WP>::kThreads, 1)
             if (s_last) join_parts<T, S::kRows, kD, S::kWarps>(a, ge, p, s_last, all);
         }
     }
+    if (lane == 0 && *(volatile int*)&s_gave_up) flag(a.c, BAD_WAIT);  // the producer may have left before
 }
 
 // The arguments with a tile of `rows` rows at most.
@@ -1136,6 +1137,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
             if (lane == 0) bar_arrive(&q_empty[qb]);
         }
     }
+    if (lane == 0 && *(volatile int*)&s_gave_up) flag(a.c, BAD_WAIT);
 }
 
 // ---- weights, many rows --------------------------------------------------------------------------------------------

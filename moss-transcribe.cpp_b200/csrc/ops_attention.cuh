@@ -300,7 +300,7 @@ __device__ Line find_line_warp(const AttnArgs& a, const Geometry& ge, int min_un
     }
     Line l{};
     l.total = __shfl_sync(0xffffffffu, x, 31);
-    int tiles = min(Cut::tiles(w, ge) * a.c.n_kv, kMaxCtas);
+    int tiles = (int)min((long long)Cut::tiles(w, ge) * a.c.n_kv, (long long)kMaxCtas);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
     l.tiles = tiles;

@@ -316,8 +316,9 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(const __grid_const
     Share sh{row, part, log_width, (runs - part + width - 1) / width * kLogitsRun, 0, 0, 0, 0, nullptr};
     Batch<T, kVec> got;
     got.fetch(reinterpret_cast<const T*>(a.x) + row * a.x_stride, sh, a.vocab, threadIdx.x * Batch<T, kVec>::per);
-    if (a.hist) sh.h0 = max(a.hist_begin[row], 0), sh.h1 = max(sh.h0, min(a.hist_end[row], a.hist_len));
-    if (a.bias_ids) sh.b0 = max(a.bias_begin[row], 0), sh.b1 = max(sh.b0, min(a.bias_end[row], a.bias_len));
+    // Both bounds inside the list: what is added to them below stays below 2^31.
+    if (a.hist) sh.h0 = min(max(a.hist_begin[row], 0), a.hist_len), sh.h1 = max(sh.h0, min(a.hist_end[row], a.hist_len));
+    if (a.bias_ids) sh.b0 = min(max(a.bias_begin[row], 0), a.bias_len), sh.b1 = max(sh.b0, min(a.bias_end[row], a.bias_len));
     if (a.mask) {
         const int m = a.mask_row ? a.mask_row[row] : row;
         if (m >= 0 && m < a.mask_rows) sh.mask = a.mask + m * a.mask_stride;

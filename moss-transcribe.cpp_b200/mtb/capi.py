@@ -757,7 +757,7 @@ def logits_process(logits, out=None, choice=None, history=None, hist_begin=None,
         _need(_NAME[mask.dtype] in ("int32", "uint32") and s1 == 1 and mask.get_device() == dev and words * 32 >= vocab
               and (mask_row is not None or mn >= rows),
               "mask must be int32 [mask rows][vocab / 32 words], with a row for each logits row or mask_row given")
-        mp, ms = mask.data_ptr(), max(ms, words)
+        mp, ms = mask.data_ptr(), (ms if mn > 1 else max(ms, words))
     n_hist = 0 if history is None else history.numel()
     n_bias = 0 if bias_ids is None else bias_ids.numel()
     p = _PACK_LOGITS(_flat(history, "history", "int32", 0, dev), n_hist, _flat(hist_begin, "hist_begin", "int32", rows, dev),

@@ -599,6 +599,24 @@ def test_logits_ranges_are_cut_to_their_buffers():
     assert torch.equal(out, want)
 
 
+def test_logits_bounds_near_the_end_of_int32():
+    """A range that begins behind its list is empty, whatever lies between its begin and 2^31, beside a list that has entries."""
+    x = normal(2, 300)
+    ids = torch.tensor([5, 6, 7], dtype=torch.int32, device=DEV)
+    far = torch.full((2,), 2**31 - 1, dtype=torch.int32, device=DEV)
+    lo, hi = torch.zeros(2, dtype=torch.int32, device=DEV), torch.full((2,), 3, dtype=torch.int32, device=DEV)
+    ones, p = torch.ones(3, device=DEV), torch.ones(2, device=DEV)
+    out = torch.empty_like(x)
+    capi.logits_process(x, out, history=ids, hist_begin=far, hist_end=far, presence=p, bias_ids=ids, bias_values=ones, bias_begin=lo, bias_end=hi)
+    want = x.clone()
+    want[:, 5:8] += 1
+    assert torch.equal(out, want)
+    capi.logits_process(x, out, history=ids, hist_begin=lo, hist_end=hi, presence=p, bias_ids=ids, bias_values=ones, bias_begin=far, bias_end=far)
+    want = x.clone()
+    want[:, 5:8] -= 1
+    assert torch.equal(out, want)
+
+
 def test_logits_repetition_is_greedy_choice_of_the_decoder(tiny_gguf):
     """With the repetition penalty alone, on the last 100 ids, the choice is mtb_greedy_choice's."""
     model = capi.Model(tiny_gguf, 0)

@@ -108,6 +108,34 @@ def test_bad_logits_arguments_are_refused(params, bad):
     assert logits(params, **bad) in (-1, -2) and error()
 
 
+@pytest.mark.parametrize("params,bad", [
+    (None, dict(vocab=(1 << 30) + 1, xs=1 << 31, ys=1 << 31)), (None, dict(vocab=(1 << 31) - 1, xs=1 << 31, ys=1 << 31)),
+    (dict(history_len=(1 << 30) + 1), {}), (dict(bias_len=1 << 40), {}), (None, dict(choice=P + 2)),
+    (dict(history=P + 1, history_begin=P, history_end=P, history_len=4, repetition=P), {}), (dict(mask=P + 2, mask_stride=32, mask_rows=2), {}),
+])
+def test_logits_sizes_and_alignments_are_refused(params, bad):
+    assert logits(params, **bad) == -2 and error()
+
+
+@pytest.mark.parametrize("name", ["page_table", "kv_len", "position", "weight", "status"])
+def test_misaligned_words_of_a_cache_are_refused(name):
+    c = cache(**{name: P + 2})
+    assert rope(c) == -2 and attend(c) == -2 and weights(c) == -2 and evict(c) == -2
+
+
+def test_misaligned_words_are_refused():
+    assert rope(cache(), cu=P + 2) == -2 and rope(cache(), pos=P + 1) == -2
+    assert attend(cache(), cu=P + 2) == -2 and attend(cache(), lse=P + 2) == -2
+    assert weights(cache(), lse=P + 2) == -2 and evict(cache(), new=P + 2) == -2
+
+
+def test_workspace_size_of_impossible_caches():
+    """Sizes beyond a cache's limits have no workspace (their product would not fit 64 bits)."""
+    assert capi.cache_evict_workspace(65535, 256, 1 << 24) == 65535 * 256 * (256 + (1 << 24) * 256)
+    for bad in ((1 << 31) - 1, 8, 10), (8, (1 << 31) - 1, 10), (65535, 257, 10), (1, 8, (1 << 24) + 1):
+        assert capi.cache_evict_workspace(*bad) < 0
+
+
 def test_calls_with_nothing_to_do_succeed_without_a_device():
     assert rope(cache(), n=0) == 0 and attend(cache(), n=0) == 0 and weights(cache(), n=0) == 0
     none = cache(n_seq=0, k=None, v=None, page_table=None, kv_len=None)
@@ -228,3 +256,13 @@ def test_python_shapes_types_and_devices_are_checked():
                 dict(choice=one, bias_ids=one, bias_values=torch.ones(1), bias_begin=one, bias_end=one)):
         with pytest.raises(capi.MtbError):
             capi.logits_process(x, stream=0, **bad)
+
+
+def test_a_mask_row_spread_over_all_rows_is_refused():
+    """A mask of stride 0 (one row for all) is no [mask rows][words] array: mask_row says which row each has."""
+    import torch
+    x, one = torch.zeros(2, 100), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(capi.MtbError, match="mask_stride"):
+        capi.logits_process(x, choice=one, mask=torch.zeros(1, 4, dtype=torch.int32).expand(2, 4), stream=0)
+    with pytest.raises(capi.MtbError, match="stride is shorter"):
+        capi.logits_process(x[:1].expand(2, 100), choice=one, stream=0)
