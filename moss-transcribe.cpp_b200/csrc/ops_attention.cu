@@ -517,7 +517,7 @@ cudaError_t launch_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensor
 // free to be rescaled.
 constexpr int kTileRows2 = 256;
 constexpr int kTileBlock = 128;
-constexpr int kTileThreads = 384;  // warps 0-3 and 4-7: the halves; 8: products; 9, 10: copies; 11: none
+constexpr int kTileThreads = 384;  // warps 0-3 and 4-7: the halves; 8: products; 9, 10: copies; 11: what has arrived
 // Registers: 168 a thread at launch; a half's threads hold a row of 128 scores,
 // so the other four warps give theirs up: 256 x 224 + 128 x 56 = 384 x 168.
 constexpr int kHalfRegs = 224, kOtherRegs = 56;
@@ -559,14 +559,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int h = 0; h < 2; ++h) {
             bar_init(&q_full[h], 1);
             bar_init(&s_full[h], 1);
-            bar_init(&p_full[h][0], 4);
+            bar_init(&p_full[h][0], h == 0 ? 5 : 4);
             bar_init(&p_full[h][1], 4);
             bar_init(&o_full[h], 1);
         }
         bar_init(&q_empty, 1);
         bar_init(&all_bar, 8);
         bar_init(&drained, 1);
-        parts.init(10);
+        parts.init(11);
         s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -662,7 +662,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                            v_lo = uniform(desc_lo_mn(ring, S::kPart));
             int e = 0;
             unsigned phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-            bool ok = true;
             auto qk = [&](int h, int entry) {
                 if (elect_one()) {
 #pragma unroll
@@ -674,72 +673,59 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 }
                 __syncwarp();
             };
-            for (unsigned turn = 0; ok && __all_sync(0xffffffffu, parts.get(turn, &p, &s_gave_up)); ++turn) {
-                const int b0 = uniform(p.b0), b1 = uniform(p.b1), len = uniform(p.len);
+            auto next_entry = [&]() {
+                const int at = e;
+                if (++e == kTileEntries) e = 0, phase ^= 1;
+                return at;
+            };
+            // A wait that ends early is not looked at: the products then run over what is there, and the call's results are
+            // void anyway.  (A vote after each wait cost 45 clocks of the some 250 that queued products hide.)
+            for (unsigned turn = 0; __all_sync(0xffffffffu, parts.get(turn, &p, &s_gave_up)); ++turn) {
+                const int b0 = uniform(p.b0), b1 = uniform(p.b1);
                 const int halves = uniform(p.n_new > (2 * p.tile + 1) * per ? 2 : 1);
-                for (int h = 0; ok && h < halves; ++h) {
-                    ok = bar_wait_warp(&q_full[h], q_phase[h], &s_gave_up);
+                for (int h = 0; h < halves; ++h) {
+                    bar_wait(&q_full[h], q_phase[h], &s_gave_up);
                     q_phase[h] ^= 1;
                 }
-                ok = ok && bar_wait_warp(&full[e], phase, &s_gave_up);
-                if (!ok) break;
+                bar_wait(&full[e], phase, &s_gave_up);
+                const int ke = next_entry();
                 tc_fence_after();
-                qk(0, e);
-                if (halves == 2) qk(1, e);
+                qk(0, ke);
+                if (halves == 2) qk(1, ke);
                 if (elect_one()) {
-                    tc_commit(&empty[e]);
+                    tc_commit(&empty[ke]);
                     if (b1 - b0 == 1) tc_commit(&q_empty);
                 }
-                if (++e == kTileEntries) e = 0, phase ^= 1;
-                for (int b = b0; ok && b < b1; ++b) {
-                    const int ve = e;
-                    ok = bar_wait_warp(&full[ve], phase, &s_gave_up);
-                    if (!ok) break;
-                    if (++e == kTileEntries) e = 0, phase ^= 1;
-                    if ((b + 1) * kTileBlock > len) {
-                        // V at or behind the sequence's end may hold anything: 0 there, since 0 * NaN is NaN.
-                        const int from = max(0, len - b * kTileBlock);
-                        uint8_t* v = smem_raw + (ring - smem_u32(smem_raw)) + ve * S::kEntry;
-                        for (int i = lane; i < kParts * (kTileBlock - from) * 8; i += 32) {
-                            const int h = i / ((kTileBlock - from) * 8), j = i % ((kTileBlock - from) * 8);
-                            *reinterpret_cast<uint4*>(v + h * S::kPart + from * 128 + j * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                    }
+                __syncwarp();
+                for (int b = b0; b < b1; ++b) {
                     const bool more = b + 1 < b1;
-                    if (more) ok = bar_wait_warp(&full[e], phase, &s_gave_up);
+                    const int v_at = next_entry(), k_at = more ? next_entry() : 0;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        if (!ok || h >= halves) break;
+                        if (h >= halves) break;
                         // P comes in two halves of the block's slots; the first one's products hide the second one's making.
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
-                            ok = ok && bar_wait_warp(&p_full[h][g], p_phase[h], &s_gave_up);
-                            if (!ok) break;
+                            bar_wait(&p_full[h][g], p_phase[h], &s_gave_up);
                             tc_fence_after();
                             if (elect_one()) {
 #pragma unroll
                                 for (int kk = g * (kTileBlock / 32); kk < (g + 1) * (kTileBlock / 32); ++kk)
-                                    tc_mma_ts(t_at + 256 + h * 128, t_at + h * 128 + kk * 8, v_lo + ve * (S::kEntry / 16) + kk * (2048 / 16),
+                                    tc_mma_ts(t_at + 256 + h * 128, t_at + h * 128 + kk * 8, v_lo + v_at * (S::kEntry / 16) + kk * (2048 / 16),
                                               kPv, b > b0 || kk > 0);
                                 if (g == 1 && !more) tc_commit(&o_full[h]);
                             }
                             __syncwarp();
                         }
-                        if (!ok) break;
                         p_phase[h] ^= 1;
-                        if (more) qk(h, e);
+                        if (more) qk(h, k_at);
                     }
-                    if (!ok) break;
-                    if (elect_one()) tc_commit(&empty[ve]);
-                    if (more) {
-                        if (elect_one()) {
-                            tc_commit(&empty[e]);
-                            if (b + 2 == b1) tc_commit(&q_empty);
-                        }
-                        if (++e == kTileEntries) e = 0, phase ^= 1;
+                    if (elect_one()) {
+                        tc_commit(&empty[v_at]);
+                        if (more) tc_commit(&empty[k_at]);
+                        if (b + 2 == b1) tc_commit(&q_empty);
                     }
+                    __syncwarp();
                 }
             }
             // Nothing that was issued is left running.
@@ -747,6 +733,38 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (elect_one()) tc_commit(&drained);
             __syncwarp();
             bar_wait(&drained, 0, &none);
+        } else {
+            // A block's V and the next one's K: that they are there counts as part of the first half's P, so the products'
+            // warp has one wait for both (two more of its own left the tensor cores idle for 400 clocks a block).
+            int e = 0;
+            unsigned phase = 0, p_phase = 0;
+            bool ok = true;
+            auto next_entry = [&]() {
+                ok = ok && bar_wait(&full[e], phase, &s_gave_up);
+                if (++e == kTileEntries) e = 0, phase ^= 1;
+            };
+            for (unsigned turn = 0; ok && parts.get(turn, &p, &s_gave_up); ++turn) {
+                next_entry();
+                for (int b = p.b0; ok && b < p.b1; ++b) {
+                    const int ve = e;
+                    next_entry();
+                    if (ok && (b + 1) * kTileBlock > p.len) {
+                        // V at or behind the sequence's end may hold anything: 0 there, since 0 * NaN is NaN.
+                        const int from = max(0, p.len - b * kTileBlock);
+                        uint8_t* v = smem_raw + (ring - smem_u32(smem_raw)) + ve * S::kEntry;
+                        for (int i = lane; i < kParts * (kTileBlock - from) * 8; i += 32) {
+                            const int h = i / ((kTileBlock - from) * 8), j = i % ((kTileBlock - from) * 8);
+                            *reinterpret_cast<uint4*>(v + h * S::kPart + from * 128 + j * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                    if (b + 1 < p.b1) next_entry();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&p_full[0][0]);
+                    ok = ok && bar_wait(&p_full[0][0], p_phase, &s_gave_up);  // not twice in one phase
+                    p_phase ^= 1;
+                }
+            }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kHalfRegs));
