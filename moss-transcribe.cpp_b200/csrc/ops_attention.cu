@@ -703,14 +703,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         if (h >= halves) break;
-                        // P comes in two halves of the block's slots; the first one's products hide the second one's making.
+                        // P comes as three quarters of the block's slots and the last one: the first products hide its making,
+                        // and few are left before the next S (halves: 70.8 us for the prompts against 69.8).
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
                             bar_wait(&p_full[h][g], p_phase[h], &s_gave_up);
                             tc_fence_after();
                             if (elect_one()) {
 #pragma unroll
-                                for (int kk = g * (kTileBlock / 32); kk < (g + 1) * (kTileBlock / 32); ++kk)
+                                for (int kk = g * 6; kk < 6 + 2 * g; ++kk)
                                     tc_mma_ts(t_at + 256 + h * 128, t_at + h * 128 + kk * 8, v_lo + v_at * (S::kEntry / 16) + kk * (2048 / 16),
                                               kPv, b > b0 || kk > 0);
                                 if (g == 1 && !more) tc_commit(&o_full[h]);
@@ -858,11 +859,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             pk[i] = pack2<T>(x.x, x.y);
                         }
                         tmem_st16<0>(t_s + c * 16, pk);
-                        if (c & 1) {
+                        if (c >= 2) {
                             tmem_wait_st();
                             tc_fence_before();
                             __syncwarp();
-                            if (lane == 0) bar_arrive(&p_full[half][c >> 1]);
+                            if (lane == 0) bar_arrive(&p_full[half][c - 2]);
                         }
                     }
                     l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
@@ -1329,17 +1330,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const uint32_t t_at = uniform(tmem), k_lo = uniform(desc_lo_k(k_at)), q_lo = uniform(desc_lo_k(q_at));
             int e = 0, kt = 0, buf = 0;
             unsigned phase = 0, s_phase = 1;  // the first wait for an empty S passes
-            bool ok = true;
-            for (unsigned turn = 0; ok && __all_sync(0xffffffffu, parts.get(turn, &p, &s_gave_up)); ++turn) {
+            // A wait that ends early is not looked at, as above.
+            for (unsigned turn = 0; __all_sync(0xffffffffu, parts.get(turn, &p, &s_gave_up)); ++turn) {
                 const int kb = kt & 1, n = uniform(p.n);
-                if (!bar_wait_warp(&k_full[kb], (kt >> 1) & 1, &s_gave_up)) break;
-                for (int b = 0; ok && b < n; ++b) {
-                    ok = bar_wait_warp(&q_full[e], phase, &s_gave_up);
+                bar_wait(&k_full[kb], (kt >> 1) & 1, &s_gave_up);
+                for (int b = 0; b < n; ++b) {
+                    bar_wait(&q_full[e], phase, &s_gave_up);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        if (!ok) break;
-                        ok = bar_wait_warp(&s_empty[h][buf], s_phase, &s_gave_up);
-                        if (!ok) break;
+                        bar_wait(&s_empty[h][buf], s_phase, &s_gave_up);
                         tc_fence_after();
                         if (elect_one()) {
 #pragma unroll
@@ -1352,13 +1351,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         }
                         __syncwarp();
                     }
-                    if (!ok) break;
                     if (elect_one()) tc_commit(&q_empty[e]);
+                    __syncwarp();
                     if (++e == kWEntries) e = 0, phase ^= 1;
                     buf ^= 1;
                     if (buf == 0) s_phase ^= 1;
                 }
-                if (ok && elect_one()) tc_commit(&k_empty[kb]);
+                if (elect_one()) tc_commit(&k_empty[kb]);
+                __syncwarp();
                 ++kt;
             }
             volatile int none = 0;

@@ -135,9 +135,6 @@ constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
 // for each product (measured: 90 clocks an issue instead of the product's 64).
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
-__device__ __forceinline__ bool bar_wait_warp(uint64_t* b, unsigned parity, volatile int* gave_up) {
-    return __all_sync(0xffffffffu, bar_wait(b, parity, gave_up));
-}
 __device__ __forceinline__ bool elect_one() {
     uint32_t is;
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(is));
