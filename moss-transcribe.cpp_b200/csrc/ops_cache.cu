@@ -19,7 +19,8 @@ namespace cg = cooperative_groups;
 // of 10^6 leaves an error of 0.06), so it is formed and reduced to [-pi, pi] in
 // f64; its sine and cosine are f32 (the results have 16 bits).  They depend on
 // the token alone, so a CTA forms them once in shared memory for all heads.
-// Bound: bytes (q, k, v read and written once); a step's few tokens: latency.
+// Bound: bytes (q, k, v read and written once): 9730 f32 tokens of 16 + 2 x 8 heads of 128 into
+// f16 take 45 us (5.3 TB/s); a step's few tokens: latency (3.2 us).
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeTokens = 4;  // tokens a CTA at most
@@ -188,7 +189,10 @@ cudaError_t rope_typed(const RopeArgs& a, cudaStream_t s) {
 // recording); k_evict_rank, one CTA, takes longer lists and books that are not 16-byte
 // aligned.  The second, k_evict_move, copies the listed rows:
 // sources lie at or behind `keep`, gaps below it, so no row is both and the
-// copies need no order.
+// copies need no order.  Bound: the ranking by latency (three histograms, one after the other: 13 us for one CTA
+// a list, 23 us for clusters of four), the copies by bytes in rows of 256 (four recordings of 25000
+// cut to 8192: some 180 MB in 42 us, 4.3 TB/s; four rows of a warp in flight and as many CTAs as rows
+// want rather than one wave: 72.1 -> 69.5 us in all).
 
 constexpr int kRankThreads = 1024;
 constexpr int kRankBins = 2048;
@@ -510,7 +514,7 @@ __global__ void __launch_bounds__(kRankThreads) k_evict_rank_regs(EvictArgs a, i
 }
 
 constexpr int kMoveThreads = 256;
-constexpr int kMoveBatch = 8;  // rows of a warp in flight
+constexpr int kMoveBatch = 4;  // rows of a warp in flight
 
 __global__ void __launch_bounds__(kMoveThreads) k_evict_move(EvictArgs a, int lists) {
     asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the ranking still runs
@@ -596,7 +600,7 @@ cudaError_t launch_cache_evict(const EvictArgs& a, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const long long most = std::min<long long>(a.keep, most_len / 2);
     const int rows = kMoveThreads / 32 * kMoveBatch;
-    const int wide = (int)std::max<long long>(1, std::min<long long>((most + rows - 1) / rows, 1 + 148 * 8 / lists));
+    const int wide = (int)std::max<long long>(1, std::min<long long>((most + rows - 1) / rows, 1 + 148 * 32 / lists));
     cfg.gridDim = dim3(wide, std::min(lists, 65535));
     cfg.blockDim = dim3(kMoveThreads);
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

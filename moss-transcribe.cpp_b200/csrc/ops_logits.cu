@@ -1,19 +1,21 @@
 // mtb_logits_process: penalties for repeated tokens, biases and grammar masks
 // on logits rows, with the greedy choice.
 //
-// Bound: bytes (each logit read and written once); one row of 152 k values: latency.
+// Bound: bytes (each logit read and written once); one row of 152 k values: latency (7.5 us).
+// 256 f32 rows, half of the ids masked: 55 us without lists (5.7 TB/s, a plain copy 49 us), 85 us
+// with 4096 ids of history and 300 biases a row (3.7 TB/s): a CTA forms its lists before its stream starts.
 // A row belongs to 1 to 16 CTAs, as many as fill the SMs (one from 128 rows on: two
 // CTAs to an SM, each a row; clusters of more take longer to place than they save).
 // The vocabulary goes round a row's CTAs in runs of 1024 ids, since histories crowd at
-// low ids.  What touches few ids is set apart: a hash table in shared memory takes the ids of
-// the row's history and biases that are the CTA's, with their counts (low half of a
-// word) and last bias entry + 1 (high half), and a bitmap says which ids it has.  The
-// table's words then become the ids' new values.  The logits stream through once: masked ones to
-// -inf, those of the bitmap from the table (writing them behind the stream instead cost 256 rows
-// with 4096 ids of history 35 us in sectors written twice, and penalties within the
-// stream as much in divergence).  Lists of more than 6144
-// entries, or shares of more than 262144 ids, go in slices of 8192 ids with two words each
-// instead.  The row's choice joins the CTAs' in the first one's shared
+// low ids.  What touches few ids is set apart: a bitmap in shared memory says which of the
+// CTA's ids are in the row's history or biases; an id's rank among them (the bits before its
+// word, summed once, and those before it in the word) is its place in a list of words, with its count (low
+// half) and last bias entry + 1 (high half), and in a list of its new value.  The logits
+// stream through once: masked ones to -inf, those of the bitmap from the list (writing them behind the
+// stream instead cost 256 rows with 4096 ids of history 35 us in sectors written twice,
+// penalties within the stream as much in divergence, a hash table's search there 10 us).
+// Lists of more than 6144 entries, or shares of more than 262144 ids, go in slices of
+// 8192 ids with two words each instead.  The row's choice joins the CTAs' in the first one's shared
 // memory: no workspace, no atomics on values, and an order that does not matter
 // (largest value, then lowest id).
 #include "ops_common.cuh"
@@ -30,10 +32,11 @@ namespace cg = cooperative_groups;
 
 constexpr int kLogitsThreads = 512;
 constexpr int kLogitsRun = 1024;
-constexpr int kTableSlots = 8192;         // hash table: ids, then words; or a slice's two words an id
-constexpr int kTableMost = 6144;          // entries of history and biases that it takes
+constexpr int kTableSlots = 8192;         // ids of a slice, two words each
+constexpr int kTableMost = 6144;          // entries of history and biases that the lists by rank take
 constexpr int kShareMost = 32768 * 8;     // ids of the bitmap
 constexpr int kTableBytes = kTableSlots * 8;
+static_assert(kTableMost * 8 + kShareMost / 32 * 2 <= kTableBytes, "words, values and the words' sums of bits in a slice's place");
 constexpr int kLogitsBatch = 5;           // 16-byte loads of a thread in flight
 constexpr int kLogitsHeld = 8;            // history ids a thread reads ahead
 
@@ -105,11 +108,11 @@ struct Penalties {
 };
 
 // Places [s0, s0 + n) through: penalties and biases for those of the bitmap (of the n
-// places, or null), as `change` of place and value has them; masks; the choice.  `got`
-// holds the first batch.
-template <class T, bool kVec, class F>
+// places, or null), as `change` of a value or `patch` of a vector has them; masks; the
+// choice.  `got` holds the first batch.
+template <class T, bool kVec, class F, class G>
 __device__ __forceinline__ void stream(const LogitsArgs& a, const Share& sh, const T* x, T* y, Batch<T, kVec>& got, int s0, int n,
-                                       const unsigned* s_bits, F&& change, Best& best) {
+                                       const unsigned* s_bits, F&& change, G&& patch, Best& best) {
     constexpr int per = Batch<T, kVec>::per;
 #pragma unroll 1
     for (int i0 = threadIdx.x * per; i0 < n; i0 += Batch<T, kVec>::kStep) {
@@ -117,22 +120,14 @@ __device__ __forceinline__ void stream(const LogitsArgs& a, const Share& sh, con
         for (int u = 0; u < kLogitsBatch; ++u) {
             const int i = i0 + u * kLogitsThreads * per, id = sh.id_of(s0 + i);
             if (i >= n || id >= a.vocab) break;
-            const unsigned touched = s_bits ? s_bits[i >> 5] >> (i & 31) : 0u;
+            const unsigned word = s_bits ? s_bits[i >> 5] : 0u, touched = word >> (i & 31);
             if (id + per <= a.vocab) {
                 const T* t = reinterpret_cast<const T*>(&got.raw[u]);
                 float v[per];
 #pragma unroll
                 for (int e = 0; e < per; ++e) v[e] = to_f32<T>(t[e]);
-#pragma unroll 1
-                for (unsigned bits = touched & got.allowed[u] & ((1u << per) - 1); bits; bits &= bits - 1) {
-                    const int at = __ffs(bits) - 1;
-                    float w = v[0];
-#pragma unroll
-                    for (int e = 1; e < per; ++e) w = e == at ? v[e] : w;
-                    w = change(i + at, id + at, w);
-#pragma unroll
-                    for (int e = 0; e < per; ++e) v[e] = e == at ? w : v[e];
-                }
+                const unsigned hit = touched & got.allowed[u] & ((1u << per) - 1);
+                if (hit) patch(v, word, hit, i, id);
                 if (sh.mask) {
 #pragma unroll
                     for (int e = 0; e < per; ++e)
@@ -170,88 +165,128 @@ __device__ __forceinline__ void stream(const LogitsArgs& a, const Share& sh, con
     }
 }
 
-// The share with its touched ids in the hash table.
+// The share with its touched ids in lists by their rank.
 template <class T, bool kVec>
-__device__ __forceinline__ Best share_hashed(const LogitsArgs& a, const Share& sh, Batch<T, kVec>& got, unsigned* s_table, unsigned* s_bits) {
+__device__ __forceinline__ Best share_ranked(const LogitsArgs& a, const Share& sh, Batch<T, kVec>& got, unsigned* s_table, unsigned* s_bits) {
+    __shared__ int s_warp[kLogitsThreads / 32];
+    constexpr int per = Batch<T, kVec>::per;
     const T* x = reinterpret_cast<const T*>(a.x) + sh.row * a.x_stride;
     T* y = a.y ? reinterpret_cast<T*>(a.y) + sh.row * a.y_stride : nullptr;
     const bool few = sh.h1 > sh.h0 || sh.b1 > sh.b0;
-    // Slots: twice the entries at least, a power of two.
-    const int entries = sh.h1 - sh.h0 + sh.b1 - sh.b0;
-    const int log_slots = min(13, max(9, 33 - __clz(entries | 1))), slots = 1 << log_slots;
-    int* s_id = reinterpret_cast<int*>(s_table);
-    unsigned* s_word = s_table + slots;
+    unsigned* s_word = s_table;
+    float* s_value = reinterpret_cast<float*>(s_table + kTableMost);
+    uint16_t* s_before = reinterpret_cast<uint16_t*>(s_table + 2 * kTableMost);
+    auto rank = [&](int place) { return s_before[place >> 5] + __popc(s_bits[place >> 5] & ((1u << (place & 31)) - 1)); };
     Best best{-INFINITY, -1};
-    got.masks(sh, a.vocab, threadIdx.x * Batch<T, kVec>::per);
+    got.masks(sh, a.vocab, threadIdx.x * per);
     if (few) {
-        int held[kLogitsHeld];
+        int at[kLogitsHeld];  // places of the first ids, negative: not the CTA's
+        float value[kLogitsHeld];
 #pragma unroll
         for (int k = 0; k < kLogitsHeld; ++k) {
             const int i = sh.h0 + threadIdx.x + k * kLogitsThreads;
-            held[k] = i < sh.h1 ? a.hist[i] : -1;
+            at[k] = i < sh.h1 ? a.hist[i] : -1;
         }
-        for (int i = threadIdx.x * 4; i < slots; i += kLogitsThreads * 4) {
-            *reinterpret_cast<int4*>(s_id + i) = make_int4(-1, -1, -1, -1);
-            *reinterpret_cast<uint4*>(s_word + i) = make_uint4(0, 0, 0, 0);
+        const int entries = sh.h1 - sh.h0 + sh.b1 - sh.b0, words = sh.places / 32;
+        for (int i = threadIdx.x; i < entries; i += kLogitsThreads) s_word[i] = 0u;
+        for (int i = threadIdx.x; i < words; i += kLogitsThreads) s_bits[i] = 0u;
+#pragma unroll
+        for (int k = 0; k < kLogitsHeld; ++k) {
+            const int id = at[k];
+            at[k] = sh.place_of(id, a.vocab);
+            value[k] = at[k] >= 0 ? to_f32<T>(x[id]) : 0.f;
         }
-        for (int i = threadIdx.x; i < sh.places / 32; i += kLogitsThreads) s_bits[i] = 0u;
         __syncthreads();
-        // The id's slot, taken if it is new; negative if it is not the CTA's.
-        // There are fewer entries than slots: the search ends.
-        auto slot_of = [&](int id) {
-            const int at = sh.place_of(id, a.vocab);
-            if (at < 0) return -1;
-            unsigned slot = ((unsigned)id * 2654435769u) >> (32 - log_slots);
-#pragma unroll 1
-            for (int tries = 0; tries < slots; ++tries) {
-                const int had = atomicCAS(&s_id[slot], -1, id);
-                if (had == -1) atomicOr(&s_bits[at >> 5], 1u << (at & 31));
-                if (had == -1 || had == id) return (int)slot;
-                slot = (slot + 1) & (slots - 1);
-            }
-            return -1;
+        // Entries behind those that the thread holds, and the biases.
+        const int h_rest = sh.h0 + kLogitsHeld * kLogitsThreads;
+        auto mark = [&](int place) {
+            if (place >= 0) atomicOr(&s_bits[place >> 5], 1u << (place & 31));
         };
+#pragma unroll
+        for (int k = 0; k < kLogitsHeld; ++k) mark(at[k]);
+#pragma unroll 1
+        for (int i = h_rest + threadIdx.x; i < sh.h1; i += kLogitsThreads) mark(sh.place_of(a.hist[i], a.vocab));
+#pragma unroll 1
+        for (int i = sh.b0 + threadIdx.x; i < sh.b1; i += kLogitsThreads) mark(sh.place_of(a.bias_ids[i], a.vocab));
+        __syncthreads();
+        // Bits before each word: a thread has consecutive words, an odd number (no two lanes of a warp on one bank).
+        const int each = (words / kLogitsThreads + 1) | 1;
+        const int w0 = min(words, (int)threadIdx.x * each), w1 = min(words, w0 + each), lane = threadIdx.x & 31;
+        int sum = 0;
+#pragma unroll 1
+        for (int i = w0; i < w1; ++i) sum += __popc(s_bits[i]);
+        int upto = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int z = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += z;
+        }
+        if (lane == 31) s_warp[threadIdx.x >> 5] = upto;
+        __syncthreads();
+        int before = upto - sum;
+#pragma unroll
+        for (int w = 0; w < kLogitsThreads / 32; ++w)
+            if (w < (int)(threadIdx.x >> 5)) before += s_warp[w];
+#pragma unroll 1
+        for (int i = w0; i < w1; ++i) {
+            s_before[i] = (uint16_t)before;
+            before += __popc(s_bits[i]);
+        }
+        __syncthreads();
         if (sh.b1 > sh.b0) {
 #pragma unroll 1
             for (int i = sh.b0 + threadIdx.x; i < sh.b1; i += kLogitsThreads) {
-                const int slot = slot_of(a.bias_ids[i]);
-                if (slot >= 0) atomicMax(&s_word[slot], ((unsigned)(i - sh.b0) + 1u) << 16);
+                const int place = sh.place_of(a.bias_ids[i], a.vocab);
+                if (place >= 0) atomicMax(&s_word[rank(place)], ((unsigned)(i - sh.b0) + 1u) << 16);
             }
             __syncthreads();  // counts are added below the bias entries
         }
-        auto count = [&](int id) {
-            const int slot = slot_of(id);
-            if (slot >= 0) atomicAdd(&s_word[slot], 1u);
+#pragma unroll
+        for (int k = 0; k < kLogitsHeld; ++k)
+            if (at[k] >= 0) atomicAdd(&s_word[rank(at[k])], 1u);
+#pragma unroll 1
+        for (int i = h_rest + threadIdx.x; i < sh.h1; i += kLogitsThreads) {
+            const int place = sh.place_of(a.hist[i], a.vocab);
+            if (place >= 0) atomicAdd(&s_word[rank(place)], 1u);
+        }
+        __syncthreads();
+        // The new values; an id that occurs several times gets the same one each time.
+        const Penalties penalties(a, sh);
+        auto renew = [&](int place, float v) {
+            if (place < 0) return;
+            const int r = rank(place);
+            s_value[r] = penalties(v, s_word[r] & 0xffffu, (int)(s_word[r] >> 16) - 1);
         };
 #pragma unroll 1
-        for (int k = 0; k < kLogitsHeld; ++k) {
-            int id = -1;
+        for (int k = 0; k < kLogitsHeld && k * kLogitsThreads < sh.h1 - sh.h0; ++k) {
+            int place = -1;
+            float v = 0.f;
 #pragma unroll
-            for (int j = 0; j < kLogitsHeld; ++j) id = j == k ? held[j] : id;
-            if (sh.h0 + threadIdx.x + k * kLogitsThreads < sh.h1) count(id);
+            for (int j = 0; j < kLogitsHeld; ++j)
+                if (j == k) place = at[j], v = value[j];
+            renew(place, v);
         }
 #pragma unroll 1
-        for (int i = sh.h0 + threadIdx.x + kLogitsHeld * kLogitsThreads; i < sh.h1; i += kLogitsThreads) count(a.hist[i]);
-        __syncthreads();
-    }
-    if (few) {
-        const Penalties penalties(a, sh);
-#pragma unroll 4
-        for (int k = threadIdx.x; k < slots; k += kLogitsThreads) {
-            const int id = s_id[k];
-            if (id < 0) continue;
-            const unsigned word = s_word[k];
-            s_word[k] = __float_as_uint(penalties(to_f32<T>(x[id]), word & 0xffffu, (int)(word >> 16) - 1));
+        for (int i = h_rest + threadIdx.x; i < sh.h1; i += kLogitsThreads) {
+            const int id = a.hist[i], place = sh.place_of(id, a.vocab);
+            if (place >= 0) renew(place, to_f32<T>(x[id]));
+        }
+#pragma unroll 1
+        for (int i = sh.b0 + threadIdx.x; i < sh.b1; i += kLogitsThreads) {
+            const int id = a.bias_ids[i], place = sh.place_of(id, a.vocab);
+            if (place >= 0) renew(place, to_f32<T>(x[id]));
         }
         __syncthreads();
     }
-    auto change = [&](int, int id, float) {
-        unsigned slot = ((unsigned)id * 2654435769u) >> (32 - log_slots);
-#pragma unroll 1
-        for (int tries = 0; tries < slots && s_id[slot] != id; ++tries) slot = (slot + 1) & (slots - 1);
-        return __uint_as_float(s_word[slot]);
+    auto change = [&](int place, int, float) { return s_value[rank(place)]; };
+    auto patch = [&](float (&v)[per], unsigned word, unsigned hit, int place, int) {
+        const int first = s_before[place >> 5] + __popc(word & ((1u << (place & 31)) - 1));
+        const unsigned touched = word >> (place & 31);
+#pragma unroll
+        for (int e = 0; e < per; ++e)
+            if ((hit >> e) & 1u) v[e] = s_value[first + __popc(touched & ((1u << e) - 1))];
     };
-    stream<T, kVec>(a, sh, x, y, got, 0, sh.places, few ? s_bits : nullptr, change, best);
+    stream<T, kVec>(a, sh, x, y, got, 0, sh.places, few ? s_bits : nullptr, change, patch, best);
     return best;
 }
 
@@ -262,7 +297,20 @@ __device__ __forceinline__ Best share_sliced(const LogitsArgs& a, const Share& s
     T* y = a.y ? reinterpret_cast<T*>(a.y) + sh.row * a.y_stride : nullptr;
     unsigned *s_count = s_table, *s_entry = s_table + kTableSlots;
     const Penalties penalties(a, sh);
+    constexpr int per = Batch<T, kVec>::per;
     auto change = [&](int place, int, float v) { return penalties(v, (int)s_count[place], (int)s_entry[place] - 1); };
+    auto patch = [&](float (&v)[per], unsigned, unsigned hit, int place, int id) {
+#pragma unroll 1
+        for (; hit; hit &= hit - 1) {
+            const int at = __ffs(hit) - 1;
+            float w = v[0];
+#pragma unroll
+            for (int e = 1; e < per; ++e) w = e == at ? v[e] : w;
+            w = change(place + at, id + at, w);
+#pragma unroll
+            for (int e = 0; e < per; ++e) v[e] = e == at ? w : v[e];
+        }
+    };
     Best best{-INFINITY, -1};
     for (int s0 = 0; s0 < sh.places; s0 += kTableSlots) {
         const int n = min(kTableSlots, sh.places - s0);
@@ -288,7 +336,7 @@ __device__ __forceinline__ Best share_sliced(const LogitsArgs& a, const Share& s
         __syncthreads();
         got.fetch(x, sh, a.vocab, s0 + threadIdx.x * Batch<T, kVec>::per);
         got.masks(sh, a.vocab, s0 + threadIdx.x * Batch<T, kVec>::per);
-        stream<T, kVec>(a, sh, x, y, got, s0, n, s_bits, change, best);
+        stream<T, kVec>(a, sh, x, y, got, s0, n, s_bits, change, patch, best);
         __syncthreads();  // the words are used again
     }
     return best;
@@ -325,7 +373,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(const __grid_const
     }
     const long long entries = (long long)(sh.h1 - sh.h0) + (sh.b1 - sh.b0);
     Best best = entries > 0 && (entries > kTableMost || sh.places > kShareMost) ? share_sliced<T, kVec>(a, sh, got, s_table, s_bits)
-                                                                               : share_hashed<T, kVec>(a, sh, got, s_table, s_bits);
+                                                                               : share_ranked<T, kVec>(a, sh, got, s_table, s_bits);
     best = warp_best(best);
     if ((threadIdx.x & 31) == 0) s_best[threadIdx.x >> 5] = best;
     __syncthreads();
