@@ -17,8 +17,8 @@ namespace {
 using namespace ops;
 
 // Units that stand for a tile's own cost, and those of a CTA's interval at least.
-// Tiles of a chunk: prompts of 33 .. 2048 rows take 101 us without them, 77.5 with 1, 74.8
-// with 2, 77.8 with 3.  Few rows: eight ragged sequences 61.0 us with 1, 57.4 with 2, 56.5
+// Tiles of a chunk: prompts of 1 .. 2048 rows take 73.7 us with 1, 70.0 with 2, 72.5
+// with 3.  Few rows: eight ragged sequences 61.0 us with 1, 57.4 with 2, 56.5
 // with 4, 56.2 with 6; one token over 408 slots 13.2 us cut at 8 units, 8.3 at 16.
 constexpr int kRowsExtra = 4, kRowsMinUnits = 16;    // of 64 slots
 constexpr int kTilesExtra = 2, kTilesMinUnits = 4;  // of 128 slots
@@ -111,7 +111,9 @@ bool encode_q(CUtensorMap* map, const AttnArgs& a, int rows) {
 // registers as the second product's operand), so that no page costs a barrier among them;
 // they are joined when the tile's part ends.  16 rows: two such sets of
 // four warps take the pages in turn (a page is a chain of dependent steps, two
-// chains fill each other's gaps).
+// chains fill each other's gaps).  16 heads of 128 over 8 KV heads: one token over 27000
+// slots 25.9 us (4.3 TB/s: the start, the last pages and the join are a third of it), 32 sequences of 2048
+// slots 51 us (5.3 TB/s), eight ragged sequences of 1 .. 8 new tokens 57 us (5.4 TB/s).
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -514,7 +516,12 @@ cudaError_t launch_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensor
 // so maxima and sums need no other thread) turn S into P, the tensor cores work for the
 // other.  P takes the place of S.  A half's products run in order, so S of block
 // j + 1 is issued behind P V of block j without a wait, and once S is there O is
-// free to be rescaled.
+// free to be rescaled.  2048 new tokens over 24576 slots, 16 heads of 128: 313 us,
+// 1.26 PFLOP/s, 75% of what a library product reaches in a burst and 91% of what it holds for
+// seconds; a fresh prompt of 4096 tokens 81 us (0.85 PFLOP/s counting what is
+// masked as not done).  A steady block takes 3200 clocks for both halves where the products
+// alone take 2048: a half's chain from S over its maximum (450) and exponentials (1540) to P
+// and the next S is as long as that.
 constexpr int kTileRows2 = 256;
 constexpr int kTileBlock = 128;
 constexpr int kTileThreads = 384;  // warps 0-3 and 4-7: the halves; 8: products; 9, 10: copies; 11: what has arrived
@@ -740,15 +747,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             int e = 0;
             unsigned phase = 0, p_phase = 0;
             bool ok = true;
-            auto next_entry = [&]() {
-                ok = ok && bar_wait(&full[e], phase, &s_gave_up);
+            auto next_entry = [&](bool wait) {
+                if (wait) ok = ok && bar_wait(&full[e], phase, &s_gave_up);
                 if (++e == kTileEntries) e = 0, phase ^= 1;
             };
             for (unsigned turn = 0; ok && parts.get(turn, &p, &s_gave_up); ++turn) {
-                next_entry();
+                // The first K: the products' warp waits for it, and may have given it back, and seen it filled again, before
+                // this warp comes by.  The others are not given back without this warp's arrival.
+                next_entry(false);
                 for (int b = p.b0; ok && b < p.b1; ++b) {
                     const int ve = e;
-                    next_entry();
+                    next_entry(true);
                     if (ok && (b + 1) * kTileBlock > p.len) {
                         // V at or behind the sequence's end may hold anything: 0 there, since 0 * NaN is NaN.
                         const int from = max(0, p.len - b * kTileBlock);
@@ -759,7 +768,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     }
-                    if (b + 1 < p.b1) next_entry();
+                    if (b + 1 < p.b1) next_entry(true);
                     __syncwarp();
                     if (lane == 0) bar_arrive(&p_full[0][0]);
                     ok = ok && bar_wait(&p_full[0][0], p_phase, &s_gave_up);  // not twice in one phase
@@ -948,6 +957,7 @@ cudaError_t launch_tiles(const AttnArgs& a, const CUtensorMap& km, const CUtenso
 // set of four warps takes a page, 16 slots a warp, two sets in turn; a thread adds its rows' probabilities of
 // its columns, and eight lanes' sums make a slot's.  All rows of a (sequence, KV head)
 // pass over the part's pages 64 at a time, so nothing is joined between CTAs.
+// Eight ragged sequences of 1 .. 8 new tokens, 64 .. 27000 slots: 36 us for 154 MB of K.
 constexpr int kWRows = 64;
 constexpr int kWWarps = 8, kWThreads = (kWWarps + 1) * 32;
 
@@ -1165,12 +1175,14 @@ __global__ void __launch_bounds__(kWThreads, 1)
 // one thread's.  A tile of 256 slots (two halves of 128, four warps each) stays in
 // shared memory while the rows that see it stream past, 128 / G whole tokens at a time
 // with their log-sums; S is double-buffered in tensor memory, so the products run
-// ahead.  The exponentials bound it: one for each product of 128 dims.
+// ahead.  The exponentials bound it: one for each product of 128 dims.  2048 new
+// tokens over 24576 slots, 16 heads: 256 us (0.77 PFLOP/s); 768 tiles on 148 SMs
+// leave a seventh of that idle (smaller tiles of slots read the rows more often).
 constexpr int kWTileSlots = 256, kWTileRows = 128;
 constexpr int kWEntries = 2;  // ring of row tiles
 // Of eight pairs of exponentials, those that go to the FMA units (the polynomial
 // above) and not to the special function units: the long chunk takes 274 us with none,
-// 256 with 1, 255 with 2, 269 with 3, 322 with 4.  (The attention is fastest with none, 340 us; 344, 356, 366, 376.)
+// 256 with 1, 255 with 2, 269 with 3, 322 with 4.
 constexpr int kPolyOf8 = 2;
 constexpr int kWLse = 4;      // ring of their log-sums
 
