@@ -1177,7 +1177,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
 // with their log-sums; S is double-buffered in tensor memory, so the products run
 // ahead.  The exponentials bound it: one for each product of 128 dims.  2048 new
 // tokens over 24576 slots, 16 heads: 256 us (0.77 PFLOP/s); 768 tiles on 148 SMs
-// leave a seventh of that idle (smaller tiles of slots read the rows more often).
+// leave a seventh of that idle.  Tiles of 128 slots whose rows the halves take in turn: a
+// fresh prompt of 4096 tokens 83 us instead of 115, this chunk 262, 128 rows over 8192 slots 27 instead of 19.
 constexpr int kWTileSlots = 256, kWTileRows = 128;
 constexpr int kWEntries = 2;  // ring of row tiles
 // Of eight pairs of exponentials, those that go to the FMA units (the polynomial
