@@ -249,6 +249,17 @@ def test_attention_many_sequences():
     run_attention(ref.make_cache(kv, 1, 64, torch.bfloat16, DEV), new, 2, decay=0.0)
 
 
+@pytest.mark.parametrize("dim,group", [(64, 1), (128, 2), (64, 8), (128, 3)])
+def test_attention_chunks_of_many_ragged_sequences(dim, group):
+    """Tiles of one and of two halves, of one block and of many, in turn within a CTA's interval; the same bits each time."""
+    new = [(0, 1, 5, 64, 65, 130, 257, 33)[i % 8] for i in range(61)]
+    kv = [n + (53 * i * i) % 700 for i, n in enumerate(new)]
+    c = ref.make_cache(kv, 3, dim, torch.bfloat16, DEV)
+    first = run_attention(c, new, 3 * group, decay=0.0)[1]
+    for _ in range(3):
+        assert torch.equal(run_attention(c, new, 3 * group, decay=0.0)[1], first)
+
+
 @pytest.mark.parametrize("new", [[3, 2, 1, 4], [300, 140, 1, 150]])
 def test_attention_rows_that_see_nothing(new):
     """Sequences shorter than their new tokens: the rows before the first slot see nothing."""
@@ -561,6 +572,15 @@ def test_logits_parts_alone_and_many_rows():
     for part in ("repetition", "presence", "frequency"):
         run_logits(4, 777, torch.float32, hist=50, parts=(part,))
     run_logits(300, 501, torch.bfloat16, hist=20, biases=3, masked=0.5)
+
+
+@pytest.mark.parametrize("rows,vocab,hist,biases", [
+    (2, 151936, 4096, 1), (2, 20011, 4097, 300), (130, 5003, 4500, 100), (130, 1000, 6100, 44), (130, 1000, 6100, 45), (3, 9999, 1, 6143),
+    (3, 9999, 6145, 0), (130, 262144, 40, 3), (130, 262145, 40, 3)])
+def test_logits_list_lengths_and_shares_at_their_limits(rows, vocab, hist, biases):
+    """Entries beyond those that a thread holds, lists of 6144 entries and one more, a share of 262144 ids and one more."""
+    run_logits(rows, vocab, torch.float16, hist=hist, biases=biases, masked=0.3, seed=rows + hist)
+    run_logits(rows, vocab, torch.float16, hist=hist, biases=biases, seed=hist, in_place=True, lead=1)
 
 
 def test_logits_nothing_allowed_nan_and_shared_masks():
