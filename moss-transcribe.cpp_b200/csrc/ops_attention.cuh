@@ -268,10 +268,11 @@ struct Line {
 };
 
 // As many CTAs as there are, but fewer where their intervals would be shorter
-// than min_units, unless there is a tile for each.
+// than min_units, unless there is a tile for each.  Never more than units: a split
+// tile's parts are counted by the intervals it spans, so none of them may be empty.
 __device__ __forceinline__ void cut_line(Line* l, int min_units) {
     const long long fit = max(max(1ll, l->tiles), l->total / min_units);
-    l->ctas = l->total ? (int)min((long long)gridDim.x, fit) : 0;
+    l->ctas = (int)min(min((long long)gridDim.x, fit), l->total);
     l->lo = l->hi = 0;
     if ((int)blockIdx.x < l->ctas) {
         l->lo = share_of(l->total, blockIdx.x, l->ctas);
@@ -315,12 +316,15 @@ template <int kThreads, class Cut>
 __device__ __noinline__ Line find_line_cta(const AttnArgs& a, const Geometry ge, int min_units, long long* s_scan) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     constexpr int kWarps = kThreads / 32;
-    auto units_of = [&](int s, bool report) {
+    __shared__ int s_tiles[kWarps];
+    int tiles = 0;
+    auto units_of = [&](int s, bool first) {
         SeqWork w{0, 0, 0};
         if (s < a.c.n_seq) {
             w = seq_work(a, s);
-            if (report && w.n_new > w.len && blockIdx.x == 0) flag(a.c, BAD_LEN);
+            if (first && w.n_new > w.len && blockIdx.x == 0) flag(a.c, BAD_LEN);
         }
+        if (first) tiles += (int)min((long long)Cut::tiles(w, ge) * a.c.n_kv, (long long)kMaxCtas);
         return head_units<Cut>(w, ge) * a.c.n_kv;
     };
     long long mine = 0, sum = 0;
@@ -329,13 +333,21 @@ __device__ __noinline__ Line find_line_cta(const AttnArgs& a, const Geometry ge,
         sum += mine;
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) s_scan[warp] = sum;
+    for (int o = 16; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    }
+    if (lane == 0) {
+        s_scan[warp] = sum;
+        s_tiles[warp] = tiles;
+    }
     __syncthreads();
     Line l{};
 #pragma unroll 1
-    for (int w = 0; w < kWarps; ++w) l.total += s_scan[w];
-    l.tiles = kMaxCtas;  // more sequences than 32: hardly fewer tiles than CTAs
+    for (int w = 0; w < kWarps; ++w) {
+        l.total += s_scan[w];
+        l.tiles += s_tiles[w];
+    }
     cut_line(&l, min_units);
     long long base = 0;
     for (int s0 = 0; s0 < a.c.n_seq; s0 += kThreads) {
