@@ -1205,8 +1205,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         drained;
     __shared__ PartRing<kPartRing> parts;
     __shared__ long long s_scan[16];
-    __shared__ __align__(16) float s_less[kWLse][kWTileRows];  // - lse log2 e
+    __shared__ __align__(16) float s_less[kWLse][kWTileRows];  // - lse log2 e; -inf adds nothing
     __shared__ int s_sees[kWLse][kWTileRows];                  // slots that the row sees
+    __shared__ int s_nan[kWLse];                               // slots that a row sees whose log-sum is NaN
     __shared__ int s_gave_up;
     __shared__ uint32_t s_tmem;
     const uint32_t k_at = (smem_u32(smem_raw) + 1023) & ~1023u;
@@ -1321,19 +1322,25 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         ok = false;
                         break;
                     }
+                    unsigned nan = 0;
 #pragma unroll
                     for (int i = 0; i < kWTileRows / 32; ++i) {
                         const int r = i * 32 + lane, tok = (q0 + b) * per + ge.by_G(r);
                         float less = 0.f;
                         int sees = 0;
                         if (r < live && tok < p.n_new) {
-                            less = -a.lse[(long long)(p.tok0 + tok) * a.n_heads + p.head * G + r - ge.by_G(r) * G] * kLog2e;
+                            const float x = -a.lse[(long long)(p.tok0 + tok) * a.n_heads + p.head * G + r - ge.by_G(r) * G] * kLog2e;
                             sees = base + tok + 1;
-                            if (sees <= 0) less = 0.f;  // sees nothing: all masked, and -inf + inf would be NaN
+                            // No slot (lse -inf: none at all, or bad pages only) and NaN: -inf, for a masked score's -inf plus
+                            // either would be NaN where the row sees nothing.  What a NaN row does see becomes NaN at the end.
+                            less = x < INFINITY ? x : -INFINITY;
+                            if (isnan(x)) nan = max(nan, (unsigned)max(sees, 0));
                         }
                         s_less[e][r] = less;
                         s_sees[e][r] = sees;
                     }
+                    nan = __reduce_max_sync(0xffffffffu, nan);
+                    if (lane == 0) s_nan[e] = (int)nan;
                     bar_arrive(&l_full[e]);
                     if (++e == kWLse) e = 0, ++round;
                 }
@@ -1430,6 +1437,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     sum[0] = __fadd2_rn(sum[0], x);
                     sum[1] = __fadd2_rn(sum[1], y);
                 }
+                if (slot < s_nan[e]) sum[0].x = NAN;
                 __syncwarp();
                 if (lane == 0) bar_arrive(&l_empty[e]);
                 if (++e == kWLse) e = 0, phase ^= 1;

@@ -56,3 +56,83 @@ def test_sparse_batches_are_joined(n_seq, kv_heads, group, active):
     attend(ref.make_cache(kv, kv_heads, 64, torch.bfloat16, DEV), new, kv_heads * group, ws)
     attend(ref.make_cache([5000, 300, 2500], 2, 128, torch.bfloat16, DEV), [1, 1, 1], 4, ws)
     attend(ref.make_cache([3000, 700], 2, 128, torch.bfloat16, DEV), [200, 100], 4, ws)
+
+
+# ---- weights: rows that see bad pages only, rows that are NaN --------------------------------------------------------
+
+
+def weights_of(c, new, q, skip=()):
+    """(the weight each slot received in 64 bits, slots that hold one): slots of pages outside the pool count as masked; rows whose
+    log-sum is -inf, and (token, head) of `skip`, give nothing."""
+    D, G = c["dim"], q.shape[1] // c["kv_heads"]
+    want, held = torch.zeros(c["weight"].shape, dtype=torch.float64, device=DEV), torch.zeros(c["weight"].shape, dtype=torch.bool, device=DEV)
+    at = 0
+    for s, (n, m) in enumerate(zip(c["kv"], new)):
+        page, place = ref.rows_of(c, s, n)
+        good = (page >= 0) & (page < c["pool"].shape[0])
+        sees = (torch.arange(n, device=DEV)[None] <= (n - m + torch.arange(m, device=DEV))[:, None]) & good[None]
+        page, place, sees = page[good], place[good], sees[:, good]
+        for h in range(q.shape[1] if m else 0):
+            a = (q[at:at + m, h].double() @ c["k"][page, h // G, place].double().T / math.sqrt(D)).masked_fill(~sees, -math.inf)
+            p = torch.softmax(a, 1).masked_fill(~sees, 0.0)  # a row without slots: NaN, all masked
+            for t, head in skip:
+                if head == h and at <= t < at + m:
+                    p[t - at] = 0.0
+            want[page, h // G, place] += p.sum(0)
+        if m:
+            held[page, :, place] = True
+        at += m
+    return want, held
+
+
+def check_weights(got, want, held, old, decay, terms):
+    """Each term's relative error is below 2^-17 (scores of normal values: 2 e + the log-sum's error + 2^-20 of test_gpu_ops.py, whose e is
+    (D + 4) 2^-24 S with S below 40 here), and `terms` of them are added in 32 bits."""
+    want = want + decay * old.double()
+    assert torch.equal(got[~held], old[~held])
+    off = ((got.double() - want).abs() - (2.0 ** -10 + terms * 2.0 ** -24) * want.abs() - 1e-37)[held]
+    assert bool((off <= 0).all()), float(off.max())
+
+
+@pytest.mark.parametrize("max_tokens", [1, 0])  # the kernel for few rows, and the one for many
+@pytest.mark.parametrize("new,bad", [([130], [0]), ([130, 70], [0]), ([300, 40], [0, 2]), ([200], [1]), ([64], [0])])
+@pytest.mark.parametrize("before", [0, 100])
+def test_weights_of_rows_that_see_bad_pages_only(new, bad, before, max_tokens):
+    """A bad page's slots count as masked; rows that see no others add nothing anywhere, and nothing is written there."""
+    c = ref.make_cache([n + before for n in new], 2, 64, torch.bfloat16, DEV)
+    for p in bad:
+        c["table"][0, p] = -1 if p else 1 << 30
+    q = ops.normal(sum(new), 4, 64, dtype=torch.bfloat16, scale=1.5)
+    out, lse, cu = torch.zeros_like(q), torch.zeros(sum(new), 4, device=DEV), ref.cu_of(new, DEV)
+    want, held = weights_of(c, new, q)
+    for decay in (0.0, 0.5):
+        old = torch.rand(c["weight"].shape, device=DEV)
+        c["weight"].copy_(old)
+        cache = ops.view(c, weight=c["weight"])
+        capi.paged_attention(cache, cu, q, out, ops.space(), lse=lse, max_tokens=max_tokens)
+        capi.attention_weights(cache, cu, q, lse, decay=decay, max_tokens=max_tokens)
+        torch.cuda.synchronize()
+        assert int(c["status"]) == capi.BAD_PAGE
+        check_weights(c["weight"], want, held, old, decay, 2 * max(new))
+
+
+@pytest.mark.parametrize("max_tokens", [1, 0])
+def test_weights_of_a_nan_row_stay_with_the_slots_it_sees(max_tokens):
+    """A NaN query makes the weights of the slots that its row sees NaN, under its KV head; the new tokens behind it are not among them."""
+    new, row = [150, 90], 20
+    c = ref.make_cache([150, 190], 2, 64, torch.float16, DEV)
+    q = ops.normal(sum(new), 4, 64, dtype=torch.float16, scale=1.5)
+    clean, cu = q.clone(), ref.cu_of(new, DEV)
+    q[row, 1, 5] = math.nan
+    want, held = weights_of(c, new, clean, skip=[(row, 1)])
+    page, place = ref.rows_of(c, 0, row + 1)
+    out, lse, old = torch.zeros_like(q), torch.zeros(sum(new), 4, device=DEV), torch.rand(c["weight"].shape, device=DEV)
+    c["weight"].copy_(old)
+    cache = ops.view(c, weight=c["weight"])
+    capi.paged_attention(cache, cu, q, out, ops.space(), lse=lse, max_tokens=max_tokens)
+    capi.attention_weights(cache, cu, q, lse, decay=0.0, max_tokens=max_tokens)
+    torch.cuda.synchronize()
+    got = c["weight"].clone()
+    assert bool(got[page, 0, place].isnan().all())
+    got[page, 0, place] = want[page, 0, place].float()
+    check_weights(got, want, held, old, 0.0, 2 * max(new))
