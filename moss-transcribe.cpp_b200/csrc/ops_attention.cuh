@@ -451,10 +451,25 @@ struct Walk {
         tile = 0;
         if (++head < a.c.n_kv) return;
         head = 0;
+        // The next sequence that has tiles: a lane a sequence, since thousands without may lie between.
+        const int lane = threadIdx.x & 31;
         while (at < line.hi) {
-            w = seq_work(a, ++seq);
-            tiles = Cut::tiles(w, ge);
-            if (tiles > 0) break;
+            if (++seq >= a.c.n_seq) {  // lengths that changed under the kernel
+                at = line.hi;
+                break;
+            }
+            const SeqWork x = seq + lane < a.c.n_seq ? seq_work(a, seq + lane) : SeqWork{0, 0, 0};
+            const int n = Cut::tiles(x, ge);
+            const unsigned some = __ballot_sync(0xffffffffu, n > 0);
+            if (!some) {
+                seq += 31;
+                continue;
+            }
+            const int from = __ffs(some) - 1;
+            seq += from;
+            w = SeqWork{__shfl_sync(0xffffffffu, x.len, from), __shfl_sync(0xffffffffu, x.tok0, from), __shfl_sync(0xffffffffu, x.n_new, from)};
+            tiles = __shfl_sync(0xffffffffu, n, from);
+            break;
         }
     }
     __device__ bool next(Part* p) {

@@ -58,6 +58,27 @@ def test_sparse_batches_are_joined(n_seq, kv_heads, group, active):
     attend(ref.make_cache([3000, 700], 2, 128, torch.bfloat16, DEV), [200, 100], 4, ws)
 
 
+@pytest.mark.parametrize("new", [1, 40])
+def test_thousands_of_sequences_without_tokens_between_two(new):
+    """The first and the last of 65535 sequences have tokens, and a CTA's interval holds the end of the one and the start of the other."""
+    n_seq = 65535
+    kv, counts = [0] * n_seq, [0] * n_seq
+    kv[0], counts[0], kv[-1], counts[-1] = 70 + new, new, 20000, new
+    c = ref.make_cache([kv[0], kv[-1]], 1, 64, torch.bfloat16, DEV)
+    table = torch.full((n_seq, c["table"].shape[1]), -1, dtype=torch.int32, device=DEV)
+    table[0], table[-1] = c["table"][0], c["table"][1]
+    small = dict(c)
+    c.update(table=table, kv_len=torch.tensor(kv, dtype=torch.int32, device=DEV), kv=kv)
+    ws, q = ops.space(), ops.normal(2 * new, 2, 64, dtype=torch.bfloat16)
+    want, want_lse = torch.zeros_like(q), torch.zeros(2 * new, 2, device=DEV)
+    capi.paged_attention(ops.view(small), ref.cu_of([new, new], DEV), q, want, ops.space(), lse=want_lse)
+    got, lse = attend(c, counts, 2, ws, q=q)[1:]
+    assert int(c["status"]) == 0
+    # The same tokens as a batch of two; cut otherwise, so roundings differ as check_attention allows each.
+    assert (got.float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
+    assert (lse - want_lse).abs().max() <= 2.0 ** -18
+
+
 # ---- weights: rows that see bad pages only, rows that are NaN --------------------------------------------------------
 
 
