@@ -330,8 +330,9 @@ enum {
                            and a sequence that has one is not evicted from */
     MTB_BAD_LEN = 2,    /* kv_len outside [0, 64 table_stride] (clamped to it), or smaller than the new tokens */
     MTB_BAD_TOKENS = 4, /* cu_tokens not ascending inside [0, n_tokens]: the sequence counts as one without tokens */
-    MTB_BAD_WAIT = 8    /* a kernel's wait for its own copies ran out (seconds): that call's results are void, its
-                           workspace must be zeroed again */
+    MTB_BAD_WAIT = 8    /* a wait inside the attention or its weights ran out (two seconds; none lasts longer than a CTA's
+                           share of one tile of rows, which takes that long from some 10^8 slots on): that call's
+                           results are void, its workspace must be zeroed again */
 };
 
 /* A view of one layer's paged cache in the caller's pool: 64 positions per
@@ -416,6 +417,9 @@ int mtb_paged_attention(const mtb_paged_cache* cache, const int32_t* cu_tokens, 
 int mtb_attention_weights(const mtb_paged_cache* cache, const int32_t* cu_tokens, int n_tokens, int max_tokens,
                           const void* q, int64_t q_stride, int n_heads, float scale, const float* lse, float decay,
                           void* stream);
+/* Test hook: the kernels of the next n calls of the two hand out none of their work,
+ * so that their waits run out and MTB_BAD_WAIT is set (0 clears).  Process-wide. */
+void mtb_debug_stall_attention(int n);
 
 /* Device bytes of mtb_cache_evict's workspace (needs no GPU); -2 for sizes that
  * a cache cannot have (n_seq and n_kv_heads at most 65535, their product and table_stride

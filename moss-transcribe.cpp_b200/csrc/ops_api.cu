@@ -4,6 +4,7 @@
 #include "ops.hpp"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <string>
@@ -18,6 +19,8 @@ static_assert(int(MTB_T_F32) == OP_F32 && int(MTB_T_F16) == OP_F16 && int(MTB_T_
 static_assert(int(MTB_BAD_PAGE) == BAD_PAGE && int(MTB_BAD_LEN) == BAD_LEN && int(MTB_BAD_TOKENS) == BAD_TOKENS && int(MTB_BAD_WAIT) == BAD_WAIT,
               "one set of bits");
 static_assert((long long)MTB_ATTENTION_WORKSPACE == kAttnWorkspace, "the header's size is the kernels'");
+
+std::atomic<int> g_stall{0};  // calls that are to stall (mtb_debug_stall_attention)
 
 int fail(int code, const std::string& text) {
     mtb_set_global_error(text.c_str());
@@ -121,6 +124,8 @@ int attention_args(const char* what, const mtb_paged_cache* cache, const int32_t
     a->scale = scale;
     a->G = n_heads / cache->n_kv_heads;
     a->by_G = FastDiv::of(a->G);
+    for (int left = g_stall.load(); left > 0;)
+        if (g_stall.compare_exchange_weak(left, left - 1)) a->c.n_seq = left = 0;
     return 0;
 }
 
@@ -254,6 +259,8 @@ int mtb_attention_weights(const mtb_paged_cache* cache, const int32_t* cu_tokens
         return launched("attention_weights", launch_attention_weights(a, static_cast<cudaStream_t>(stream)));
     });
 }
+
+void mtb_debug_stall_attention(int n) { g_stall.store(n > 0 ? n : 0); }
 
 int64_t mtb_cache_evict_workspace(int n_seq, int n_kv_heads, int table_stride) {
     if (n_seq < 0 || n_seq > 65535 || n_kv_heads < 1 || n_kv_heads > 65535 || int64_t(n_seq) * n_kv_heads > (1 << 24) || table_stride < 1 ||

@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WP>::kThreads, 1)
             }
         }
         p.n = 0;
-        parts.put(turn, p, &s_gave_up);
+        if (a.c.n_seq > 0) parts.put(turn, p, &s_gave_up);
         // No copy is left in flight when the CTA ends: each stage's last fill has landed.
         volatile int none = 0;
         #pragma unroll 1
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 }
             }
             p.n = 0;
-            parts.put(turn, p, &s_gave_up);
+            if (a.c.n_seq > 0) parts.put(turn, p, &s_gave_up);
             #pragma unroll 1
             for (int i = 0; i < kTileEntries; ++i) {  // every copy has landed before the CTA ends
                 const int fills = round + (i < e ? 1 : 0);
@@ -1065,7 +1065,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
             }
         }
         p.n = 0;
-        parts.put(turn, p, &s_gave_up);
+        if (a.c.n_seq > 0) parts.put(turn, p, &s_gave_up);
         volatile int none = 0;
         #pragma unroll 1
         for (int i = 0; i < S::kStages; ++i) {
@@ -1299,7 +1299,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 }
             }
             p.n = 0;
-            parts.put(turn, p, &s_gave_up);
+            if (a.c.n_seq > 0) parts.put(turn, p, &s_gave_up);
             volatile int none = 0;
             #pragma unroll 1
             for (int i = 0; i < kWEntries; ++i) {

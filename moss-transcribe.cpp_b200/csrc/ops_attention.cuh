@@ -34,7 +34,9 @@ __device__ __forceinline__ void bar_arrive(uint64_t* b) {
 __device__ __forceinline__ void bar_expect(uint64_t* b, unsigned bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
 }
-constexpr int kWaitTries = 1 << 21;  // 17 ms at 15 clocks a try; a wait here is for copies, products or warps of the same CTA
+// Waits are for copies, products or warps of the same CTA.  The longest last as long as
+// one CTA's share of a tile (warps that have nothing to do in it): 1.7 us for 128 slots.
+constexpr int kWaitTries = 1 << 19;  // two seconds: a try that fails takes 4 us (measured)
 
 // Waits for a phase; false once the wait ran out or another wait of this CTA
 // did (`gave_up`, shared memory), so that every role leaves its loop.
@@ -500,7 +502,8 @@ struct PartRing {
             bar_init(&taken[i], warps);
         }
     }
-    // The producer warp, the i-th part; false: the wait for room ran out.
+    // The producer warp, the i-th part; false: the wait for room ran out.  Without sequences (calls that
+    // mtb_debug_stall_attention picks; no others are launched) nothing is put, so that the others' waits run out.
     __device__ bool put(unsigned i, const Part& p, volatile int* gave_up) {
         if (i >= kRing && !bar_wait(&taken[i % kRing], (i / kRing - 1) & 1, gave_up)) return false;
         if ((threadIdx.x & 31) == 0) {

@@ -152,6 +152,7 @@ SIGNATURES = {
                                       _vp, _vp, C.c_size_t, _vp]),
     "mtb_attention_weights": (C.c_int, [_vp, _vp, C.c_int, C.c_int, _vp, C.c_int64, C.c_int, C.c_float, _vp, C.c_float,
                                         _vp]),
+    "mtb_debug_stall_attention": (None, [C.c_int]),
     "mtb_cache_evict_workspace": (C.c_int64, [C.c_int, C.c_int, C.c_int]),
     "mtb_cache_evict": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_size_t, _vp]),
     "mtb_logits_process": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int64, _vp, _vp, C.c_int64, _vp, _vp]),

@@ -2,6 +2,7 @@
 rows whose pages are all bad, rows that are NaN, softmax weights far below the largest, waits that run out.  The bounds are
 test_gpu_ops.py's (a rounding to type t is off by at most eps(t) / 2 relative); what a test adds is derived beside it."""
 import math
+import time
 
 import pytest
 
@@ -157,3 +158,32 @@ def test_weights_of_a_nan_row_stay_with_the_slots_it_sees(max_tokens):
     assert bool(got[page, 0, place].isnan().all())
     got[page, 0, place] = want[page, 0, place].float()
     check_weights(got, want, held, old, 0.0, 2 * max(new))
+
+
+# ---- waits that run out ------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("call", ["attention", "weights"])
+@pytest.mark.parametrize("new,max_tokens,n_seq", [(2, 2, 2), (150, 0, 2), (1, 1, 40)])
+def test_a_wait_that_runs_out_is_reported(call, new, max_tokens, n_seq):
+    """A call whose kernel hands out no work ends after two seconds with its bit set; the next one, on a zeroed workspace, is right."""
+    c = ref.make_cache([300] * n_seq, 2, 64, torch.bfloat16, DEV)
+    q, cu, counts = ops.normal(new * n_seq, 4, 64, dtype=torch.bfloat16), ref.cu_of([new] * n_seq, DEV), [new] * n_seq
+    out, lse, ws = torch.zeros_like(q), torch.zeros(new * n_seq, 4, device=DEV), ops.space()
+    cache = ops.view(c, weight=c["weight"])
+    if call == "weights":
+        capi.paged_attention(cache, cu, q, out, ws, lse=lse, max_tokens=max_tokens)
+    torch.cuda.synchronize()
+    capi.lib().mtb_debug_stall_attention(1)
+    start = time.time()
+    if call == "attention":
+        capi.paged_attention(cache, cu, q, out, ws, lse=lse, max_tokens=max_tokens)
+    else:
+        capi.attention_weights(cache, cu, q, lse, decay=0.0, max_tokens=max_tokens)
+    torch.cuda.synchronize()
+    assert 1.0 < time.time() - start < 20.0
+    assert int(c["status"]) == capi.BAD_WAIT
+    c["status"].zero_()
+    ws.zero_()
+    attend(c, counts, 4, ws, q=q, max_tokens=max_tokens)
+    assert int(c["status"]) == 0
