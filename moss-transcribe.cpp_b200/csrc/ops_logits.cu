@@ -4,7 +4,7 @@
 // Bound: bytes (each logit read and written once); one row of 152 k values: latency (7.5 us).
 // 256 f32 rows, half of the ids masked: 55 us without lists (5.7 TB/s, a plain copy 49 us), 85 us
 // with 4096 ids of history and 300 biases a row (3.7 TB/s): a CTA forms its lists before its stream starts.
-// A row belongs to 1 to 16 CTAs, as many as fill the SMs (one from 128 rows on: two
+// A row belongs to 1 to 16 CTAs, as many as fill the SMs (one from 129 rows on: two
 // CTAs to an SM, each a row; clusters of more take longer to place than they save).
 // The vocabulary goes round a row's CTAs in runs of 1024 ids, since histories crowd at
 // low ids.  What touches few ids is set apart: a bitmap in shared memory says which of the
@@ -349,17 +349,8 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(const __grid_const
     unsigned* s_bits = s_table + 2 * kTableSlots;
     __shared__ Best s_best[kLogitsThreads / 32];
     __shared__ Best s_row[16];
-    __shared__ __align__(8) uint64_t s_done;
     const int width = 1 << log_width, row = blockIdx.x >> log_width, part = blockIdx.x & (width - 1);
-    const uint32_t done = (uint32_t)__cvta_generic_to_shared(&s_done);
-    if (width > 1) {
-        if (threadIdx.x == 0) {
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(done), "r"(width) : "memory");
-            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        }
-        __syncwarp();
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for where the choice is joined
-    }
+    if (width > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for where the choice is joined
     const int runs = (a.vocab + kLogitsRun - 1) / kLogitsRun;
     Share sh{row, part, log_width, (runs - part + width - 1) / width * kLogitsRun, 0, 0, 0, 0, nullptr};
     Batch<T, kVec> got;
@@ -378,28 +369,17 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) k_logits(const __grid_const
     if ((threadIdx.x & 31) == 0) s_best[threadIdx.x >> 5] = best;
     __syncthreads();
     if (width > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs have begun
-    if (!a.choice || threadIdx.x >= 32) return;
-    best = warp_best(threadIdx.x < kLogitsThreads / 32 ? s_best[threadIdx.x] : Best{-INFINITY, -1});
+    if (!a.choice) return;
+    if (threadIdx.x < 32) {
+        best = warp_best(threadIdx.x < kLogitsThreads / 32 ? s_best[threadIdx.x] : Best{-INFINITY, -1});
+        // Into the first CTA's memory, which stays until all have come.
+        if (width > 1 && threadIdx.x == 0) *cg::this_cluster().map_shared_rank(&s_row[part], 0) = best;
+        __syncwarp();
+    }
     if (width > 1) {
-        if (threadIdx.x == 0) {
-            // Into the first CTA's memory; it alone stays until all have come.
-            *cg::this_cluster().map_shared_rank(&s_row[part], 0) = best;
-            uint32_t there;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(done));
-            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(there) : "memory");
-        }
-        if (part) return;
-        bool ok = false;
-#pragma unroll 1
-        for (int left = 1 << 22; !ok && left > 0; --left) {
-            uint32_t is;
-            asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0;\n selp.u32 %0, 1, 0, p;\n}\n"
-                         : "=r"(is)
-                         : "r"(done)
-                         : "memory");
-            ok = is;
-        }
-        best = warp_best(ok && (int)threadIdx.x < width ? s_row[threadIdx.x] : Best{-INFINITY, -1});
+        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (part || threadIdx.x >= 32) return;
+        best = warp_best((int)threadIdx.x < width ? s_row[threadIdx.x] : Best{-INFINITY, -1});
     }
     if (threadIdx.x == 0) a.choice[row] = best.i;
 }

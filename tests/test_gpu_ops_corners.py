@@ -187,3 +187,27 @@ def test_a_wait_that_runs_out_is_reported(call, new, max_tokens, n_seq):
     ws.zero_()
     attend(c, counts, 4, ws, q=q, max_tokens=max_tokens)
     assert int(c["status"]) == 0
+
+
+# ---- logits: a row in several CTAs -------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows", [1, 8, 9, 16, 17, 32, 33, 64, 65, 128, 129])
+def test_the_choice_is_found_in_every_share_of_a_row(rows):
+    """Up to 128 rows several CTAs have a row, in runs of 1024 ids: the largest value in each run in turn, equal ones in two runs, none."""
+    vocab = 20 * 1024 + 7
+    runs = -(-vocab // 1024)
+    x = ops.normal(rows, vocab, seed=rows)
+    at = torch.arange(rows, device=DEV)
+    choice = torch.empty(rows, dtype=torch.int32, device=DEV)
+    for run in range(runs):
+        low = torch.clamp(run * 1024 + (at * 37) % 1024, max=vocab - 1)
+        high = torch.clamp(low + 1024, max=vocab - 1)
+        y = x.clone()
+        y[at, low] = 50.0
+        y[at, high] = 50.0
+        y[rows // 2] = -math.inf
+        capi.logits_process(y, None, choice)
+        want = torch.minimum(low, high).to(torch.int32)
+        want[rows // 2] = -1
+        assert torch.equal(choice, want)
