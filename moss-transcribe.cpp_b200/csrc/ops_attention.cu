@@ -1,10 +1,13 @@
 // mtb_paged_attention and mtb_attention_weights.
 //
 // o = sum_j exp(s_j - lse) v_j with s = scale q.k, one pass over the cache: a
-// running maximum m and sum l of exp2(s log2 e - m), the sums of p v rescaled when m
-// has grown by more than 8 (p then stays below 2^8, which 16 bits hold as exactly as
-// values below 1; l and the sums are f32).  p is rounded to the cache's type for
-// the product with v, as the tensor cores want it; l adds it unrounded.
+// running base m and sum l of p = exp2(s log2 e - m), the sums of p v rescaled when the
+// maximum has grown by more than 8 since m was set (l and the sums are f32).  p is
+// rounded to the cache's type for the product with v, as the tensor cores want it; l
+// adds it unrounded.  bf16 holds any p as exactly as 1.  fp16 loses bits below 2^-14
+// and everything below 2^-25, so m lies 7 below the maximum there: p stays below 2^15,
+// and one that is 2^-21 of the largest keeps its bits (a first position that takes
+// nearly all of the weight is no rare sight).
 #include "ops_attention.cuh"
 
 #include <algorithm>
@@ -52,6 +55,10 @@ __device__ __forceinline__ float2 exp2_poly(float2 x0) {
     p.y = x0.y >= -125.f ? p.y : max_nan(x0.y, 0.f);
     return p;
 }
+// How far m lies below the maximum that it was set by.
+template <class T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
+
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -358,12 +365,12 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WP>::kThreads, 1)
                         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
                         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
                     }
-                    // The maximum follows only when it has grown by more than 8.
-                    const bool grown[2] = {top[0] > m[mt][0] + 8.f, top[1] > m[mt][1] + 8.f};
+                    // The base follows only when the maximum has grown by more than 8.
+                    const bool grown[2] = {top[0] > m[mt][0] + (8.f + kLift<T>), top[1] > m[mt][1] + (8.f + kLift<T>)};
                     if (__any_sync(0xffffffffu, grown[0] || grown[1])) {
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const float to = grown[e] ? top[e] : m[mt][e];  // a row goes by its own scores alone
+                            const float to = grown[e] ? top[e] - kLift<T> : m[mt][e];  // a row goes by its own scores alone
                             const float f = to == -INFINITY ? 1.f : exp2_fast(m[mt][e] - to);
                             m[mt][e] = to;
                             l[mt][e] *= f;
@@ -834,9 +841,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], s[124 + j]);
                     top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                     const float reach = top[0] * to_log2;
-                    const bool grown = reach > m + 8.f;
+                    const bool grown = reach > m + (8.f + kLift<T>);
                     if (__any_sync(0xffffffffu, grown)) {
-                        const float to = grown ? reach : m;  // a row goes by its own scores alone
+                        const float to = grown ? reach - kLift<T> : m;  // a row goes by its own scores alone
                         const float f = to == -INFINITY ? 1.f : exp2_fast(m - to);
                         m = to;
                         l *= f;

@@ -7,7 +7,7 @@
 // all (sequence, KV head, tile) stand in one line, each tile behind some units for its own cost, and CTA c of g takes the
 // c-th of g equal intervals of it, whatever the lengths are.  A tile that lies in
 // one interval is finished there.  One that spans several leaves its parts (f32
-// sums, row maxima and row sums) in the workspace, and whichever CTA comes last
+// sums, row bases and row sums) in the workspace, and whichever CTA comes last
 // joins them in the order of the intervals: no order of arrival changes a bit,
 // and no CTA waits for another.
 #pragma once
@@ -527,7 +527,7 @@ struct PartRing {
 
 // Counters (one for each CTA that begins a split tile), then two parts for each
 // CTA: of the tile that reached into its interval, and of the one that begins
-// there.  A part: row maxima (log2), row sums, f32 sums of p v.
+// there.  A part: row bases (log2), row sums, f32 sums of p v.
 constexpr size_t kPartsAt = 8192;
 
 template <int kRows, int kD>
@@ -581,7 +581,7 @@ __device__ __forceinline__ int parts_if_last(const AttnArgs& a, const Part& p) {
 }
 
 // Joins a split tile's parts, by kWarps warps numbered from 0.  First each row's
-// factors, which take the maxima's place: few rows a warp each, a lane a part; many
+// factors, which take the bases' place: few rows a warp each, a lane a part; many
 // rows a thread each.  Then the sums: four columns a thread; the loads wait for
 // nothing, and go out for eight parts (few rows) or eight rows (many) at a time.
 template <class T, int kRows, int kD, int kWarps>

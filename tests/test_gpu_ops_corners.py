@@ -211,3 +211,22 @@ def test_the_choice_is_found_in_every_share_of_a_row(rows):
         want = torch.minimum(low, high).to(torch.int32)
         want[rows // 2] = -1
         assert torch.equal(choice, want)
+
+
+# ---- probabilities far below the largest -----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("new,kv", [(1, 4096), (8, 4096), (40, 4096), (1, 300), (150, 4096)])
+def test_a_first_slot_that_takes_nearly_all(dtype, new, kv):
+    """Slot 0 outweighs any other by e^14.5 and its V is 0, so that the result is made of probabilities of 2^-21: within
+    check_attention's bound, which lets a probability be off by half a step of 16 bits relative to itself."""
+    c = ref.make_cache([kv], 1, 64, dtype, DEV)
+    page, place = ref.rows_of(c, 0, kv)
+    c["k"][page, 0, place] = 0.0
+    c["k"][page[0], 0, 0, 0] = 14.5  # times q's 8 and the scale of 1 / 8: the score
+    c["v"][page[0], 0, 0] = 0.0
+    c["v"][page[1:], 0, place[1:]] += 2.0
+    q = torch.zeros(new, 2, 64, dtype=dtype, device=DEV)
+    q[:, :, 0] = 8.0
+    attend(c, [new], 2, ops.space(), q=q)
