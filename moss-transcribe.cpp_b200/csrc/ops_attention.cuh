@@ -633,7 +633,7 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, const Geometry& ge
         long long token;
         int head;
         if ((!kFew || lane == 0) && a.lse && row_place(ge, p, r, &token, &head))
-            a.lse[token * a.n_heads + head] = sum == 0.f ? -INFINITY : (m + __log2f(sum)) * kLn2;
+            a.lse[token * a.n_heads + head] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
     }
     all.sync();
     constexpr int kCols = kD / 4, kItems = kFew ? 1 : 8, kParts = kFew ? 8 : 1;

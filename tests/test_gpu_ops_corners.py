@@ -230,3 +230,20 @@ def test_a_first_slot_that_takes_nearly_all(dtype, new, kv):
     q = torch.zeros(new, 2, 64, dtype=dtype, device=DEV)
     q[:, :, 0] = 8.0
     attend(c, [new], 2, ops.space(), q=q)
+
+
+@pytest.mark.parametrize("kv", [9001, 20011, 27000])
+def test_log_sums_do_not_depend_on_the_cut(kv):
+    """Scores of 0 once and of -20 log2 units else: log(1 + (kv - 1) 2^-20), where the logarithm of a split tile has to be as exact as
+    that of a whole one.  The terms are off by 2^-19 relative (the scale's product with log2 e, times 20, and the exponential); their
+    sums are multiples of 2^-20 below 2 but for that, so the f32 additions lose nothing; the logarithm and its product: 2^-22 relative."""
+    c = ref.make_cache([kv], 1, 64, torch.bfloat16, DEV)
+    page, place = ref.rows_of(c, 0, kv)
+    c["k"][page, 0, place] = 0.0
+    c["k"][page[1:], 0, place[1:], 0] = -20.0
+    q = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device=DEV)
+    q[:, :, 0] = 1.0
+    lse = torch.zeros(1, 1, device=DEV)
+    capi.paged_attention(ops.view(c), ref.cu_of([1], DEV), q, torch.zeros_like(q), ops.space(), lse=lse, scale=math.log(2.0))
+    tail = (kv - 1) * 2.0 ** -20
+    assert abs(float(lse) - math.log1p(tail)) <= 2.0 ** -19 * tail + 2.0 ** -22 * math.log1p(tail)
