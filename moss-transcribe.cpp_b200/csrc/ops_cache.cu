@@ -65,6 +65,9 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(RopeArgs a, int pe
         }
         s_tok[threadIdx.x] = r;
     }
+    // Bounds that do not ascend are reported for every sequence, also where no token finds it.
+    if (blockIdx.x == 0)
+        for (int s = kRopeThreads - 1 - threadIdx.x; s < c.n_seq; s += kRopeThreads) seq_tokens(c, a.cu, a.n_tokens, s);
     for (int i = threadIdx.x; i < per_cta * half; i += kRopeThreads) {
         const int t = t0 + i / half, j = i % half;
         if (t < a.n_tokens) angle(a, a.positions[t], j, &s_cos[i / half][j], &s_sin[i / half][j]);

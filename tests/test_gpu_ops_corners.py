@@ -247,3 +247,25 @@ def test_log_sums_do_not_depend_on_the_cut(kv):
     capi.paged_attention(ops.view(c), ref.cu_of([1], DEV), q, torch.zeros_like(q), ops.space(), lse=lse, scale=math.log(2.0))
     tail = (kv - 1) * 2.0 ** -20
     assert abs(float(lse) - math.log1p(tail)) <= 2.0 ** -19 * tail + 2.0 ** -22 * math.log1p(tail)
+
+
+# ---- what the append checks -------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("cu,n", [([0, 4, 2, 6, 8], 8), ([0, 3, 3, 9, 2, 6], 6), ([0, 2, 4, 6, 99], 6), ([-1, 2, 4], 4), ([0, 6] + [5] * 300, 6)])
+def test_append_and_attention_report_the_same_bounds_of_tokens(cu, n):
+    """Bounds that do not ascend inside [0, n_tokens] set their bit in the append as in the attention, also where no token is
+    found in the sequence that has them."""
+    n_seq = len(cu) - 1
+    bits = []
+    bounds = torch.tensor(cu, dtype=torch.int32, device=DEV)
+    q = ops.normal(n, 2, 64, dtype=torch.bfloat16)
+    inv = torch.from_numpy(capi.rope_frequencies(64, 1e4)[0]).to(DEV)
+    for call in ("append", "attention"):
+        c = ref.make_cache([70] * n_seq, 2, 64, torch.bfloat16, DEV)
+        if call == "append":
+            capi.rope_append(ops.view(c), bounds, torch.zeros(n, dtype=torch.int32, device=DEV), q, q, q, inv, torch.empty_like(q))
+        else:
+            capi.paged_attention(ops.view(c), bounds, q, torch.empty_like(q), ops.space())
+        bits.append(int(c["status"]))
+    assert bits == [capi.BAD_TOKENS, capi.BAD_TOKENS]
