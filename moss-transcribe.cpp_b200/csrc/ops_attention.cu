@@ -3,8 +3,8 @@
 // o = sum_j exp(s_j - lse) v_j with s = scale q.k, one pass over the cache: a
 // running base m and sum l of p = exp2(s log2 e - m), the sums of p v rescaled when the
 // maximum has grown by more than 8 since m was set (l and the sums are f32).  p is
-// rounded to the cache's type for the product with v, as the tensor cores want it; l
-// adds it unrounded.  bf16 holds any p as exactly as 1.  fp16 loses bits below 2^-14
+// rounded to the cache's type for the product with v, as the tensor cores want it (for
+// at most 16 rows the rest goes into a second product); l adds it unrounded.  bf16 holds any p as exactly as 1.  fp16 loses bits below 2^-14
 // and everything below 2^-25, so m lies 7 below the maximum there: p stays below 2^15,
 // and one that is 2^-21 of the largest keeps its bits (a first position that takes
 // nearly all of the weight is no rare sight).
@@ -72,6 +72,15 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// What pack2 left of the two values, packed in turn.
+__device__ __forceinline__ float2 unpack2(uint32_t x, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
+__device__ __forceinline__ float2 unpack2(uint32_t x, __nv_bfloat16) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
+template <class T>
+__device__ __forceinline__ uint32_t pack2_rest(uint32_t packed, float lo, float hi) {
+    const float2 y = unpack2(packed, T());
+    return pack2<T>(lo - y.x, hi - y.y);
+}
+
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
@@ -118,7 +127,11 @@ bool encode_q(CUtensorMap* map, const AttnArgs& a, int rows) {
 // registers as the second product's operand), so that no page costs a barrier among them;
 // they are joined when the tile's part ends.  16 rows: two such sets of
 // four warps take the pages in turn (a page is a chain of dependent steps, two
-// chains fill each other's gaps).  16 heads of 128 over 8 KV heads: one token over 27000
+// chains fill each other's gaps), and what P's rounding to 16 bits left goes into a
+// second product: results are then as near as f32 probabilities bring them (bf16, one
+// token over 408 slots: 0.0017 relative, the result's own rounding, instead of 0.0028) for 1% of the
+// time of heads of 128 (32 sequences 50.1 -> 50.7 us), 6% of heads of 64 (four tokens of 4 x 9000
+// slots 20.1 -> 21.3); 32 rows would pay a ninth (45 -> 50 us) and go without.  16 heads of 128 over 8 KV heads: one token over 27000
 // slots 25.9 us (4.3 TB/s: the start, the last pages and the join are a third of it), 32 sequences of 2048
 // slots 51 us (5.3 TB/s), eight ragged sequences of 1 .. 8 new tokens 57 us (5.4 TB/s).
 
@@ -159,6 +172,8 @@ struct RowsShape {
     // A stage always falls to the same set of warps: each waits for every fill
     // of its stages, or a barrier's parity would say nothing.
     static constexpr int kStages = (kFit > 12 ? 12 : kFit) / WP * WP;
+    // What P's rounding left goes into a second product, where another set of warps fills its time.
+    static constexpr bool kRest = WP > 1;
     static constexpr int kSmem = 1024 + kStages * kStage + 2 * kQ + kJoin;
 };
 constexpr int kPartRing = 8;
@@ -346,7 +361,7 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WP>::kThreads, 1)
                         mma16<T>(s[mt][1], qf, kf[2], kf[3]);
                     }
                 }
-                uint32_t pa[MW][4];
+                uint32_t pa[MW][4], rest[MW][4];
                 const bool mask = s0 + 16 > least;
 #pragma unroll
                 for (int mt = 0; mt < MW; ++mt) {
@@ -391,6 +406,10 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WP>::kThreads, 1)
                         }
                         pa[mt][2 * n] = pack2<T>(s[mt][n][0], s[mt][n][1]);
                         pa[mt][2 * n + 1] = pack2<T>(s[mt][n][2], s[mt][n][3]);
+                        if constexpr (S::kRest) {
+                            rest[mt][2 * n] = pack2_rest<T>(pa[mt][2 * n], s[mt][n][0], s[mt][n][1]);
+                            rest[mt][2 * n + 1] = pack2_rest<T>(pa[mt][2 * n + 1], s[mt][n][2], s[mt][n][3]);
+                        }
                     }
                 }
                 // V at or behind the sequence's end may hold anything: 0 there, since 0 * NaN is NaN.
@@ -401,22 +420,30 @@ __global__ void __launch_bounds__(RowsShape<kD, MW, WP>::kThreads, 1)
                     lo_on = (first_slot < p.len ? 0xffffu : 0u) | (first_slot + 1 < p.len ? 0xffff0000u : 0u);
                     hi_on = (first_slot + 8 < p.len ? 0xffffu : 0u) | (first_slot + 9 < p.len ? 0xffff0000u : 0u);
                 }
+                // Two 16-dim columns at a time, so that a result's two products have others between them.
 #pragma unroll
-                for (int nd = 0; nd < kD / 16; ++nd) {
-                    uint32_t vf[4];
-                    const int slot = sw * 16 + (lane & 15), ch = nd * 2 + (lane >> 4);
-                    ldsm4t(vf, vb + (ch / 8) * S::kHalf + slot * 128 + (((ch & 7) ^ (slot & 7)) * 16));
-                    if (tail) {
-                        vf[0] &= lo_on;
-                        vf[1] &= hi_on;
-                        vf[2] &= lo_on;
-                        vf[3] &= hi_on;
+                for (int nd = 0; nd < kD / 16; nd += 2) {
+                    uint32_t vf[2][4];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int slot = sw * 16 + (lane & 15), ch = (nd + i) * 2 + (lane >> 4);
+                        ldsm4t(vf[i], vb + (ch / 8) * S::kHalf + slot * 128 + (((ch & 7) ^ (slot & 7)) * 16));
+                        if (tail) {
+                            vf[i][0] &= lo_on;
+                            vf[i][1] &= hi_on;
+                            vf[i][2] &= lo_on;
+                            vf[i][3] &= hi_on;
+                        }
                     }
 #pragma unroll
-                    for (int mt = 0; mt < MW; ++mt) {
-                        mma16<T>(o[mt][2 * nd], pa[mt], vf[0], vf[1]);
-                        mma16<T>(o[mt][2 * nd + 1], pa[mt], vf[2], vf[3]);
-                    }
+                    for (int pass = 0; pass < (S::kRest ? 2 : 1); ++pass)
+#pragma unroll
+                        for (int mt = 0; mt < MW; ++mt)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                mma16<T>(o[mt][2 * (nd + i)], pass ? rest[mt] : pa[mt], vf[i][0], vf[i][1]);
+                                mma16<T>(o[mt][2 * (nd + i) + 1], pass ? rest[mt] : pa[mt], vf[i][2], vf[i][3]);
+                            }
                 }
             }
             __syncwarp();

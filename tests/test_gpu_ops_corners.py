@@ -269,3 +269,27 @@ def test_append_and_attention_report_the_same_bounds_of_tokens(cu, n):
             capi.paged_attention(ops.view(c), bounds, q, torch.empty_like(q), ops.space())
         bits.append(int(c["status"]))
     assert bits == [capi.BAD_TOKENS, capi.BAD_TOKENS]
+
+
+# ---- what P's rounding leaves ------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,kv_heads,group,new,kv", [(128, 8, 2, [1, 1, 1], [40, 300, 129]), (64, 2, 4, [4, 1, 2], [200, 64, 300]),
+                                                       (128, 1, 16, [1], [300]), (64, 1, 1, [16, 3], [150, 33]), (128, 2, 2, [8], [300])])
+def test_steps_hold_probabilities_to_more_than_16_bits(dtype, dim, kv_heads, group, new, kv):
+    """At most 16 rows a KV head: P goes into the product with V with what its rounding left, so it is off by h^2, not by h.
+    The scores are whole numbers times 1/8, exact: e is 2^-22 of the largest (the scale's product with log2 e, and a subtraction);
+    the rest as in test_gpu_ops.py."""
+    c = ref.make_cache(kv, kv_heads, dim, dtype, DEV)
+    g = torch.Generator().manual_seed(dim + group)
+    whole = lambda shape: torch.randint(-2, 3, shape, generator=g).to(dtype).to(DEV)
+    c["k"].copy_(whole(c["k"].shape))
+    q = whole((sum(new), kv_heads * group, dim))
+    out = torch.zeros_like(q)
+    capi.paged_attention(ops.view(c), ref.cu_of(new, DEV), q, out, ops.space(), scale=0.125, max_tokens=max(new))
+    w = ref.attention(c, new, q, 0.125)
+    h, e = ops.half(dtype), 2.0 ** -22 * w["size"][..., None]
+    tol = h * w["out"].abs() + (h * h + 2 * e + 2.0 ** -19 + max(kv) * 2.0 ** -24) * w["spread"]
+    off = (out.double() - w["out"]).abs()
+    assert bool((off <= tol * 1.001 + 2.0 ** -25).all()), float((off / tol).max())  # 2^-25: half a step of fp16's smallest values
