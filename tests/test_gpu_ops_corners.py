@@ -293,3 +293,25 @@ def test_steps_hold_probabilities_to_more_than_16_bits(dtype, dim, kv_heads, gro
     tol = h * w["out"].abs() + (h * h + 2 * e + 2.0 ** -19 + max(kv) * 2.0 ** -24) * w["spread"]
     off = (out.double() - w["out"]).abs()
     assert bool((off <= tol * 1.001 + 2.0 ** -25).all()), float((off / tol).max())  # 2^-25: half a step of fp16's smallest values
+
+
+# ---- eviction by one CTA a list ------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kv,heads,keep,sinks,recent,table_len,shift", [
+    ([0, 1, 63, 64, 65, 100, 514, 1300], 2, 100, 4, 16, None, 1),   # books that are not 16-byte aligned
+    ([700, 2000], 3, 64, 3, 7, None, 3),
+    ([1300, 65], 2, 0, 0, 0, None, 2),
+    ([9000, 300, 64], 2, 200, 4, 64, 1100, 0),                      # a table of more than 65536 slots
+    ([41000, 40960], 1, 8192, 4, 512, 1100, 0),                     # more keys than shared memory holds, and as many
+    ([70001], 1, 30000, 4, 100, None, 0),
+])
+@pytest.mark.parametrize("ties", [False, True])
+def test_evict_by_one_cta_a_list(kv, heads, keep, sinks, recent, table_len, shift, ties):
+    c = ref.make_cache(kv, heads, 64, torch.bfloat16, DEV, table_len=table_len)
+    for name in ("position", "weight"):
+        room = torch.zeros(c[name].numel() + 4, dtype=c[name].dtype, device=DEV)
+        c[name] = room[shift:shift + c[name].numel()].view(c[name].shape)
+    ops.fill_books(c, seed=len(kv), ties=ties)
+    c["weight"][:, :, 5::9] = math.nan
+    ops.run_evict(c, keep, sinks, recent, alias=ties)
