@@ -397,8 +397,8 @@ enum { MTB_ATTENTION_WORKSPACE = 64 << 20 };
  * sequence's n sees the slots <= kv_len - n + i, so its own (appended before).
  * q and out [n_tokens][n_heads][head_dim] of the cache's type (16-byte aligned,
  * strides multiples of 8 elements); n_heads a multiple of n_kv_heads, at most
- * 64 for each; head h reads KV head h / (n_heads / n_kv_heads).  scale times q.k
- * (64-bit host value of the softmax's scale, 1 / sqrt(head_dim) usually).
+ * 64 for each, n_tokens * n_heads / n_kv_heads at most 2^30; head h reads KV head
+ * h / (n_heads / n_kv_heads).  Scores are scale times q.k (1 / sqrt(head_dim) usually).
  * lse [n_tokens][n_heads] f32 (or NULL) gets log sum exp of the row's scores.
  * A row that sees nothing gets out 0 and lse -inf; rows behind the last
  * sequence are left as they are.  Slots a row does not see may hold anything
@@ -411,7 +411,7 @@ int mtb_paged_attention(const mtb_paged_cache* cache, const int32_t* cu_tokens, 
 /* The softmax weight each cached position received in that attention:
  * cache->weight[slot] = decay * cache->weight[slot] + sum of exp(score - lse) over the
  * new tokens that see the slot and the query heads of its KV head (decay 0
- * ignores the old value).  A page whose weights are written belongs to one
+ * ignores the old value; a row whose lse is -inf adds nothing).  A page whose weights are written belongs to one
  * sequence.  Slots at or behind kv_len are left as they are;
  * sequences without new tokens too.  Arguments as above. */
 int mtb_attention_weights(const mtb_paged_cache* cache, const int32_t* cu_tokens, int n_tokens, int max_tokens,

@@ -132,8 +132,8 @@ bool encode_q(CUtensorMap* map, const AttnArgs& a, int rows) {
 // token over 408 slots: 0.0017 relative, the result's own rounding, instead of 0.0028) for 1% of the
 // time of heads of 128 (32 sequences 50.1 -> 50.7 us), 6% of heads of 64 (four tokens of 4 x 9000
 // slots 20.1 -> 21.3); 32 rows would pay a ninth (45 -> 50 us) and go without.  16 heads of 128 over 8 KV heads: one token over 27000
-// slots 25.9 us (4.3 TB/s: the start, the last pages and the join are a third of it), 32 sequences of 2048
-// slots 51 us (5.3 TB/s), eight ragged sequences of 1 .. 8 new tokens 57 us (5.4 TB/s).
+// slots 26.1 us (4.2 TB/s: the start, the last pages and the join are a third of it), 32 sequences of 2048
+// slots 51 us (5.3 TB/s), eight ragged sequences of 1 .. 8 new tokens 57 us (5.3 TB/s).
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -550,9 +550,12 @@ cudaError_t launch_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensor
 // so maxima and sums need no other thread) turn S into P, the tensor cores work for the
 // other.  P takes the place of S.  A half's products run in order, so S of block
 // j + 1 is issued behind P V of block j without a wait, and once S is there O is
-// free to be rescaled.  2048 new tokens over 24576 slots, 16 heads of 128: 313 us,
-// 1.26 PFLOP/s, 75% of what a library product reaches in a burst and 91% of what it holds for
-// seconds; a fresh prompt of 4096 tokens 81 us (0.85 PFLOP/s counting what is
+// free to be rescaled.  P has 16 bits here: its rounding's rest in a second product too (as
+// for few rows) brings bf16 results from 0.0023 .. 0.0020 relative to 0.0017 .. 0.0016, the result's own
+// rounding, and takes 437 us for the chunk below, 87 for prompts of 64 dims (70 without).
+// 2048 new tokens over 24576 slots, 16 heads of 128: 311 us alone,
+// 1.27 PFLOP/s, 76% of what a library product reaches in a burst; for seconds on end 371 us (1.07, 77% of
+// what the product holds for seconds; the power limit has the clock at 1.54 GHz); a fresh prompt of 4096 tokens 81 us (0.85 PFLOP/s counting what is
 // masked as not done).  A steady block takes 3200 clocks for both halves where the products
 // alone take 2048: a half's chain from S over its maximum (450) and exponentials (1540) to P
 // and the next S is as long as that.
@@ -991,7 +994,8 @@ cudaError_t launch_tiles(const AttnArgs& a, const CUtensorMap& km, const CUtenso
 // set of four warps takes a page, 16 slots a warp, two sets in turn; a thread adds its rows' probabilities of
 // its columns, and eight lanes' sums make a slot's.  All rows of a (sequence, KV head)
 // pass over the part's pages 64 at a time, so nothing is joined between CTAs.
-// Eight ragged sequences of 1 .. 8 new tokens, 64 .. 27000 slots: 36 us for 154 MB of K.
+// Eight ragged sequences of 1 .. 8 new tokens, 64 .. 27000 slots: 36 us for 154 MB of K, 68 us with
+// a decay (the old weights are read where the new ones are written, by the warps that hold the page).
 constexpr int kWRows = 64;
 constexpr int kWWarps = 8, kWThreads = (kWWarps + 1) * 32;
 
@@ -1210,8 +1214,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
 // shared memory while the rows that see it stream past, 128 / G whole tokens at a time
 // with their log-sums; S is double-buffered in tensor memory, so the products run
 // ahead.  The exponentials bound it: one for each product of 128 dims.  2048 new
-// tokens over 24576 slots, 16 heads: 256 us (0.77 PFLOP/s); 768 tiles on 148 SMs
-// leave a seventh of that idle.  Tiles of 128 slots whose rows the halves take in turn: a
+// tokens over 24576 slots, 16 heads: 255 .. 300 us by the clock that the power limit leaves
+// (0.77 .. 0.66 PFLOP/s; for seconds on end 274); 768 tiles on 148 SMs leave a seventh of that idle.  Tiles of 128 slots whose rows the halves take in turn: a
 // fresh prompt of 4096 tokens 83 us instead of 115, this chunk 262, 128 rows over 8192 slots 27 instead of 19.
 constexpr int kWTileSlots = 256, kWTileRows = 128;
 constexpr int kWEntries = 2;  // ring of row tiles
@@ -1494,6 +1498,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
+// Up to 64 rows pages stream past the rows, from 65 on rows past the slots.  Measured (16 heads of 128 over 8 KV heads,
+// us here and there): 4 x 8192 slots 32 rows 20.9 and 23.0, 48 rows 25.4 and 23.2, 64 rows 30.0 and 23.1; 16 x 8192
+// 70.6 and 77.2, 88.8 and 76.0, 110 and 76; 16 x 1024 14.6 and 16.3, 17.2 and 15.9, 19.0 and 15.8.  So the two meet
+// near 40 rows; 64 is what a pass of the first kernel holds.
 template <class T, int kD>
 cudaError_t launch_weights(const AttnArgs& a, const CUtensorMap& km, int sms, cudaStream_t s) {
     const long long rows = (long long)a.max_tokens * a.G;
@@ -1514,6 +1522,10 @@ cudaError_t launch_weights(const AttnArgs& a, const CUtensorMap& km, int sms, cu
     return cudaGetLastError();
 }
 
+// One 16-row tile at most, one 32-row tile, or 256-row tiles.  Measured (16 heads of 128 over 8 KV heads, us by each of the
+// three): 4 x 8192 slots 16 rows 33.0, 38.7, 37.7, 32 rows 42.4, 44.8, 39.2, 48 rows 58.2, 67.5, 40.8; 16 x 8192 16 rows
+// 91, 107, 99, 32 rows 169, 120, 103; 4 x 1024 16 rows 18.8, 24.2, 16.9, 32 rows 18.9, 30.0, 17.8.  So the
+// chunks' kernel is ahead of the 32-row tile by an eighth or more there.
 template <class T, int kD>
 cudaError_t launch_by_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int sms, cudaStream_t s) {
     const long long rows = (long long)a.max_tokens * a.G;

@@ -20,7 +20,9 @@ namespace cg = cooperative_groups;
 // f64; its sine and cosine are f32 (the results have 16 bits).  They depend on
 // the token alone, so a CTA forms them once in shared memory for all heads.
 // Bound: bytes (q, k, v read and written once): 9730 f32 tokens of 16 + 2 x 8 heads of 128 into
-// f16 take 45 us (5.3 TB/s); a step's few tokens: latency (3.2 us).
+// f16 take 45 us (5.3 TB/s), bf16 ones into bf16 32 us (5.0 TB/s), with position and weight 32.5; a step's few tokens:
+// latency (3.4 us).  Half pairs of dims that are no multiple of 16, or other alignments, go a pair or a dim a thread
+// with 2-byte accesses: the bf16 tokens take 125 us with 90 dims rotated, 49 with 96.
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeTokens = 4;  // tokens a CTA at most
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(RopeArgs a, int pe
 
 template <class I, class O>
 cudaError_t rope_typed(const RopeArgs& a, cudaStream_t s) {
-    // One token a CTA until the GPU is full: few tokens then spread over more
+    // One token a CTA until the GPU's 148 SMs have two each: few tokens then spread over more
     // SMs; beyond that four share the CTA's start and its angles' threads.
     const int per = a.n_tokens < 2 * 148 ? 1 : kRopeTokens;
     const int in16 = 16 / (int)sizeof(I);
